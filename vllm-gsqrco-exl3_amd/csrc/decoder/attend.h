@@ -1,0 +1,58 @@
+// What the attention kernels over the 8-bit cache share: operand layouts, conversions and the
+// softmax's statistics.
+//
+// Both products are transposed, so that a lane keeps one query row all through:
+//   S^T [tokens x rows] = K [tokens x d] . Q^T [d x rows]        v_mfma_f32_16x16x32_f16
+//   O^T [d x rows]     += V^T [d x tokens] . P^T [tokens x rows]
+// With lane = 16 g + n, an A operand holds row n's values 8g .. 8g + 7 of 32 along the sum, a B
+// operand column n's, and the result's element i is row 4g + i of column n. Which values the 32 places
+// stand for is free as long as both operands agree:
+//   - along d, lane group g takes 16 bytes at 64 s + 16 g of a key: the first eight are its part of
+//     product 2s, the others of 2s + 1;
+//   - a tile is 64 tokens, in chunks of 16 (a chunk never leaves its page). Row 4c + i of the
+//     tile's K operand tt is token 16 c + 4 tt + i, so lane group g receives the scores of chunk g,
+//     tokens 4 tt + i, and these are, in place, the P^T operand for the 16 tokens of V's chunk g, which lie in
+//     one 16-byte piece of a dim's row. Scores never cross lanes.
+#pragma once
+
+#include "dec_common.h"
+
+namespace gguf_dec {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoScore = -1e30f;  // the running maximum before any score
+
+// 4 codes -> 4 fp16, exact: a byte u under 0x64 is fp16 1024 + u
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;  // code + 128
+  const half2v off = {(_Float16)1152.0f, (_Float16)1152.0f};
+  lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
+  hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
+}
+
+__device__ __forceinline__ half8 codes8(uint32_t a, uint32_t b) {
+  uint4 w;
+  codes_to_half(a, w.x, w.y);
+  codes_to_half(b, w.z, w.w);
+  return __builtin_bit_cast(half8, w);
+}
+
+// max over the four lane groups (lanes n, n + 16, n + 32, n + 48)
+__device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+__device__ __forceinline__ float group_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// The power of two that brings a row's largest magnitude into [1, 2), so that bf16 queries of any
+// size fit fp16 exactly (but for values 2^-14 below the row's largest, rounded there); 1 for an all-zero row.
+__device__ __forceinline__ float row_factor(float amax) {
+  const int e = (int)((__float_as_uint(amax) >> 23) & 0xFF);
+  return amax > 0.0f && e >= 1 && e <= 253 ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
+}
+
+}  // namespace gguf_dec

@@ -1,0 +1,601 @@
+// The gated delta rule (include/gguf_decoder.h states the contract). For each v head, with the fp32
+// state S [dv, dk], its decay exp(g) and step beta,
+//   S <- exp(g) S,   u = beta (v - S k),   S <- S + u k^T,   o = scale S q.
+// Sequences of up to kRecurrent tokens take these steps one by one (recurrent_kernel); longer ones
+// take chunks of C tokens (prep_kernel, scan_kernel).
+#include "delta.h"
+
+namespace gguf_dec {
+
+namespace {
+
+__device__ __forceinline__ float row16_sum(float v) {  // over 16 lanes, in all of them
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, true));  // row_ror:8
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x124, 0xF, 0xF, true));
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x122, 0xF, 0xF, true));
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x121, 0xF, 0xF, true));
+  return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, int64_t i, float (&v)[4]) {
+  if constexpr (DT == kF32) {
+    const float4 a = *(const float4*)((const float*)p + i);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+    const uint2 a = *(const uint2*)((const uint16_t*)p + i);
+    const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      v[2 * e] = DT == kF16 ? gguf::half_bits_to_float(w[e] & 0xFFFF) : __uint_as_float(w[e] << 16);
+      v[2 * e + 1] = DT == kF16 ? gguf::half_bits_to_float(w[e] >> 16) : __uint_as_float(w[e] & 0xFFFF0000u);
+    }
+  }
+}
+
+// One wave holds 4 R rows of a head's state in registers: 16 lanes a row, lane sub with the keys
+// 64 c + 4 sub .. + 3. Rows are independent, so nothing leaves the wave. A token's two products with
+// the state, S k and S q, are summed over the 16 lanes together: S' q = S q + u (k . q), so the output need
+// not wait for the update.
+// Bound: HBM, the state in and out (2 x 64 KB a head of 128 x 128); at one sequence latency.
+template <int DT, int DK, int R>
+__global__ void __launch_bounds__(256) recurrent_kernel(DeltaArgs a, int most) {
+  constexpr int P = DK / 64;
+  const int lane = threadIdx.x & 63, sub = lane & 15, rr = lane >> 4;
+  const int seq = blockIdx.z, h = blockIdx.y, hk = h / a.rep;
+  const int row0 = ((int)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 * R;
+  if (row0 >= a.dv) return;
+  int r0, r1;
+  rows_of(a.rows, seq, r0, r1);
+  if (r1 - r0 > most) return;  // the chunked form's
+  const int from = a.slots[seq];
+  const int64_t head = (int64_t)a.dv * DK, slot = (int64_t)a.hv * head;
+  float s[R][P][4];
+  int row[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    row[j] = row0 + 4 * j + rr;
+    const bool have = from >= 0 && from < a.nslots && row[j] < a.dv;
+#pragma unroll
+    for (int c = 0; c < P; ++c) {
+      if (have) {
+        load4<kF32>(a.state, from * slot + h * head + (int64_t)row[j] * DK + 64 * c + 4 * sub, s[j][c]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][c][e] = 0.0f;
+      }
+    }
+  }
+  const auto put = [&](int to) {
+    if (to < 0 || to >= a.nslots) return;
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (row[j] < a.dv)
+#pragma unroll
+        for (int c = 0; c < P; ++c)
+          *(float4*)(a.state + to * slot + h * head + (int64_t)row[j] * DK + 64 * c + 4 * sub) =
+              make_float4(s[j][c][0], s[j][c][1], s[j][c][2], s[j][c][3]);
+  };
+
+  for (int t = r0; t < r1; ++t) {
+    float k[P][4], q[P][4], v[R];
+#pragma unroll
+    for (int c = 0; c < P; ++c) {
+      load4<DT>(a.k, t * a.kt + hk * a.kh + 64 * c + 4 * sub, k[c]);
+      load4<DT>(a.q, t * a.qt + hk * a.qh + 64 * c + 4 * sub, q[c]);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) v[j] = row[j] < a.dv ? load1<DT>(a.v, t * a.vt + h * a.vh + row[j]) : 0.0f;
+    const float eg = expf(a.g[t * a.gt + h]), beta = a.beta[t * a.bt + h];
+    float kk = 0.0f, qq = 0.0f, kq = 0.0f;
+#pragma unroll
+    for (int c = 0; c < P; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        kk = fmaf(k[c][e], k[c][e], kk);
+        qq = fmaf(q[c][e], q[c][e], qq);
+        kq = fmaf(k[c][e], q[c][e], kq);
+      }
+    kq = row16_sum(kq);
+    float rk = 1.0f, rq = a.scale;
+    if (a.l2norm) {
+      rk = 1.0f / sqrtf(row16_sum(kk) + kNormEps);
+      rq = a.scale / sqrtf(row16_sum(qq) + kNormEps);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      float sk = 0.0f, sq = 0.0f;
+#pragma unroll
+      for (int c = 0; c < P; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[j][c][e] *= eg;
+          sk = fmaf(s[j][c][e], k[c][e], sk);
+          sq = fmaf(s[j][c][e], q[c][e], sq);
+        }
+      sk = row16_sum(sk);
+      sq = row16_sum(sq);
+      const float u = beta * (v[j] - rk * sk) * rk;
+      const float o = rq * fmaf(u, kq, sq);
+#pragma unroll
+      for (int c = 0; c < P; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][c][e] = fmaf(u, k[c][e], s[j][c][e]);
+      if (sub == 0 && row[j] < a.dv) gguf::store_y(a.out, ((int64_t)t * a.hv + h) * a.dv + row[j], o, DT);
+    }
+    if (a.steps > 0 && t - r0 < a.steps) put(a.out_slots[(int64_t)seq * a.out_stride + (t - r0)]);
+  }
+  if (a.steps == 0) put(a.out_slots[(int64_t)seq * a.out_stride]);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Chunks. With G_i the sum of g up to token i of the chunk (its last: G_c), u_i = beta_i (v_i -
+// S_i k_i) for the state before token i's update solves (I + L) U = X,
+//   L_ij = beta_i e^{G_i - G_j} k_i.k_j (j < i),   X_i = beta_i (v_i - e^{G_i} S k_i)
+// and with T = (I + L)^-1, U = T X,
+//   o_i = scale (e^{G_i} S q_i + sum_{j <= i} e^{G_i - G_j} (q_i.k_j) u_j),
+//   S  <- e^{G_c} S + sum_j e^{G_c - G_j} u_j k_j^T.
+// T and A_ij = scale e^{G_i - G_j} q_i.k_j need no state: prep_kernel makes them for all chunks at
+// once. scan_kernel goes through a sequence's chunks, with S in registers.
+//
+// Precision: products are bf16 MFMAs with fp32 sums. A bf16 key or query is exact (its norm is
+// applied to the sums), fp16 and fp32 ones are two and three bf16 planes; fp32 values on
+// the way (S, X, U, T) are split into three planes hi + mid + lo, 24 bits, and of the products of planes i and j those
+// with i + j <= 2 are kept: what is dropped is below 2^-24. The output's own products (S q and A U)
+// keep i + j <= 1, below 2^-16, where the output is rounded to 16 bits. Differences of G are taken in 64 bits: G
+// may reach thousands where only differences near 0 matter.
+
+// planes of fp32 values
+__device__ __forceinline__ void split3(float x, __bf16& a, __bf16& b, __bf16& c) {
+  a = (__bf16)x;
+  const float r = x - (float)a;
+  b = (__bf16)r;
+  c = (__bf16)(r - (float)b);
+}
+
+// (chunk slot, v head): one workgroup
+template <int DT, int DK, int C>
+__global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkWs ws) {
+  typedef Layout<DT, DK, C> Lay;
+  constexpr int NK = Lay::NK, CT = C / 16;
+  constexpr int KR = Lay::KR, CR = Lay::CR;
+  extern __shared__ __align__(16) char lds[];
+  __bf16* kp = (__bf16*)lds;                 // [NK][C][KR], then q alike
+  __bf16* qp = kp + NK * C * KR;
+  float* L = (float*)(qp + NK * C * KR);     // [C][C + 4]
+  float* T = L + C * (C + 4);                // [C][C + 4]
+  __shared__ double G[C];
+  __shared__ float beta[C], rk[C], rq[C];
+  constexpr int LS = C + 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int h = blockIdx.y, hk = h / a.rep;
+
+  // the chunk: slot base(s) + c, base(s) = cu[s] / C + s (rows_of's offsets are never negative)
+  int seq, r0, r1, c;
+  {
+    int lo = 0, hi = a.rows.seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      const int b = min(max(a.rows.cu[mid], 0), a.rows.tokens) / C + mid;
+      if (b <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+    }
+    seq = lo;
+    rows_of(a.rows, seq, r0, r1);
+    c = (int)blockIdx.x - (r0 / C + seq);
+  }
+  if (r1 - r0 <= most || c < 0 || c * C >= r1 - r0) return;
+  const int t0 = r0 + c * C, nt = min(C, r1 - t0);
+
+  // keys and queries as planes, with their norms: 256 / C threads a row
+  constexpr int TR = 256 / C, PER = DK / TR / 8;  // threads a row, 8-value pieces a thread
+  {
+    const int i = tid / TR, part = tid % TR;
+    float kk = 0.0f, qq = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const int at = 8 * (part + TR * p);
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (i < nt) {
+          if (x == 0) load8<DT>(a.k, (int64_t)(t0 + i) * a.kt + hk * a.kh + at, v);
+          else load8<DT>(a.q, (int64_t)(t0 + i) * a.qt + hk * a.qh + at, v);
+        }
+        bf16x8 w[3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sum = fmaf(v[e], v[e], sum);
+          __bf16 p0, p1, p2;
+          split3(v[e], p0, p1, p2);
+          w[0][e] = p0; w[1][e] = p1; w[2][e] = p2;
+        }
+#pragma unroll
+        for (int pl = 0; pl < NK; ++pl) *(bf16x8*)((x ? qp : kp) + (pl * C + i) * KR + at) = w[pl];
+      }
+      (x ? qq : kk) = sum;
+    }
+#pragma unroll
+    for (int off = 1; off < TR; off <<= 1) {
+      kk += __shfl_xor(kk, off, 64);
+      qq += __shfl_xor(qq, off, 64);
+    }
+    if (part == 0) {
+      rk[i] = a.l2norm ? 1.0f / sqrtf(kk + kNormEps) : 1.0f;
+      rq[i] = a.l2norm ? a.scale / sqrtf(qq + kNormEps) : a.scale;
+    }
+  }
+  if (wave == 0) {
+    // a decay below e^-1e5 is 0 in fp32; cut there, sums and differences stay finite
+    double s = 0.0;
+    if (lane < nt) {
+      const float gv = a.g[(int64_t)(t0 + lane) * a.gt + h];
+      s = gv < -1e5f ? -1e5 : (double)gv;
+    }
+#pragma unroll
+    for (int off = 1; off < C; off <<= 1) {
+      const double o = __shfl_up(s, off, 64);
+      if (lane >= off) s += o;
+    }
+    if (lane < C) {
+      G[lane] = s;
+      beta[lane] = lane < nt ? a.beta[(int64_t)(t0 + lane) * a.bt + h] : 0.0f;
+    }
+  }
+  __syncthreads();
+
+  char* kq = ws.kq + ((int64_t)blockIdx.x * a.hk + hk) * Lay::kKq;
+  char* tp = ws.t + ((int64_t)blockIdx.x * a.hv + h) * Lay::kT;
+  // factors of a token: beta, of S k in X, of S q in o, of u in S; and the chunk's decay
+  if (tid < C) {
+    float4 f;
+    const float eg = (float)exp(G[tid]);
+    f.x = beta[tid];
+    f.y = beta[tid] * eg * rk[tid];
+    f.z = eg * rq[tid];
+    f.w = (float)exp(G[C - 1] - G[tid]) * rk[tid];
+    ((float4*)(tp + Lay::kFactors))[tid] = f;
+    if (tid == 0) ((float4*)(tp + Lay::kFactors))[C] = make_float4((float)exp(G[C - 1]), 0, 0, 0);
+  }
+  if (h % a.rep == 0) {  // keys, queries and turned keys, once a k head
+    for (int i = tid; i < NK * C * (DK / 8); i += 256) {
+      const int row = i / (DK / 8), at = 8 * (i % (DK / 8));
+      *(bf16x8*)((__bf16*)(kq + Lay::kK) + row * KR + at) = *(const bf16x8*)(kp + row * KR + at);
+      *(bf16x8*)((__bf16*)(kq + Lay::kQ) + row * KR + at) = *(const bf16x8*)(qp + row * KR + at);
+    }
+    for (int i = tid; i < NK * DK * (C / 8); i += 256) {
+      const int d = i % DK, at = 8 * (i / DK % (C / 8)), pl = i / (DK * (C / 8));
+      bf16x8 w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = kp[(pl * C + at + e) * KR + d];
+      *(bf16x8*)((__bf16*)(kq + Lay::kKT) + (pl * DK + d) * CR + at) = w;
+    }
+  }
+
+  // k k^T and q k^T, 16 rows a wave (and turn)
+  __bf16* Ap = (__bf16*)(tp + Lay::kA);
+  for (int it = wave; it < CT; it += 4) {
+    floatx4 kk[CT], qk[CT];
+#pragma unroll
+    for (int jt = 0; jt < CT; ++jt) kk[jt] = qk[jt] = floatx4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < DK / 32; ++s) {
+      bf16x8 ka[NK], qa[NK];
+#pragma unroll
+      for (int p = 0; p < NK; ++p) {
+        ka[p] = *(const bf16x8*)(kp + (p * C + 16 * it + n) * KR + 32 * s + 8 * g);
+        qa[p] = *(const bf16x8*)(qp + (p * C + 16 * it + n) * KR + 32 * s + 8 * g);
+      }
+#pragma unroll
+      for (int jt = 0; jt < CT; ++jt) {
+        if (jt > it) continue;
+#pragma unroll
+        for (int p = 0; p < NK; ++p) {
+          const bf16x8 b = *(const bf16x8*)(kp + (p * C + 16 * jt + n) * KR + 32 * s + 8 * g);
+#pragma unroll
+          for (int o = 0; o + p < 3 && o < NK; ++o) {
+            kk[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[o], b, kk[jt], 0, 0, 0);
+            qk[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qa[o], b, qk[jt], 0, 0, 0);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int jt = 0; jt < CT; ++jt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 16 * it + 4 * g + e, j = 16 * jt + n;
+        const float w = j <= i ? (float)exp(G[i] - G[j]) * rk[j] : 0.0f;
+        L[i * LS + j] = j < i ? beta[i] * rk[i] * w * kk[jt][e] : 0.0f;
+        __bf16 p[3];
+        split3(j <= i ? rq[i] * w * qk[jt][e] : 0.0f, p[0], p[1], p[2]);
+#pragma unroll
+        for (int pl = 0; pl < Lay::NA; ++pl) Ap[(pl * C + i) * CR + j] = p[pl];
+      }
+  }
+  __syncthreads();
+
+  // T: the 16 x 16 blocks on the diagonal by forward substitution, a lane a column
+  if (tid < C) {
+    const int b = 16 * (tid / 16), col = tid % 16;
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = i == col ? 1.0f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) v = fmaf(-L[(b + i) * LS + b + j], t[j], v);
+      t[i] = v;
+      T[(b + i) * LS + b + col] = v;
+    }
+  }
+  __syncthreads();
+  // below it, a wave a column of blocks: T_IJ = -T_II sum_{J <= K < I} L_IK T_KJ, in fp32 MFMAs. Sum place g
+  // of step s stands for 4 g + s, so that a result is the next product's right operand as it is.
+  for (int J = wave; J < CT; J += 4) {
+    floatx4 col[CT];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) col[0][e] = T[(16 * J + 4 * g + e) * LS + 16 * J + n];
+    for (int I = 0; I < J; ++I)  // nothing above
+#pragma unroll
+      for (int e = 0; e < 4; ++e) T[(16 * I + 4 * g + e) * LS + 16 * J + n] = 0.0f;
+#pragma unroll
+    for (int x = 1; x < CT; ++x) {
+      const int I = J + x;
+      if (I >= CT) break;
+      floatx4 m = {0, 0, 0, 0};
+#pragma unroll
+      for (int y = 0; y < x; ++y) {
+        const floatx4 l = *(const floatx4*)(L + (16 * I + n) * LS + 16 * (J + y) + 4 * g);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) m = __builtin_amdgcn_mfma_f32_16x16x4f32(l[s], col[y][s], m, 0, 0, 0);
+      }
+      const floatx4 d = *(const floatx4*)(T + (16 * I + n) * LS + 16 * I + 4 * g);
+      floatx4 r = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) r = __builtin_amdgcn_mfma_f32_16x16x4f32(-d[s], m[s], r, 0, 0, 0);
+      col[x] = r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) T[(16 * I + 4 * g + e) * LS + 16 * J + n] = r[e];
+    }
+  }
+  __syncthreads();
+  __bf16* Tp = (__bf16*)(tp + Lay::kTt);
+  for (int i = tid; i < C * C / 8; i += 256) {
+    const int row = i / (C / 8), at = 8 * (i % (C / 8));
+    bf16x8 w[3];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      __bf16 p0, p1, p2;
+      split3(T[row * LS + at + e], p0, p1, p2);
+      w[0][e] = p0; w[1][e] = p1; w[2][e] = p2;
+    }
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl) *(bf16x8*)(Tp + (pl * C + row) * CR + at) = w[pl];
+  }
+}
+
+// One wave holds 16 columns of a head's S^T [dk x dv] and takes the sequence's chunks in turn; the four waves of
+// a workgroup share what the chunk's products need besides, staged in LDS as prep_kernel left it.
+// With lane = 16 g + n: every product's result has column n = the wave's dv column n, and its tile t's row 4g + e stands for
+// place 32 (t >> 1) + 8 g + 4 (t & 1) + e of its dimension (key or token). So tiles 2s and 2s + 1 of a
+// result hold, in place, the lane's 8 consecutive values of step s of the right operand of the next
+// product: S, X and U go from product to product without leaving their lane's registers; only
+// the left operands' rows are taken in that order.
+template <int DT, int DK, int C>
+__global__ void __launch_bounds__(256, 1) scan_kernel(DeltaArgs a, int most, ChunkWs ws) {
+  typedef Layout<DT, DK, C> Lay;
+  constexpr int NK = Lay::NK, NA = Lay::NA, KR = Lay::KR, CR = Lay::CR;
+  constexpr int TT = C / 16, TS = C / 32, KT = DK / 16, KS = DK / 32;
+  constexpr int MAXO = DT == kF32 ? 2 : 1;  // highest plane sum kept for the output
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int seq = blockIdx.z, h = blockIdx.y, hk = h / a.rep;
+  int r0, r1;
+  rows_of(a.rows, seq, r0, r1);
+  if (r1 - r0 <= most) return;
+  const int dv = ((int)blockIdx.x * 4 + wave) * 16 + n;  // dv % 16 == 0: a wave is in or out as one
+  const bool in = dv < a.dv;
+  const int from = a.slots[seq];
+  const int64_t head = (int64_t)a.dv * DK, slot = (int64_t)a.hv * head;
+  const int64_t at = h * head + (int64_t)dv * DK + 8 * g;
+  floatx4 S[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+    S[t] = in && from >= 0 && from < a.nslots ? *(const floatx4*)(a.state + from * slot + at + 32 * (t >> 1) + 4 * (t & 1))
+                                              : floatx4{0, 0, 0, 0};
+  const auto put = [&](int to) {
+    if (!in || to < 0 || to >= a.nslots) return;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) *(floatx4*)(a.state + to * slot + at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
+  };
+  const int chunks = (r1 - r0 + C - 1) / C, base = r0 / C + seq;
+  const int rown = 8 * (n >> 2) + (n & 3);  // row n of an even tile of a left operand
+
+  for (int c = 0; c < chunks; ++c) {
+    const char* kq = ws.kq + ((int64_t)(base + c) * a.hk + hk) * Lay::kKq;
+    const char* tp = ws.t + ((int64_t)(base + c) * a.hv + h) * Lay::kT;
+    __syncthreads();
+    for (int i = tid; i < Lay::kKq / 16; i += 256) ((uint4*)lds)[i] = ((const uint4*)kq)[i];
+    for (int i = tid; i < Lay::kT / 16; i += 256) ((uint4*)(lds + Lay::kKq))[i] = ((const uint4*)tp)[i];
+    const int t0 = r0 + c * C;
+    float v[TT][4];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = t0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + e;
+        v[t][e] = in && tok < r1 ? load1<DT>(a.v, (int64_t)tok * a.vt + h * a.vh + dv) : 0.0f;
+      }
+    __syncthreads();
+    const __bf16* K = (const __bf16*)(lds + Lay::kK);
+    const __bf16* Q = (const __bf16*)(lds + Lay::kQ);
+    const __bf16* KTr = (const __bf16*)(lds + Lay::kKT);
+    const __bf16* Tm = (const __bf16*)(lds + Lay::kKq + Lay::kTt);
+    const __bf16* Am = (const __bf16*)(lds + Lay::kKq + Lay::kA);
+    const float4* F = (const float4*)(lds + Lay::kKq + Lay::kFactors);
+
+    // S k and S q
+    floatx4 X[TT], O[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) X[t] = O[t] = floatx4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      bf16x8 sp[3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 p0, p1, p2;
+        split3(S[2 * s + (e >> 2)][e & 3], p0, p1, p2);
+        sp[0][e] = p0; sp[1][e] = p1; sp[2][e] = p2;
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+#pragma unroll
+        for (int p = 0; p < NK; ++p) {
+          const bf16x8 k = *(const bf16x8*)(K + (p * C + row) * KR + 32 * s + 8 * g);
+          const bf16x8 q = *(const bf16x8*)(Q + (p * C + row) * KR + 32 * s + 8 * g);
+#pragma unroll
+          for (int o = 0; o + p <= 2; ++o) X[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, sp[o], X[t], 0, 0, 0);
+#pragma unroll
+          for (int o = 0; o + p <= MAXO; ++o) O[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, sp[o], O[t], 0, 0, 0);
+        }
+      }
+    }
+    // X
+    float f2[TT][4];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 f = F[32 * (t >> 1) + 8 * g + 4 * (t & 1) + e];
+        X[t][e] = f.x * v[t][e] - f.y * X[t][e];
+        O[t][e] *= f.z;
+        f2[t][e] = f.w;
+      }
+    // U = T X
+    floatx4 U[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) U[t] = floatx4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < TS; ++s) {
+      bf16x8 xp[3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 p0, p1, p2;
+        split3(X[2 * s + (e >> 2)][e & 3], p0, p1, p2);
+        xp[0][e] = p0; xp[1][e] = p1; xp[2][e] = p2;
+      }
+#pragma unroll
+      for (int t = 2 * s; t < TT; ++t) {  // T is 0 above its diagonal
+        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const bf16x8 m = *(const bf16x8*)(Tm + (p * C + row) * CR + 32 * s + 8 * g);
+#pragma unroll
+          for (int o = 0; o + p <= 2; ++o) U[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, xp[o], U[t], 0, 0, 0);
+        }
+      }
+    }
+    // O += A U;   S = e^{G_c} S + K^T (e^{G_c - G} U)
+    const float dec = F[C].x;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) S[t] *= dec;
+#pragma unroll
+    for (int s = 0; s < TS; ++s) {
+      bf16x8 up[3], wp[3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 p0, p1, p2;
+        split3(U[2 * s + (e >> 2)][e & 3], p0, p1, p2);
+        up[0][e] = p0; up[1][e] = p1; up[2][e] = p2;
+        split3(U[2 * s + (e >> 2)][e & 3] * f2[2 * s + (e >> 2)][e & 3], p0, p1, p2);
+        wp[0][e] = p0; wp[1][e] = p1; wp[2][e] = p2;
+      }
+#pragma unroll
+      for (int t = 2 * s; t < TT; ++t) {
+        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+#pragma unroll
+        for (int p = 0; p < NA; ++p) {
+          const bf16x8 m = *(const bf16x8*)(Am + (p * C + row) * CR + 32 * s + 8 * g);
+#pragma unroll
+          for (int o = 0; o + p <= MAXO; ++o) O[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, up[o], O[t], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+#pragma unroll
+        for (int p = 0; p < NK; ++p) {
+          const bf16x8 m = *(const bf16x8*)(KTr + (p * DK + row) * CR + 32 * s + 8 * g);
+#pragma unroll
+          for (int o = 0; o + p <= 2; ++o) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, wp[o], S[t], 0, 0, 0);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = t0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + e;
+        if (in && tok < r1) gguf::store_y(a.out, ((int64_t)tok * a.hv + h) * a.dv + dv, O[t][e], DT);
+      }
+  }
+  put(a.out_slots[(int64_t)seq * a.out_stride]);
+}
+
+template <int DT, int DK>
+hipError_t launch(const DeltaArgs& a, int64_t max_new, void* wsp, hipStream_t stream) {
+  const bool chunked = wsp != nullptr;
+  const int most = chunked ? kRecurrent : 0x7FFFFFFF;
+  constexpr int R = 4;
+  recurrent_kernel<DT, DK, R><<<dim3((a.dv + 16 * R - 1) / (16 * R), a.hv, a.rows.seqs), 256, 0, stream>>>(a, most);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !chunked) return e;
+  constexpr int C = Chunk<DT>::C;
+  typedef Layout<DT, DK, C> Lay;
+  const int64_t slots = a.rows.tokens / C + a.rows.seqs;
+  ChunkWs ws{(char*)wsp, (char*)wsp + slots * a.hk * Lay::kKq};
+  constexpr int prep_lds = Lay::NK * C * Lay::KR * 4 + 2 * C * (C + 4) * 4, scan_lds = Lay::kKq + Lay::kT;
+  int dev = 0;
+  if ((e = hipGetDevice(&dev)) != hipSuccess) return e;
+  struct Tag {};
+  gguf::once_per_device<Tag>(dev, [&] {
+    (void)hipFuncSetAttribute((const void*)prep_kernel<DT, DK, C>, hipFuncAttributeMaxDynamicSharedMemorySize, prep_lds);
+    (void)hipFuncSetAttribute((const void*)scan_kernel<DT, DK, C>, hipFuncAttributeMaxDynamicSharedMemorySize, scan_lds);
+  });
+  prep_kernel<DT, DK, C><<<dim3((unsigned)slots, a.hv), 256, prep_lds, stream>>>(a, most, ws);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  scan_kernel<DT, DK, C><<<dim3((a.dv + 63) / 64, a.hv, a.rows.seqs), 256, scan_lds, stream>>>(a, most, ws);
+  return hipGetLastError();
+}
+
+template <int DT>
+size_t ws_bytes(int dk, int hk, int hv, int64_t tokens, int64_t seqs) {
+  constexpr int C = Chunk<DT>::C;
+  const int64_t slots = tokens / C + seqs;
+  const size_t kq = dk == 64 ? Layout<DT, 64, C>::kKq : Layout<DT, 128, C>::kKq;
+  const size_t t = dk == 64 ? Layout<DT, 64, C>::kT : Layout<DT, 128, C>::kT;
+  return slots * (hk * kq + hv * t);
+}
+
+}  // namespace
+
+size_t delta_workspace(int dtype, int dk, int hk, int hv, int64_t tokens, int64_t seqs, int64_t max_new, bool steps) {
+  if (steps || max_new <= kRecurrent) return 0;
+  return dtype == kF32   ? ws_bytes<kF32>(dk, hk, hv, tokens, seqs)
+         : dtype == kF16 ? ws_bytes<kF16>(dk, hk, hv, tokens, seqs)
+                         : ws_bytes<kBF16>(dk, hk, hv, tokens, seqs);
+}
+
+// ws: of delta_workspace's bytes, or null: every sequence in the recurrent form
+hipError_t launch_delta(const DeltaArgs& a, int dtype, int dk, int64_t max_new, void* ws, hipStream_t stream) {
+#define GGUF_DEC_DELTA(DT) return dk == 64 ? launch<DT, 64>(a, max_new, ws, stream) : launch<DT, 128>(a, max_new, ws, stream)
+  switch (dtype) {
+    case kF32: GGUF_DEC_DELTA(kF32);
+    case kF16: GGUF_DEC_DELTA(kF16);
+    default: GGUF_DEC_DELTA(kBF16);
+  }
+#undef GGUF_DEC_DELTA
+}
+
+}  // namespace gguf_dec
