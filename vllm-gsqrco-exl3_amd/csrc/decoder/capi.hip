@@ -89,7 +89,7 @@ int64_t stride_of(const gguf_tensor* t, int i) {
 bool shaped(const gguf_tensor* t, int ndim) {
   if (!t || t->ndim != ndim) return false;
   for (int i = 0; i < ndim; ++i)
-    if (t->size[i] < 0 || t->size[i] > INT_MAX || t->stride[i] < 0) return false;
+    if (t->size[i] < 0 || t->size[i] > INT_MAX || t->stride[i] < 0 || (t->ndim == 3 && i < 2 && t->size[i] > 1 && t->stride[i] > INT_MAX)) return false;
   return true;
 }
 

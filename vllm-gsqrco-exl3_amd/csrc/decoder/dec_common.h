@@ -17,6 +17,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef short short8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 // The paged 8-bit KV cache as the kernels take it.
 struct Kv8 {
@@ -68,7 +69,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (DT == kF16) {
     return (uint32_t)__half_as_ushort(__float2half_rn(a)) | (uint32_t)__half_as_ushort(__float2half_rn(b)) << 16;
   } else {
-    return (uint32_t)gguf::f32_to_bf16_bits(a) | (uint32_t)gguf::f32_to_bf16_bits(b) << 16;
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {(__bf16)a, (__bf16)b};  // one v_cvt_pk_bf16_f32, to nearest even
+    return __builtin_bit_cast(uint32_t, v);
   }
 }
 
@@ -91,6 +94,13 @@ __device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) 
     *(uint4*)((uint16_t*)p + i) =
         make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7]));
   }
+}
+
+template <int DT>
+__device__ __forceinline__ void store1(void* p, int64_t i, float v) {
+  if constexpr (DT == kF32) ((float*)p)[i] = v;
+  else if constexpr (DT == kF16) ((_Float16*)p)[i] = (_Float16)v;
+  else ((__bf16*)p)[i] = (__bf16)v;
 }
 
 template <int DT>

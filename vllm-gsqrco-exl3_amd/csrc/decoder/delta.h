@@ -42,13 +42,29 @@ struct Chunk {
 template <int DT, int DK, int C>
 struct Layout {
   static constexpr int NK = DT == kBF16 ? 1 : DT == kF16 ? 2 : 3;  // planes of a key or query
-  static constexpr int NA = DT == kF32 ? 3 : 2;                    // planes of A
-  static constexpr int KR = DK + 8, CR = C + 8;                    // row lengths
-  // bytes: keys [NK][C][KR], queries alike, keys turned [NK][DK][CR]
-  static constexpr int kK = 0, kQ = NK * C * KR * 2, kKT = 2 * kQ, kKq = kKT + NK * DK * CR * 2;
-  // T [3][C][CR], A [NA][C][CR], factors float4 [C + 1]
-  static constexpr int kTt = 0, kA = 3 * C * CR * 2, kFactors = kA + NA * C * CR * 2, kT = kFactors + (C + 1) * 16;
-  static_assert(kKq % 16 == 0 && kT % 16 == 0 && kKq + kT <= 160 * 1024, "LDS");
+  static constexpr int NA = DT == kF32 ? 3 : 2;                    // planes of A that the output takes
+  static constexpr int KR = DK + 8;                                // row length of keys and queries
+  // bytes: keys [NK][C][KR], queries alike; whole KB
+  static constexpr int kK = 0, kQ = NK * C * KR * 2, kKq = (2 * kQ + 1023) / 1024 * 1024;
+  // T and A in fp32, by steps of 32 columns, of which step s has the rows from 32 s on (above they are 0):
+  // row i, column j lies at kTt + 4 tri(i, j)
+  static constexpr int RS = 36;
+  static constexpr __host__ __device__ int tri(int i, int j) {
+    const int s = j / 32;
+    return (s * C - 16 * s * (s - 1) + i - 32 * s) * RS + j % 32;
+  }
+  static constexpr int kTri = (tri(C - 1, C - 1) + 1 + 4) / 4 * 4 * 4;
+  // T, A, factors float4 [C + 1]; whole KB, shared out evenly with the above over the scan's waves, which copy
+  // 1 KB at a time
+  static constexpr int kTt = 0, kA = kTri, kFactors = 2 * kTri;
+  static constexpr int ND = DT == kF16 ? 4 : 2;     // groups of 16 values of a head that a workgroup of the scan takes
+  static constexpr int WAVES = C / 16 * ND, kPart = WAVES * 1024;
+  static constexpr int kT = (kKq + kFactors + (C + 1) * 16 + kPart - 1) / kPart * kPart - kKq;
+  // behind them in LDS: the planes of S, X and U as right operands, 1 KB for 32 places of the sum
+  static constexpr int NU = DT == kF32 ? 6 : 5;     // U's planes: three for S, the others for the output
+  static constexpr int kS = kKq + kT, kX = kS + ND * 3 * (DK / 32) * 1024, kU = kX + ND * 3 * (C / 32) * 1024;
+  static constexpr int kLds = kU + ND * NU * (C / 32) * 1024;
+  static_assert(kLds <= 160 * 1024, "LDS");
 };
 
 }  // namespace gguf_dec

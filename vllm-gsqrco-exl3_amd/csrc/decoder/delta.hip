@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256) recurrent_kernel(DeltaArgs a, int most) {
       load4<DT>(a.q, t * a.qt + hk * a.qh + 64 * c + 4 * sub, q[c]);
     }
 #pragma unroll
-    for (int j = 0; j < R; ++j) v[j] = row[j] < a.dv ? load1<DT>(a.v, t * a.vt + h * a.vh + row[j]) : 0.0f;
+    for (int j = 0; j < R; ++j) v[j] = load1<DT>(a.v, t * a.vt + h * a.vh + min(row[j], a.dv - 1));
     const float eg = expf(a.g[t * a.gt + h]), beta = a.beta[t * a.bt + h];
     float kk = 0.0f, qq = 0.0f, kq = 0.0f;
 #pragma unroll
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256) recurrent_kernel(DeltaArgs a, int most) {
       for (int c = 0; c < P; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][c][e] = fmaf(u, k[c][e], s[j][c][e]);
-      if (sub == 0 && row[j] < a.dv) gguf::store_y(a.out, ((int64_t)t * a.hv + h) * a.dv + row[j], o, DT);
+      if (sub == 0 && row[j] < a.dv) store1<DT>(a.out, ((int64_t)t * a.hv + h) * a.dv + row[j], o);
     }
     if (a.steps > 0 && t - r0 < a.steps) put(a.out_slots[(int64_t)seq * a.out_stride + (t - r0)]);
   }
@@ -145,12 +145,95 @@ __global__ void __launch_bounds__(256) recurrent_kernel(DeltaArgs a, int most) {
 // keep i + j <= 1, below 2^-16, where the output is rounded to 16 bits. Differences of G are taken in 64 bits: G
 // may reach thousands where only differences near 0 matter.
 
-// planes of fp32 values
-__device__ __forceinline__ void split3(float x, __bf16& a, __bf16& b, __bf16& c) {
-  a = (__bf16)x;
-  const float r = x - (float)a;
-  b = (__bf16)r;
-  c = (__bf16)(r - (float)b);
+// P planes of 8 fp32 values, two a conversion
+template <int P>
+__device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&planes)[P]) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bf16x2 v = {(__bf16)r[2 * e], (__bf16)r[2 * e + 1]};
+      w[e] = __builtin_bit_cast(uint32_t, v);
+      if (p + 1 < P) {
+        r[2 * e] -= __uint_as_float(w[e] << 16);
+        r[2 * e + 1] -= __uint_as_float(w[e] & 0xFFFF0000u);
+      }
+    }
+    planes[p] = __builtin_bit_cast(bf16x8, uintx4{w[0], w[1], w[2], w[3]});
+  }
+}
+
+// an element's bits, their value, and access through a buffer descriptor
+template <int DT>
+struct Bits {
+  typedef uint16_t type;
+  static __device__ __forceinline__ float value(uint16_t b) {
+    return DT == kF16 ? gguf::half_bits_to_float(b) : __uint_as_float((uint32_t)b << 16);
+  }
+  static __device__ __forceinline__ uint16_t load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+  }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t at, float v) {
+    const uint16_t b = DT == kF16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : __builtin_bit_cast(uint16_t, (__bf16)v);
+    __builtin_amdgcn_raw_buffer_store_b16(b, r, at, 0, 0);
+  }
+};
+template <>
+struct Bits<kF32> {
+  typedef float type;
+  static __device__ __forceinline__ float value(float b) { return b; }
+  static __device__ __forceinline__ float load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
+  }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t at, float v) {
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, at, 0, 0);
+  }
+};
+
+struct Lane8 {
+  float x[8];
+};
+
+__device__ __forceinline__ Lane8 lane8(floatx4 a, floatx4 b) {
+  return Lane8{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+}
+
+template <int P>
+__device__ __forceinline__ void split(const Lane8& x, bf16x8 (&planes)[P]) {
+  split(x.x, planes);
+}
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ short4v turned(const __bf16* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p);
+}
+
+__device__ __forceinline__ bf16x8 join(short4v a, short4v b) {
+  return __builtin_bit_cast(bf16x8, short8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+}
+
+// P planes of 4 fp32 values
+template <int P>
+__device__ __forceinline__ void split4(const floatx4& x, uint2 (&planes)[P]) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  floatx4 r = x;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const bf16x2 a = {(__bf16)r[0], (__bf16)r[1]}, b = {(__bf16)r[2], (__bf16)r[3]};
+    planes[p] = make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+    if (p + 1 < P) {
+      r[0] -= __uint_as_float(planes[p].x << 16);
+      r[1] -= __uint_as_float(planes[p].x & 0xFFFF0000u);
+      r[2] -= __uint_as_float(planes[p].y << 16);
+      r[3] -= __uint_as_float(planes[p].y & 0xFFFF0000u);
+    }
+  }
 }
 
 // (chunk slot, v head): one workgroup
@@ -158,7 +241,7 @@ template <int DT, int DK, int C>
 __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkWs ws) {
   typedef Layout<DT, DK, C> Lay;
   constexpr int NK = Lay::NK, CT = C / 16;
-  constexpr int KR = Lay::KR, CR = Lay::CR;
+  constexpr int KR = Lay::KR;
   extern __shared__ __align__(16) char lds[];
   __bf16* kp = (__bf16*)lds;                 // [NK][C][KR], then q alike
   __bf16* qp = kp + NK * C * KR;
@@ -202,14 +285,10 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
           if (x == 0) load8<DT>(a.k, (int64_t)(t0 + i) * a.kt + hk * a.kh + at, v);
           else load8<DT>(a.q, (int64_t)(t0 + i) * a.qt + hk * a.qh + at, v);
         }
-        bf16x8 w[3];
+        bf16x8 w[NK];
+        split(v, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sum = fmaf(v[e], v[e], sum);
-          __bf16 p0, p1, p2;
-          split3(v[e], p0, p1, p2);
-          w[0][e] = p0; w[1][e] = p1; w[2][e] = p2;
-        }
+        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
 #pragma unroll
         for (int pl = 0; pl < NK; ++pl) *(bf16x8*)((x ? qp : kp) + (pl * C + i) * KR + at) = w[pl];
       }
@@ -249,31 +328,24 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
   // factors of a token: beta, of S k in X, of S q in o, of u in S; and the chunk's decay
   if (tid < C) {
     float4 f;
-    const float eg = (float)exp(G[tid]);
+    const float eg = expf((float)G[tid]);
     f.x = beta[tid];
     f.y = beta[tid] * eg * rk[tid];
     f.z = eg * rq[tid];
-    f.w = (float)exp(G[C - 1] - G[tid]) * rk[tid];
+    f.w = expf((float)(G[C - 1] - G[tid])) * rk[tid];
     ((float4*)(tp + Lay::kFactors))[tid] = f;
-    if (tid == 0) ((float4*)(tp + Lay::kFactors))[C] = make_float4((float)exp(G[C - 1]), 0, 0, 0);
+    if (tid == 0) ((float4*)(tp + Lay::kFactors))[C] = make_float4(expf((float)G[C - 1]), 0, 0, 0);
   }
-  if (h % a.rep == 0) {  // keys, queries and turned keys, once a k head
+  if (h % a.rep == 0) {  // keys and queries, once a k head
     for (int i = tid; i < NK * C * (DK / 8); i += 256) {
       const int row = i / (DK / 8), at = 8 * (i % (DK / 8));
       *(bf16x8*)((__bf16*)(kq + Lay::kK) + row * KR + at) = *(const bf16x8*)(kp + row * KR + at);
       *(bf16x8*)((__bf16*)(kq + Lay::kQ) + row * KR + at) = *(const bf16x8*)(qp + row * KR + at);
     }
-    for (int i = tid; i < NK * DK * (C / 8); i += 256) {
-      const int d = i % DK, at = 8 * (i / DK % (C / 8)), pl = i / (DK * (C / 8));
-      bf16x8 w;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = kp[(pl * C + at + e) * KR + d];
-      *(bf16x8*)((__bf16*)(kq + Lay::kKT) + (pl * DK + d) * CR + at) = w;
-    }
   }
 
   // k k^T and q k^T, 16 rows a wave (and turn)
-  __bf16* Ap = (__bf16*)(tp + Lay::kA);
+  float* Ap = (float*)(tp + Lay::kA);
   for (int it = wave; it < CT; it += 4) {
     floatx4 kk[CT], qk[CT];
 #pragma unroll
@@ -305,12 +377,9 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 16 * it + 4 * g + e, j = 16 * jt + n;
-        const float w = j <= i ? (float)exp(G[i] - G[j]) * rk[j] : 0.0f;
+        const float w = j <= i ? expf((float)(G[i] - G[j])) * rk[j] : 0.0f;
         L[i * LS + j] = j < i ? beta[i] * rk[i] * w * kk[jt][e] : 0.0f;
-        __bf16 p[3];
-        split3(j <= i ? rq[i] * w * qk[jt][e] : 0.0f, p[0], p[1], p[2]);
-#pragma unroll
-        for (int pl = 0; pl < Lay::NA; ++pl) Ap[(pl * C + i) * CR + j] = p[pl];
+        if (j / 32 <= i / 32) Ap[Lay::tri(i, j)] = j <= i ? rq[i] * w * qk[jt][e] : 0.0f;
       }
   }
   __syncthreads();
@@ -359,188 +428,217 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
     }
   }
   __syncthreads();
-  __bf16* Tp = (__bf16*)(tp + Lay::kTt);
-  for (int i = tid; i < C * C / 8; i += 256) {
-    const int row = i / (C / 8), at = 8 * (i % (C / 8));
-    bf16x8 w[3];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      __bf16 p0, p1, p2;
-      split3(T[row * LS + at + e], p0, p1, p2);
-      w[0][e] = p0; w[1][e] = p1; w[2][e] = p2;
-    }
-#pragma unroll
-    for (int pl = 0; pl < 3; ++pl) *(bf16x8*)(Tp + (pl * C + row) * CR + at) = w[pl];
+  float* Tp = (float*)(tp + Lay::kTt);
+  for (int i = tid; i < C * C / 4; i += 256) {
+    const int row = i / (C / 4), at = 4 * (i % (C / 4));
+    if (at / 32 <= row / 32) *(floatx4*)(Tp + Lay::tri(row, at)) = *(const floatx4*)(T + row * LS + at);
   }
 }
 
-// One wave holds 16 columns of a head's S^T [dk x dv] and takes the sequence's chunks in turn; the four waves of
-// a workgroup share what the chunk's products need besides, staged in LDS as prep_kernel left it.
-// With lane = 16 g + n: every product's result has column n = the wave's dv column n, and its tile t's row 4g + e stands for
-// place 32 (t >> 1) + 8 g + 4 (t & 1) + e of its dimension (key or token). So tiles 2s and 2s + 1 of a
-// result hold, in place, the lane's 8 consecutive values of step s of the right operand of the next
-// product: S, X and U go from product to product without leaving their lane's registers; only
-// the left operands' rows are taken in that order.
+// A workgroup takes 16 ND columns (values) of a head through the sequence's chunks in turn. Wave (wt, wd) has of
+// its 16 columns wd: the wt-th 16 tokens of X, U and the output, and the wt-th part of S's rows (keys).
+// The chunk's left operands lie in LDS as prep_kernel left them. S, X and U become right operands: each wave splits
+// its own part into planes, and all read them from LDS; three barriers a chunk.
+//
+// With lane = 16 g + n, a result has column n = value n, and row 4g + e of its tile t stands for place
+// 32 (t >> 1) + 8 g + 4 (t & 1) + e of its dimension (keys or tokens): tiles 2s and 2s + 1 hold, in place, the lane's
+// 8 consecutive values of step s of a right operand, so planes are written as they are read, 16
+// bytes a lane; only the left operands' rows are taken in that order.
+//
+// Bound: for one sequence of 48 heads, the latency of the chain S k -> X -> U -> S through a chunk.
 template <int DT, int DK, int C>
-__global__ void __launch_bounds__(256, 1) scan_kernel(DeltaArgs a, int most, ChunkWs ws) {
+__global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kernel(DeltaArgs a, int most, ChunkWs ws) {
   typedef Layout<DT, DK, C> Lay;
-  constexpr int NK = Lay::NK, NA = Lay::NA, KR = Lay::KR, CR = Lay::CR;
-  constexpr int TT = C / 16, TS = C / 32, KT = DK / 16, KS = DK / 32;
+  constexpr int NK = Lay::NK, NA = Lay::NA, KR = Lay::KR, WAVES = Lay::WAVES;
+  constexpr int TT = C / 16, TS = C / 32, KT = DK / 16, KS = DK / 32, KW = KT / TT;
   constexpr int MAXO = DT == kF32 ? 2 : 1;  // highest plane sum kept for the output
   extern __shared__ __align__(16) char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const int seq = blockIdx.z, h = blockIdx.y, hk = h / a.rep;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
+  const int wt = wave % TT, wd = wave / TT;
+  const int seq = blockIdx.z, h = blockIdx.x, hk = h / a.rep;
   int r0, r1;
   rows_of(a.rows, seq, r0, r1);
   if (r1 - r0 <= most) return;
-  const int dv = ((int)blockIdx.x * 4 + wave) * 16 + n;  // dv % 16 == 0: a wave is in or out as one
+  const int dv = ((int)blockIdx.y * Lay::ND + wd) * 16 + n;  // dv % 16 == 0: a wave is in or out as one
   const bool in = dv < a.dv;
   const int from = a.slots[seq];
   const int64_t head = (int64_t)a.dv * DK, slot = (int64_t)a.hv * head;
   const int64_t at = h * head + (int64_t)dv * DK + 8 * g;
-  floatx4 S[KT];
+  const auto key = [&](int t) { return 32 * ((wt * KW + t) >> 1) + 4 * ((wt * KW + t) & 1); };  // of the wave's tile t, less 8 g
+  floatx4 S[KW];
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
-    S[t] = in && from >= 0 && from < a.nslots ? *(const floatx4*)(a.state + from * slot + at + 32 * (t >> 1) + 4 * (t & 1))
-                                              : floatx4{0, 0, 0, 0};
-  const auto put = [&](int to) {
-    if (!in || to < 0 || to >= a.nslots) return;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) *(floatx4*)(a.state + to * slot + at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
-  };
+  for (int t = 0; t < KW; ++t)
+    S[t] = in && from >= 0 && from < a.nslots ? *(const floatx4*)(a.state + from * slot + at + key(t)) : floatx4{0, 0, 0, 0};
   const int chunks = (r1 - r0 + C - 1) / C, base = r0 / C + seq;
   const int rown = 8 * (n >> 2) + (n & 3);  // row n of an even tile of a left operand
+  const int tok0 = 32 * (wt >> 1) + 4 * (wt & 1);  // the wave's tokens are tok0 + 8 g + e
+
+  // v and out through buffer descriptors over the chunk's rows: a lane without a token (or column) reads 0 and its
+  // stores are dropped, without branches, across which the compiler would wait for every load and store in flight
+  constexpr uint32_t ES = DT == kF32 ? 4 : 2, kNowhere = 0x7FFFFF00u;
+  const uint32_t vt = (uint32_t)a.vt * ES, ot = (uint32_t)(a.hv * a.dv) * ES;
+  const auto place = [&](int e, int nt, uint32_t stride) __attribute__((always_inline)) {
+    const int i = tok0 + 8 * g + e;
+    return in && i < nt ? (uint32_t)i * stride + (uint32_t)dv * ES : kNowhere;
+  };
+  // The next chunk's operands go to LDS, and its v to registers, during this one's last products: by then
+  // this one's are in registers.
+  typename Bits<DT>::type vnext[4];  // as they are: converting them here would wait for them here
+  const auto fetch = [&](int c) __attribute__((always_inline)) {
+    const char* kq = ws.kq + ((int64_t)(base + c) * a.hk + hk) * Lay::kKq;
+    const char* tp = ws.t + ((int64_t)(base + c) * a.hv + h) * Lay::kT - Lay::kKq;
+#pragma unroll
+    for (int i = 0; i < (Lay::kKq + Lay::kT) / Lay::kPart; ++i) {
+      const int o = (WAVES * i + wave) * 1024;
+      __builtin_amdgcn_global_load_lds((const void*)((o < Lay::kKq ? kq : tp) + o + 16 * lane),
+                                       (__attribute__((address_space(3))) void*)(lds + o), 16, 0, 0);
+    }
+    const int nt = min(C, r1 - r0 - c * C);
+    const __amdgpu_buffer_rsrc_t rs = gguf::buffer_rsrc((const char*)a.v + ((int64_t)(r0 + c * C) * a.vt + h * a.vh) * ES, (C - 1) * vt + a.dv * ES);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vnext[e] = Bits<DT>::load(rs, place(e, nt, vt));
+  };
+  const __bf16* K = (const __bf16*)(lds + Lay::kK);
+  const __bf16* Q = (const __bf16*)(lds + Lay::kQ);
+  const float* Tm = (const float*)(lds + Lay::kKq + Lay::kTt);
+  const float* Am = (const float*)(lds + Lay::kKq + Lay::kA);
+  const float4* F = (const float4*)(lds + Lay::kKq + Lay::kFactors);
+  // plane p, step s of the wave's columns
+  char* const sl = lds + Lay::kS + wd * 3 * KS * 1024 + 16 * lane;
+  char* const xl = lds + Lay::kX + wd * 3 * TS * 1024 + 16 * lane;
+  char* const ul = lds + Lay::kU + wd * Lay::NU * TS * 1024 + 16 * lane;
+
+  fetch(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
   for (int c = 0; c < chunks; ++c) {
-    const char* kq = ws.kq + ((int64_t)(base + c) * a.hk + hk) * Lay::kKq;
-    const char* tp = ws.t + ((int64_t)(base + c) * a.hv + h) * Lay::kT;
-    __syncthreads();
-    for (int i = tid; i < Lay::kKq / 16; i += 256) ((uint4*)lds)[i] = ((const uint4*)kq)[i];
-    for (int i = tid; i < Lay::kT / 16; i += 256) ((uint4*)(lds + Lay::kKq))[i] = ((const uint4*)tp)[i];
-    const int t0 = r0 + c * C;
-    float v[TT][4];
+    const int nt = min(C, r1 - r0 - c * C);  // tokens of the chunk
+    float v[4];
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
+    for (int e = 0; e < 4; ++e) v[e] = Bits<DT>::value(vnext[e]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int tok = t0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + e;
-        v[t][e] = in && tok < r1 ? load1<DT>(a.v, (int64_t)tok * a.vt + h * a.vh + dv) : 0.0f;
-      }
+    for (int t = 0; t < KW; ++t) {
+      uint2 w[3];
+      split4(S[t], w);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *(uint2*)(sl + (p * KS + (wt * KW + t) / 2) * 1024 + 8 * ((wt * KW + t) & 1)) = w[p];
+    }
     __syncthreads();
-    const __bf16* K = (const __bf16*)(lds + Lay::kK);
-    const __bf16* Q = (const __bf16*)(lds + Lay::kQ);
-    const __bf16* KTr = (const __bf16*)(lds + Lay::kKT);
-    const __bf16* Tm = (const __bf16*)(lds + Lay::kKq + Lay::kTt);
-    const __bf16* Am = (const __bf16*)(lds + Lay::kKq + Lay::kA);
-    const float4* F = (const float4*)(lds + Lay::kKq + Lay::kFactors);
 
     // S k and S q
-    floatx4 X[TT], O[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) X[t] = O[t] = floatx4{0, 0, 0, 0};
+    floatx4 X[3] = {}, O[2] = {};  // sums of their own: MFMAs that follow each other do not wait for each other
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       bf16x8 sp[3];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        __bf16 p0, p1, p2;
-        split3(S[2 * s + (e >> 2)][e & 3], p0, p1, p2);
-        sp[0][e] = p0; sp[1][e] = p1; sp[2][e] = p2;
-      }
+      for (int p = 0; p < 3; ++p) sp[p] = *(const bf16x8*)(sl + (p * KS + s) * 1024);
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+      for (int p = 0; p < NK; ++p) {
+        const bf16x8 k = *(const bf16x8*)(K + (p * C + tok0 + rown) * KR + 32 * s + 8 * g);
+        const bf16x8 q = *(const bf16x8*)(Q + (p * C + tok0 + rown) * KR + 32 * s + 8 * g);
 #pragma unroll
-        for (int p = 0; p < NK; ++p) {
-          const bf16x8 k = *(const bf16x8*)(K + (p * C + row) * KR + 32 * s + 8 * g);
-          const bf16x8 q = *(const bf16x8*)(Q + (p * C + row) * KR + 32 * s + 8 * g);
-#pragma unroll
-          for (int o = 0; o + p <= 2; ++o) X[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, sp[o], X[t], 0, 0, 0);
-#pragma unroll
-          for (int o = 0; o + p <= MAXO; ++o) O[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, sp[o], O[t], 0, 0, 0);
+        for (int o = 0; o + p <= 2; ++o) {
+          X[o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, sp[o], X[o], 0, 0, 0);
+          if (o + p <= MAXO) O[o & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, sp[o], O[o & 1], 0, 0, 0);
         }
       }
     }
     // X
-    float f2[TT][4];
+    floatx4 x, f2;
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
+    for (int e = 0; e < 4; ++e) {
+      const float4 f = F[tok0 + 8 * g + e];
+      x[e] = f.x * v[e] - f.y * (X[0][e] + (X[1][e] + X[2][e]));
+      O[0][e] = (O[0][e] + O[1][e]) * f.z;
+      O[1][e] = 0.0f;
+      f2[e] = f.w;
+    }
+    const float dec = F[C].x;
+    {
+      uint2 w[3];
+      split4(x, w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 f = F[32 * (t >> 1) + 8 * g + 4 * (t & 1) + e];
-        X[t][e] = f.x * v[t][e] - f.y * X[t][e];
-        O[t][e] *= f.z;
-        f2[t][e] = f.w;
-      }
-    // U = T X
-    floatx4 U[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) U[t] = floatx4{0, 0, 0, 0};
+      for (int p = 0; p < 3; ++p) *(uint2*)(xl + (p * TS + wt / 2) * 1024 + 8 * (wt & 1)) = w[p];
+    }
+    // K^T's rows are keys: the transposing read gives a lane 4 tokens of its key, from the 4 rows that its group of 16
+    // lanes addresses (lane 4 r + c: 4 keys of row r)
+    bf16x8 tm[TS][3], am[TS][NA], km[NK][TS][KW];
 #pragma unroll
     for (int s = 0; s < TS; ++s) {
+      if (s <= wt / 2) {
+        const int o = Lay::tri(tok0 + rown, 32 * s + 8 * g);
+        split(lane8(*(const floatx4*)(Tm + o), *(const floatx4*)(Tm + o + 4)), tm[s]);
+        split(lane8(*(const floatx4*)(Am + o), *(const floatx4*)(Am + o + 4)), am[s]);
+      }
+#pragma unroll
+      for (int p = 0; p < NK; ++p)
+#pragma unroll
+        for (int t = 0; t < KW; ++t) {
+          const __bf16* k = K + (p * C + 32 * s + 8 * g + (n >> 2)) * KR + key(t) + 8 * (n & 3);
+          km[p][s][t] = join(turned(k), turned(k + 4 * KR));
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the chunk's operands are here
+    __syncthreads();
+    fetch(min(c + 1, chunks - 1));  // taken within this turn, so that its wait does not take in the stores
+
+    // U = T X; T is 0 above its diagonal
+    floatx4 U[3] = {};
+#pragma unroll
+    for (int s = 0; s < TS; ++s) {
+      if (s > wt / 2) break;
       bf16x8 xp[3];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        __bf16 p0, p1, p2;
-        split3(X[2 * s + (e >> 2)][e & 3], p0, p1, p2);
-        xp[0][e] = p0; xp[1][e] = p1; xp[2][e] = p2;
-      }
+      for (int p = 0; p < 3; ++p) xp[p] = *(const bf16x8*)(xl + (p * TS + s) * 1024);
 #pragma unroll
-      for (int t = 2 * s; t < TT; ++t) {  // T is 0 above its diagonal
-        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+      for (int p = 0; p < 3; ++p)
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          const bf16x8 m = *(const bf16x8*)(Tm + (p * C + row) * CR + 32 * s + 8 * g);
-#pragma unroll
-          for (int o = 0; o + p <= 2; ++o) U[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, xp[o], U[t], 0, 0, 0);
-        }
-      }
+        for (int o = 0; o + p <= 2; ++o) U[o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tm[s][p], xp[o], U[o], 0, 0, 0);
     }
-    // O += A U;   S = e^{G_c} S + K^T (e^{G_c - G} U)
-    const float dec = F[C].x;
+    const floatx4 u = U[0] + (U[1] + U[2]);
+    {
+      uint2 w[3], o[MAXO + 1];
+      split4(u * f2, w);
+      split4(u, o);
 #pragma unroll
-    for (int t = 0; t < KT; ++t) S[t] *= dec;
+      for (int p = 0; p < 3; ++p) *(uint2*)(ul + (p * TS + wt / 2) * 1024 + 8 * (wt & 1)) = w[p];
+#pragma unroll
+      for (int p = 0; p <= MAXO; ++p) *(uint2*)(ul + ((3 + p) * TS + wt / 2) * 1024 + 8 * (wt & 1)) = o[p];
+    }
+    __syncthreads();
+
+    // S = e^{G_c} S + K^T (e^{G_c - G} U);   O += A U
+#pragma unroll
+    for (int t = 0; t < KW; ++t) S[t] *= dec;
 #pragma unroll
     for (int s = 0; s < TS; ++s) {
-      bf16x8 up[3], wp[3];
+      bf16x8 wp[3], up[MAXO + 1];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        __bf16 p0, p1, p2;
-        split3(U[2 * s + (e >> 2)][e & 3], p0, p1, p2);
-        up[0][e] = p0; up[1][e] = p1; up[2][e] = p2;
-        split3(U[2 * s + (e >> 2)][e & 3] * f2[2 * s + (e >> 2)][e & 3], p0, p1, p2);
-        wp[0][e] = p0; wp[1][e] = p1; wp[2][e] = p2;
-      }
+      for (int p = 0; p < 3; ++p) wp[p] = *(const bf16x8*)(ul + (p * TS + s) * 1024);
 #pragma unroll
-      for (int t = 2 * s; t < TT; ++t) {
-        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+      for (int p = 0; p <= MAXO; ++p) up[p] = *(const bf16x8*)(ul + ((3 + p) * TS + s) * 1024);
 #pragma unroll
-        for (int p = 0; p < NA; ++p) {
-          const bf16x8 m = *(const bf16x8*)(Am + (p * C + row) * CR + 32 * s + 8 * g);
+      for (int p = 0; p < NK; ++p)
 #pragma unroll
-          for (int o = 0; o + p <= MAXO; ++o) O[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, up[o], O[t], 0, 0, 0);
-        }
-      }
+        for (int o = 0; o + p <= 2; ++o)
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const int row = 32 * (t >> 1) + 4 * (t & 1) + rown;
+          for (int t = 0; t < KW; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(km[p][s][t], wp[o], S[t], 0, 0, 0);
+      if (s > wt / 2) continue;  // A is 0 above its diagonal
 #pragma unroll
-        for (int p = 0; p < NK; ++p) {
-          const bf16x8 m = *(const bf16x8*)(KTr + (p * DK + row) * CR + 32 * s + 8 * g);
+      for (int p = 0; p < NA; ++p)
 #pragma unroll
-          for (int o = 0; o + p <= 2; ++o) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, wp[o], S[t], 0, 0, 0);
-        }
-      }
+        for (int o = 0; o + p <= MAXO; ++o)
+          O[(o + p) & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(am[s][p], up[o], O[(o + p) & 1], 0, 0, 0);
     }
+    const __amdgpu_buffer_rsrc_t rs = gguf::buffer_rsrc((char*)a.out + (int64_t)(r0 + c * C) * ot + (int64_t)h * a.dv * ES, (C - 1) * ot + a.dv * ES);
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int tok = t0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + e;
-        if (in && tok < r1) gguf::store_y(a.out, ((int64_t)tok * a.hv + h) * a.dv + dv, O[t][e], DT);
-      }
+    for (int e = 0; e < 4; ++e) Bits<DT>::store(rs, place(e, nt, ot), O[0][e] + O[1][e]);
+    __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4): all but these stores
   }
-  put(a.out_slots[(int64_t)seq * a.out_stride]);
+  const int to = a.out_slots[(int64_t)seq * a.out_stride];
+  if (in && to >= 0 && to < a.nslots)
+#pragma unroll
+    for (int t = 0; t < KW; ++t) *(floatx4*)(a.state + to * slot + at + key(t)) = S[t];
 }
 
 template <int DT, int DK>
@@ -555,7 +653,7 @@ hipError_t launch(const DeltaArgs& a, int64_t max_new, void* wsp, hipStream_t st
   typedef Layout<DT, DK, C> Lay;
   const int64_t slots = a.rows.tokens / C + a.rows.seqs;
   ChunkWs ws{(char*)wsp, (char*)wsp + slots * a.hk * Lay::kKq};
-  constexpr int prep_lds = Lay::NK * C * Lay::KR * 4 + 2 * C * (C + 4) * 4, scan_lds = Lay::kKq + Lay::kT;
+  constexpr int prep_lds = Lay::NK * C * Lay::KR * 4 + 2 * C * (C + 4) * 4, scan_lds = Lay::kLds;
   int dev = 0;
   if ((e = hipGetDevice(&dev)) != hipSuccess) return e;
   struct Tag {};
@@ -565,7 +663,8 @@ hipError_t launch(const DeltaArgs& a, int64_t max_new, void* wsp, hipStream_t st
   });
   prep_kernel<DT, DK, C><<<dim3((unsigned)slots, a.hv), 256, prep_lds, stream>>>(a, most, ws);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  scan_kernel<DT, DK, C><<<dim3((a.dv + 63) / 64, a.hv, a.rows.seqs), 256, scan_lds, stream>>>(a, most, ws);
+  // heads first: workgroups of one head, which share its operands, then run on one XCD where heads are a multiple of 8
+  scan_kernel<DT, DK, C><<<dim3(a.hv, (a.dv + 16 * Lay::ND - 1) / (16 * Lay::ND), a.rows.seqs), 64 * Lay::WAVES, scan_lds, stream>>>(a, most, ws);
   return hipGetLastError();
 }
 
