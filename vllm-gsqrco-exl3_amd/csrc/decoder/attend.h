@@ -55,4 +55,53 @@ __device__ __forceinline__ float row_factor(float amax) {
   return amax > 0.0f && e >= 1 && e <= 253 ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
 }
 
+// Where a 16-token chunk lies (page * heads + head, first token in the page), and its scales.
+struct Chunk {
+  int ph, off;
+  float ks, vs;
+};
+
+// Chunk ch of a sequence. One past position `see` has scales of 0; a page out of range reads as NaN, and a V scale
+// that is not finite is NaN for the rows that see it and no measure for the others. ph is always a page's.
+__device__ __forceinline__ Chunk chunk_of(const Kv8& c, const int32_t* table, int page16, int head, int64_t ch, int see) {
+  const bool seen = see >= 0 && ch <= see / 16;
+  const int pi = seen ? (int)ch / page16 : 0;
+  const int pid = table[pi];
+  const bool ok = seen && pid >= 0 && pid < c.pages;
+  Chunk r;
+  r.ph = (ok ? pid : 0) * c.heads + head;
+  r.off = seen ? ((int)ch - pi * page16) * 16 : 0;
+  const float none = seen ? __builtin_nanf("") : 0.0f;
+  r.ks = ok ? c.ks[r.ph] : none;
+  r.vs = ok ? c.vs[r.ph] : none;
+  if (!(r.vs <= 3.0e38f)) r.vs = __builtin_nanf("");
+  return r;
+}
+
+// max over lanes l and l ^ 32
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// What a call is made of.
+struct AttnArgs {
+  Kv8 c;
+  const void* q;
+  int64_t qt, qh;  // strides of a token and a head, in elements
+  const int32_t* lens;
+  Ragged rows;
+  int hq, group;   // query heads; query heads a KV head
+  float scale;     // times log2 e
+  int span;        // tokens of a split, a multiple of 256 (the last split takes what is left)
+  int splits;
+  void* out;       // [tokens, hq, d]
+  float* part;     // of a split call: [splits][tokens * hq][d] sums, then m and l: [splits][tokens * hq][2]
+  float* stat;
+};
+
+// attention_rows.hip: many rows
+constexpr int kRowsTile = 128;  // rows of a workgroup
+hipError_t launch_attend_rows(const AttnArgs& a, int dtype, int64_t row_tiles, hipStream_t stream);
+
 }  // namespace gguf_dec

@@ -8,20 +8,6 @@ namespace {
 constexpr int kTile = 64;   // tokens a wave takes at a time
 constexpr int kWaves = 4;
 
-struct AttnArgs {
-  Kv8 c;
-  const void* q;
-  int64_t qt, qh;  // strides of a token and a head, in elements
-  const int32_t* lens;
-  Ragged rows;
-  int hq, group;   // query heads; query heads a KV head
-  float scale;     // times log2 e
-  int tiles;       // tiles of a split (the last split takes what is left)
-  void* out;       // [tokens, hq, d]
-  float* part;     // [splits][tokens * hq][d], then m and l: [splits][tokens * hq][2]
-  float* stat;
-};
-
 // One workgroup takes RT = 16 NT query rows (token, head of the KV head's group) of one sequence and
 // KV head, and one split of its tokens; its waves take the split's tiles in turn, straight from the cache into
 // operand registers (each byte is read by one lane, so LDS would only add a hop), with statistics and
@@ -93,8 +79,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
       all = min(all, __shfl_xor(all, off, 64));
     }
     const int ntiles = (see + kTile) / kTile;  // see = -1: none
-    const int tb = split * a.tiles;
-    const int te = split == splits - 1 ? ntiles : min(ntiles, tb + a.tiles);
+    const int tb = (int)min((int64_t)split * (a.span / kTile), (int64_t)ntiles);
+    const int te = split == splits - 1 ? ntiles : min(ntiles, tb + a.span / kTile);
     if (splits > 1 && tb >= te) {  // uniform: nothing of these rows lies in the split
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -116,17 +102,10 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
 
     for (int tile = tb + wave; tile < te; tile += kWaves) {
       // chunk g of the tile: its page, scales; the K operand's rows lie in chunk n >> 2
-      const int ch = 4 * tile + g;
-      const int pi = ch / page16;
-      int pid = -1;
-      if (16 * ch <= see) pid = table[pi];
-      const bool ok = pid >= 0 && pid < a.c.pages;
-      const int64_t ph = ok ? (int64_t)pid * a.c.heads + head : 0;
-      const float bad = 16 * ch <= see ? __builtin_nanf("") : 0.0f;
-      const float ks = ok ? a.c.ks[ph] : bad;
-      float vs = ok ? a.c.vs[ph] : bad;
-      if (!(vs <= 3.0e38f)) vs = __builtin_nanf("");  // not finite: NaN for those that see the page, no reference for the others
-      const int off = (ch - pi * page16) * 16;
+      const Chunk ck = chunk_of(a.c, table, page16, head, (int64_t)4 * tile + g, see);
+      const int64_t ph = ck.ph;
+      const int off = ck.off;
+      const float ks = ck.ks, vs = ck.vs;
       const int8_t* vp = a.c.v + ph * a.c.page * D + (int64_t)n * a.c.page + off;
       const int64_t koff = (ph * a.c.page + off) * D;
       const int64_t kc = __shfl(koff, 16 * (n >> 2), 64);
@@ -285,58 +264,55 @@ hipError_t launch_attend(const AttnArgs& a, dim3 grid, hipStream_t stream) {
 
 }  // namespace
 
-// tiles of a split, and the splits of a call: as many as fill the CUs twice, of at least one tile a wave
-static void attn_plan(int64_t blocks, int64_t max_len, int& tiles, int& splits) {
-  const int64_t ntiles = (max_len + kTile - 1) / kTile;
-  int64_t want = blocks > 0 ? (2 * gguf::device_cus() + blocks - 1) / blocks : 1;
-  int64_t per = (ntiles + want - 1) / want;
-  per = (per + kWaves - 1) / kWaves * kWaves;
-  if (per < kWaves) per = kWaves;
-  int64_t n = (ntiles + per - 1) / per;
-  if (n < 1) n = 1;
-  if (n > 512) {
-    per = ((ntiles + 511) / 512 + kWaves - 1) / kWaves * kWaves;
-    n = (ntiles + per - 1) / per;
-  }
-  tiles = (int)(per < (1 << 25) ? per : (1 << 25));
-  splits = (int)n;
-}
+// How a call is cut: rows of a workgroup, and tokens of a split so that the CUs have two workgroups each, in
+// steps of a tile a wave.
+struct AttnPlan {
+  bool many;
+  int nt, span, splits;
+  int64_t row_tiles;
+};
 
-static int attn_nt(int64_t rows) { return rows > 16 ? 2 : 1; }
+static AttnPlan attn_plan(int64_t rows, int64_t groups, int64_t max_len, int64_t most_splits) {
+  AttnPlan p;
+  p.many = rows > 64;
+  p.nt = rows > 16 ? 2 : 1;
+  const int64_t tile = p.many ? kRowsTile : 16 * p.nt;
+  p.row_tiles = (rows + tile - 1) / tile;
+  const int64_t blocks = groups * p.row_tiles, step = kTile * kWaves;
+  const int64_t steps = (max_len + step - 1) / step;
+  int64_t want = (2 * gguf::device_cus() + blocks - 1) / blocks;
+  if (want > 512) want = 512;
+  if (want > most_splits) want = most_splits;
+  if (want < 1) want = 1;
+  const int64_t each = (steps + want - 1) / want;
+  p.span = (int)(each * step < (1 << 30) ? each * step : (1 << 30));
+  p.splits = (int)((steps + each - 1) / each);
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
 
 size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t seqs, int64_t max_new,
                                int64_t max_len) {
-  const int64_t rows = max_new * (hq / heads);
-  const int nt = attn_nt(rows);
-  int tiles, splits;
-  attn_plan(seqs * heads * ((rows + 16 * nt - 1) / (16 * nt)), max_len, tiles, splits);
-  return splits == 1 ? 0 : (size_t)splits * tokens * hq * (d + 2) * sizeof(float);
+  const AttnPlan p = attn_plan(max_new * (hq / heads), seqs * heads, max_len, 512);
+  return p.splits == 1 ? 0 : (size_t)p.splits * tokens * hq * (d + 2) * sizeof(float);
 }
 
 hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t qt, int64_t qh, int hq,
                                 const int32_t* lens, const Ragged& rows, int64_t max_new, int64_t max_len, float scale,
                                 void* out, void* ws, size_t ws_bytes, hipStream_t stream) {
-  const int64_t trows = max_new * (hq / c.heads);
-  const int nt = attn_nt(trows);
-  const int64_t row_tiles = (trows + 16 * nt - 1) / (16 * nt);
-  int tiles, splits;
-  attn_plan((int64_t)rows.seqs * c.heads * row_tiles, max_len, tiles, splits);
   const int64_t all = (int64_t)rows.tokens * hq;
   const int64_t fit = (int64_t)(ws_bytes / sizeof(float)) / (all * (c.d + 2));
-  if (splits > 1 && fit < splits) {
-    splits = fit < 2 ? 1 : (int)fit;
-    const int64_t ntiles = (max_len + kTile - 1) / kTile;
-    tiles = (int)((ntiles + splits - 1) / splits);
-  }
-  AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, tiles, out, (float*)ws,
-             (float*)ws + (size_t)splits * all * c.d};
-  const dim3 grid((unsigned)(row_tiles < 65535 ? row_tiles : 65535), (unsigned)(rows.seqs * c.heads), splits);
+  const AttnPlan p = attn_plan(max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len, fit < 2 ? 1 : fit);
+  const AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, p.span, p.splits, out, (float*)ws,
+                   (float*)ws + (size_t)p.splits * all * c.d};
+  const dim3 grid((unsigned)(p.row_tiles < 65535 ? p.row_tiles : 65535), (unsigned)(rows.seqs * c.heads), p.splits);
   hipError_t e = hipSuccess;
-#define GGUF_DEC_ATTEND(DT, D)                                                                    \
-  {                                                                                               \
-    e = nt == 1 ? launch_attend<DT, D, 1>(a, grid, stream) : launch_attend<DT, D, 2>(a, grid, stream); \
-    if (e == hipSuccess && splits > 1)                                                            \
-      join_kernel<DT, D><<<(unsigned)((all + 3) / 4), 256, 0, stream>>>(a.part, a.stat, all, splits, out); \
+  if (p.many) e = launch_attend_rows(a, dtype, p.row_tiles, stream);
+#define GGUF_DEC_ATTEND(DT, D)                                                                                         \
+  {                                                                                                                    \
+    if (!p.many) e = p.nt == 1 ? launch_attend<DT, D, 1>(a, grid, stream) : launch_attend<DT, D, 2>(a, grid, stream);  \
+    if (e == hipSuccess && p.splits > 1)                                                                               \
+      join_kernel<DT, D><<<(unsigned)((all + 3) / 4), 256, 0, stream>>>(a.part, a.stat, all, p.splits, out);           \
   }
 #define GGUF_DEC_ATTEND_D(DT)                 \
   switch (c.d) {                              \

@@ -145,7 +145,7 @@ int check_cache(const char* op, const gguf_kv8_cache* c, const gguf_tensor* tabl
   const int64_t p = c->k.size[0], h = c->k.size[1], page = c->k.size[2], d = c->k.size[3];
   if (p < 1 || h < 1 || page < 16 || page % 16) return fail("%s: the cache needs pages, heads and pages of a multiple of 16 tokens, got [%lld, %lld, %lld, ...]", op, (long long)p, (long long)h, (long long)page);
   if (d != 64 && d != 128 && d != 192 && d != 256) return fail("%s: head size %lld is not 64, 128, 192 or 256", op, (long long)d);
-  if (h > 16384 || page * d > (1 << 28)) return fail("%s: cache of too many heads or too large pages", op);
+  if (p * h > INT_MAX || h > 16384 || page * d > (1 << 28)) return fail("%s: cache of too many heads or too large pages", op);
   if (c->v.size[0] != p || c->v.size[1] != h || c->v.size[2] != d || c->v.size[3] != page)
     return fail("%s: v of the cache must be [pages, heads, head size, page]", op);
   if (c->k_scale.size[0] != p || c->k_scale.size[1] != h || c->v_scale.size[0] != p || c->v_scale.size[1] != h)
