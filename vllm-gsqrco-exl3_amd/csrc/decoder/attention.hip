@@ -7,6 +7,7 @@ namespace {
 
 constexpr int kTile = 64;   // tokens a wave takes at a time
 constexpr int kWaves = 4;
+constexpr int kSegment = 64;  // tiles whose chunks are looked up at a time
 
 // One workgroup takes RT = 16 NT query rows (token, head of the KV head's group) of one sequence and
 // KV head, and one split of its tokens; its waves take the split's tiles in turn, straight from the cache into
@@ -22,10 +23,14 @@ template <int DT, int D, int NT>
 __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   constexpr int S = D / 64, DD = D / 16;
   extern __shared__ __align__(16) float lds[];  // [kWaves][DD][NT][64][4]
-  __shared__ float stat[kWaves][NT * 16][2], refs[kWaves];
+  __shared__ float stat[kWaves][NT * 16][2];
+  __shared__ Chunk chunks[4 * kSegment];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
   const int seqs = a.rows.seqs;
-  const int head = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads, split = blockIdx.z, splits = gridDim.z;
+  // row tiles of one (sequence, head, split) read the same tokens: a stride of gridDim.x apart, they run on as few XCDs as
+  // there are, and share their L2. Later splits, which short sequences do not have, come last.
+  const int head = blockIdx.x % a.c.heads, seq = blockIdx.x / a.c.heads % a.rows.seqs;
+  const int split = blockIdx.x / a.c.heads / a.rows.seqs, splits = a.splits;
   int r0, r1;
   rows_of(a.rows, seq, r0, r1);
   const int64_t nrows = (int64_t)(r1 - r0) * a.group;
@@ -34,11 +39,22 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   const int page16 = a.c.page / 16;
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
 
-  for (int64_t tile0 = (int64_t)blockIdx.x * 16 * NT; tile0 < nrows; tile0 += (int64_t)gridDim.x * 16 * NT) {
+  for (int64_t tile0 = (int64_t)blockIdx.y * 16 * NT; tile0 < nrows; tile0 += (int64_t)gridDim.y * 16 * NT) {
+    // what the tile's rows see at most: they are in order of their tokens
+    const int64_t rlast = min(nrows, tile0 + 16 * NT) - 1;
+    const int see = (int)max(min((int64_t)len0 - (r1 - r0) + rlast / a.group, room - 1), (int64_t)-1);
+    const int ntiles = (see + kTile) / kTile;  // see = -1: none
+    const int tb = (int)min((int64_t)split * (a.span / kTile), (int64_t)ntiles);
+    const int te = split == splits - 1 ? ntiles : min(ntiles, tb + a.span / kTile);
+    const auto find_chunks = [&](int from, int to) __attribute__((always_inline)) {
+      for (int i = tid; i < 4 * (to - from); i += 64 * kWaves)
+        chunks[i] = chunk_of(a.c, table, page16, head, (int64_t)4 * from + i, see);
+    };
+    find_chunks(tb, min(tb + kSegment, te));  // (the previous rows are through: see the loop's end)
     // rows of this tile: row -> (token, head); last: the last position that it sees
     int64_t qrow[NT];
     int last[NT];
-    int see = -1, all = 0x7FFFFFFF;  // the last position that any / every row sees
+    int all = 0x7FFFFFFF;  // the last position that every row sees
     half8 q[NT][2 * S];
     float qs[NT];
 #pragma unroll
@@ -49,7 +65,6 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
       qrow[t] = ok ? (int64_t)(r0 + tok) * a.hq + h : -1;
       const int64_t l = ok ? (int64_t)len0 - (r1 - r0) + tok : -1;
       last[t] = (int)(l < room ? l : room - 1);
-      see = max(see, last[t]);
       if (ok) all = min(all, last[t]);
       float amax = 0.0f;
       float v[2 * S][8];
@@ -75,12 +90,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) {
-      see = max(see, __shfl_xor(see, off, 64));
       all = min(all, __shfl_xor(all, off, 64));
     }
-    const int ntiles = (see + kTile) / kTile;  // see = -1: none
-    const int tb = (int)min((int64_t)split * (a.span / kTile), (int64_t)ntiles);
-    const int te = split == splits - 1 ? ntiles : min(ntiles, tb + a.span / kTile);
     if (splits > 1 && tb >= te) {  // uniform: nothing of these rows lies in the split
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -91,7 +102,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
 
     floatx4 o[DD][NT];
     float m[NT], l[NT];
-    float ref = 0.0f;
+    float ref = 0.0f, inv_ref = 0.0f;
+    int seg = tb;  // chunks[0] is of this tile
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = kNoScore;
@@ -100,41 +112,46 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
       for (int i = 0; i < DD; ++i) o[i][t] = floatx4{0, 0, 0, 0};
     }
 
-    for (int tile = tb + wave; tile < te; tile += kWaves) {
-      // chunk g of the tile: its page, scales; the K operand's rows lie in chunk n >> 2
-      const Chunk ck = chunk_of(a.c, table, page16, head, (int64_t)4 * tile + g, see);
-      const int64_t ph = ck.ph;
-      const int off = ck.off;
-      const float ks = ck.ks, vs = ck.vs;
-      const int8_t* vp = a.c.v + ph * a.c.page * D + (int64_t)n * a.c.page + off;
-      const int64_t koff = (ph * a.c.page + off) * D;
-      const int64_t kc = __shfl(koff, 16 * (n >> 2), 64);
-      const int8_t* kp = a.c.k + kc + (n & 3) * D + 16 * g;
-
+    // K and V of a wave's next tile are on their way while it works on this one. Lane group g looks after chunk g; the K
+    // operand's rows lie in chunk n >> 2.
+    uintx4 kw[4][S], vw[DD];
+    const auto load_k = [&](int tile) __attribute__((always_inline)) {
+      const Chunk& c = chunks[4 * (tile - seg) + (n >> 2)];
+      const int8_t* kp = a.c.k + ((int64_t)c.ph * a.c.page + c.off + (n & 3)) * D + 16 * g;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int i = 0; i < S; ++i) kw[tt][i] = *(const uintx4*)(kp + 4 * tt * D + 64 * i);
+    };
+    const auto load_v = [&](int tile) __attribute__((always_inline)) {
+      const Chunk& c = chunks[4 * (tile - seg) + g];
+      const int8_t* vp = a.c.v + ((int64_t)c.ph * D + n) * a.c.page + c.off;
+#pragma unroll
+      for (int i = 0; i < DD; ++i) vw[i] = *(const uintx4*)(vp + (uint32_t)(16 * i * a.c.page));
+    };
+    const auto work = [&](int tile, int then) __attribute__((always_inline)) {
+      const float ks = chunks[4 * (tile - seg) + g].ks, vs = chunks[4 * (tile - seg) + g].vs;
       floatx4 sc[4][NT];
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[tt][t] = floatx4{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const uint4 w = *(const uint4*)(kp + 4 * tt * D + 64 * s);
-          const half8 k0 = codes8(w.x, w.y), k1 = codes8(w.z, w.w);
+        for (int i = 0; i < S; ++i) {
+          const half8 k0 = codes8(kw[tt][i][0], kw[tt][i][1]), k1 = codes8(kw[tt][i][2], kw[tt][i][3]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            sc[tt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[t][2 * s], sc[tt][t], 0, 0, 0);
-            sc[tt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[t][2 * s + 1], sc[tt][t], 0, 0, 0);
+            sc[tt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[t][2 * i], sc[tt][t], 0, 0, 0);
+            sc[tt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[t][2 * i + 1], sc[tt][t], 0, 0, 0);
           }
         }
       }
+      load_k(then);
 
       const float top = group_max(vs);
-      const float nref = fmaxf(ref, top);
-      const float shrink = nref > ref ? ref / nref : 1.0f;
-      ref = nref;
-      const float vr = ref > 0.0f ? vs / ref : vs;  // vs is 0 (or NaN) where ref is 0
       const bool masked = kTile * tile + kTile - 1 > all;
-      half8 p[NT][2];
+      float nm[NT];
+      bool grown = top > ref;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float f = qs[t] * ks;
@@ -148,37 +165,66 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
             sc[tt][t][i] = x;
             mx = fmaxf(mx, x);
           }
-        mx = fmaxf(group_max(mx), m[t]);
-        const float al = __builtin_amdgcn_exp2f(m[t] - mx);
-        m[t] = mx;
-        float sum = 0.0f;
+        // the maximum may lag: weights stay below 2^8, and the sums are scaled again only where it does not do, or
+        // where the largest V scale grew
+        mx = group_max(mx);
+        nm[t] = mx > m[t] + 8.0f ? mx : m[t];
+        grown = grown || nm[t] != m[t];
+      }
+      if (__any(grown)) {
+        const float nref = fmaxf(ref, top);
+        const float shrink = nref > ref ? ref / nref : 1.0f;
+        ref = nref;
+        inv_ref = ref > 0.0f ? 1.0f / ref : 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float al = __builtin_amdgcn_exp2f(m[t] - nm[t]);
+          m[t] = nm[t];
+          l[t] *= al;
+#pragma unroll
+          for (int i = 0; i < DD; ++i) o[i][t] *= al * shrink;
+        }
+      }
+      const float vr = vs * inv_ref;
+      half8 p[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = sc[tt][t][i];
-            const float e = __builtin_amdgcn_exp2f(x - mx);
-            sum += e;
+            const float e = __builtin_amdgcn_exp2f(x - m[t]);
+            l[t] += e;
             // a masked place adds nothing, also where its page's scale is not finite
-            p[t][tt >> 1][4 * (tt & 1) + i] = (_Float16)(x == -__builtin_inff() ? 0.0f : e * vr);
+            p[t][tt >> 1][4 * (tt & 1) + i] = (_Float16)(masked && x == -__builtin_inff() ? 0.0f : e * vr);
           }
-        l[t] = l[t] * al + sum;
-        const float r = al * shrink;
-        if (__any(r != 1.0f)) {
-#pragma unroll
-          for (int i = 0; i < DD; ++i) o[i][t] *= r;
-        }
       }
 #pragma unroll
       for (int i = 0; i < DD; ++i) {
-        const uint4 w = *(const uint4*)(vp + (int64_t)16 * i * a.c.page);
-        const half8 v0 = codes8(w.x, w.y), v1 = codes8(w.z, w.w);
+        const half8 v0 = codes8(vw[i][0], vw[i][1]), v1 = codes8(vw[i][2], vw[i][3]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           o[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[t][0], o[i][t], 0, 0, 0);
           o[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[t][1], o[i][t], 0, 0, 0);
         }
       }
+      load_v(then);
+    };
+    for (seg = tb; seg < te; seg += kSegment) {
+      const int stop = min(seg + kSegment, te);
+      if (seg != tb) {
+        __syncthreads();
+        find_chunks(seg, stop);
+      }
+      __syncthreads();
+      int tile = seg + wave;
+      if (tile < stop) {
+        load_k(tile);
+        load_v(tile);
+      }
+      // past the wave's last tile it is loaded again, for nobody
+      for (; tile < stop; tile += kWaves) work(tile, tile + kWaves < stop ? tile + kWaves : tile);
     }
 
     // join the waves: the common maximum, then the scaled sums
@@ -225,27 +271,40 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   }
 }
 
-// Joins the splits of a row: one wave a row, 4 dims a lane and turn.
+// Joins the splits of a row. One workgroup a row: its waves take the splits in turn, 4 dims a lane, and join through LDS.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, const float* __restrict__ stat,
                                                    int64_t rows, int splits, void* __restrict__ out) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 63;
+  __shared__ floatx4 sums[4][64];
+  __shared__ float ls[4];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = min(4 * lane, D - 4);
   float mx = kNoScore;
-  for (int s = 0; s < splits; ++s) mx = fmaxf(mx, stat[(s * rows + row) * 2]);
+  for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, stat[(s * rows + row) * 2]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
   float sum = 0.0f;
   floatx4 acc = {0, 0, 0, 0};
-  for (int s = 0; s < splits; ++s) {
-    const float l = stat[(s * rows + row) * 2 + 1];
-    const float f = __builtin_amdgcn_exp2f(stat[(s * rows + row) * 2] - mx);
-    if (l == 0.0f) continue;
-    sum += l * f;
-    if (4 * lane < D) acc += *(const floatx4*)(part + (s * rows + row) * D + 4 * lane) * f;
+#pragma unroll 4
+  for (int s = wave; s < splits; s += 4) {
+    const float2 ml = *(const float2*)(stat + (s * rows + row) * 2);
+    const floatx4 x = *(const floatx4*)(part + (s * rows + row) * D + at);
+    const float f = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+    sum += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += ml.y == 0.0f ? 0.0f : x[e] * f;  // an empty split's sums are not written
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const float y[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
-  if (4 * lane < D) store4<DT>(out, row * D + 4 * lane, y);
+  sums[wave][lane] = acc;
+  if (lane == 0) ls[wave] = sum;
+  __syncthreads();
+  if (wave == 0 && 4 * lane < D) {
+    sum = ls[0] + ls[1] + ls[2] + ls[3];
+    acc = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float y[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    store4<DT>(out, row * D + 4 * lane, y);
+  }
 }
 
 template <int DT, int D, int NT>
@@ -272,10 +331,10 @@ struct AttnPlan {
   int64_t row_tiles;
 };
 
-static AttnPlan attn_plan(int64_t rows, int64_t groups, int64_t max_len, int64_t most_splits) {
+static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, int64_t most_splits) {
   AttnPlan p;
   p.many = rows > 64;
-  p.nt = rows > 16 ? 2 : 1;
+  p.nt = rows > 16 && d < 256 ? 2 : 1;
   const int64_t tile = p.many ? kRowsTile : 16 * p.nt;
   p.row_tiles = (rows + tile - 1) / tile;
   const int64_t blocks = groups * p.row_tiles, step = kTile * kWaves;
@@ -293,7 +352,7 @@ static AttnPlan attn_plan(int64_t rows, int64_t groups, int64_t max_len, int64_t
 
 size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t seqs, int64_t max_new,
                                int64_t max_len) {
-  const AttnPlan p = attn_plan(max_new * (hq / heads), seqs * heads, max_len, 512);
+  const AttnPlan p = attn_plan(d, max_new * (hq / heads), seqs * heads, max_len, 512);
   return p.splits == 1 ? 0 : (size_t)p.splits * tokens * hq * (d + 2) * sizeof(float);
 }
 
@@ -302,17 +361,19 @@ hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t 
                                 void* out, void* ws, size_t ws_bytes, hipStream_t stream) {
   const int64_t all = (int64_t)rows.tokens * hq;
   const int64_t fit = (int64_t)(ws_bytes / sizeof(float)) / (all * (c.d + 2));
-  const AttnPlan p = attn_plan(max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len, fit < 2 ? 1 : fit);
+  const AttnPlan p = attn_plan(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len, fit < 2 ? 1 : fit);
   const AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, p.span, p.splits, out, (float*)ws,
                    (float*)ws + (size_t)p.splits * all * c.d};
-  const dim3 grid((unsigned)(p.row_tiles < 65535 ? p.row_tiles : 65535), (unsigned)(rows.seqs * c.heads), p.splits);
+  const dim3 grid((unsigned)(rows.seqs * c.heads * p.splits), (unsigned)(p.row_tiles < 65535 ? p.row_tiles : 65535));
   hipError_t e = hipSuccess;
   if (p.many) e = launch_attend_rows(a, dtype, p.row_tiles, stream);
 #define GGUF_DEC_ATTEND(DT, D)                                                                                         \
   {                                                                                                                    \
-    if (!p.many) e = p.nt == 1 ? launch_attend<DT, D, 1>(a, grid, stream) : launch_attend<DT, D, 2>(a, grid, stream);  \
+    if (!p.many && p.nt == 1) e = launch_attend<DT, D, 1>(a, grid, stream);                                            \
+    if constexpr (D < 256)                                                                                             \
+      if (!p.many && p.nt == 2) e = launch_attend<DT, D, 2>(a, grid, stream);                                          \
     if (e == hipSuccess && p.splits > 1)                                                                               \
-      join_kernel<DT, D><<<(unsigned)((all + 3) / 4), 256, 0, stream>>>(a.part, a.stat, all, p.splits, out);           \
+      join_kernel<DT, D><<<(unsigned)all, 256, 0, stream>>>(a.part, a.stat, all, p.splits, out);           \
   }
 #define GGUF_DEC_ATTEND_D(DT)                 \
   switch (c.d) {                              \

@@ -52,9 +52,9 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
   __shared__ __align__(16) Chunk chunks[2 * (kSegment + 3)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
   // workgroups of one (sequence, head, split) take the same tiles: a stride of gridDim.x apart, they run on as few XCDs as
-  // there are, and share their L2
-  const int split = blockIdx.x % a.splits, splits = a.splits;
-  const int head = blockIdx.x / splits % a.c.heads, seq = blockIdx.x / splits / a.c.heads;
+  // there are, and share their L2. Later splits, which short sequences do not have, come last.
+  const int head = blockIdx.x % a.c.heads, seq = blockIdx.x / a.c.heads % a.rows.seqs;
+  const int split = blockIdx.x / a.c.heads / a.rows.seqs, splits = a.splits;
   int r0, r1;
   rows_of(a.rows, seq, r0, r1);
   const int64_t nrows = (int64_t)(r1 - r0) * a.group;
