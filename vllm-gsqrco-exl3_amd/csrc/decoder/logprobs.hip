@@ -18,12 +18,19 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTopMax = 64;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // order-preserving: a < b as floats <=> key(a) < key(b); -0 = +0; NaN above +inf
 __device__ __forceinline__ uint32_t order_key(float x) {
   if (x != x) return 0xFFFFFFFFu;
   const uint32_t b = __float_as_uint(x + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// the value of an order key (not 0)
+__device__ __forceinline__ float value_of(uint32_t key) {
+  if (key == 0xFFFFFFFFu) return __builtin_nanf("");
+  return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
 __device__ __forceinline__ uint64_t full_key(float x, uint32_t index) {
@@ -95,23 +102,29 @@ struct Part {
   int before;
 };
 
+// the next float below x (x finite)
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 -> +0
+  return b == 0 ? __uint_as_float(0x80000001u) : __uint_as_float(b & 0x80000000u ? b + 1 : b - 1);
+}
+
+// One workgroup a chunk of E values a thread. VALU-bound, so what is done for every value is kept short: the rank is one comparison against the given value or the next one below it (for pieces
+// before the given token, whose equal values count too), and the best tokens go by the threads' maxima: the
+// top-th largest of a wave's bounds the chunk's top-th best from below, and only what reaches it is looked at by key. Where ties make that too many for the list, keys decide from the start (select_top).
 template <int DT, int E>
 __global__ void __launch_bounds__(kThreads) chunk_kernel(const void* __restrict__ x, int64_t stride, int vocab,
                                                          const int64_t* __restrict__ ids, int64_t id_stride, int top,
                                                          Part* __restrict__ parts, uint64_t* __restrict__ keys) {
-  constexpr int VEC = 8;
+  constexpr int VEC = 8, WAVES = kThreads / 64;
   constexpr int SIZE = DT == kF32 ? 4 : 2;
   extern __shared__ __align__(16) uint64_t lds[];  // most, list
-  __shared__ float fs[3][kThreads / 64];
-  __shared__ int is[kThreads / 64];
+  __shared__ float fs[4][WAVES];
+  __shared__ int is[WAVES], count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.y, chunk = blockIdx.x, chunks = gridDim.x;
   const char* base = (const char*)x + row * stride * SIZE;
   // chunks are cut on the 16-byte grid of memory: the row begins `skip` elements into the first piece
   const int skip = (int)((uintptr_t)base % (VEC * SIZE)) / SIZE;
-  const int64_t id = ids[row * id_stride];
-  const bool has = id >= 0 && id < vocab;
-  const float given = has ? load1<DT>(base, id) : 0.0f;
 
   float v[E];
   int first[E / VEC];  // index of each piece's first value
@@ -129,26 +142,63 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const void* __restrict_
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[p * VEC + e] = w[e];
   }
-  float m = -__builtin_inff();
+  const int64_t id = ids[row * id_stride];
+  const bool has = id >= 0 && id < vocab;
+  const float given = has ? load1<DT>(base, id) : 0.0f;
+
+  float mine = -__builtin_inff();
 #pragma unroll
-  for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
-  m = wave_max(m);
-  if (lane == 0) fs[0][wave] = m;
+  for (int e = 0; e < E; ++e) mine = fmaxf(mine, v[e]);
+  float m = wave_max(mine);
+  // the wave's bound: the top-th largest of its lanes' maxima, bit by bit of its order key
+  float bound = -__builtin_inff();
+  if (top > 0) {
+    const uint32_t order = order_key(mine);
+    uint32_t key = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t next = key | 1u << bit;
+      if (__popcll(__ballot(order >= next)) >= top) key = next;
+    }
+    if (key) bound = value_of(key);
+  }
+  if (lane == 0) {
+    fs[0][wave] = m;
+    fs[3][wave] = bound;
+  }
+  if (tid == 0) count = 0;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, fs[0][w]);
+  for (int w = 0; w < WAVES; ++w) {
+    m = fmaxf(m, fs[0][w]);
+    bound = fmaxf(bound, fs[3][w]);
+  }
   // a chunk of -inf alone has Z = A = 0
   const float mm = m == -__builtin_inff() ? 0.0f : m;
   float z = 0.0f, a = 0.0f;
   int before = 0;
+  const bool plain = given > -__builtin_inff() && given < __builtin_inff();
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float d = v[e] - mm;
-    const float t = __expf(d);
-    z += t;
-    a += t == 0.0f ? 0.0f : t * d;  // also where d is -inf
-    const int i = first[e / VEC] + e % VEC;
-    before += i >= 0 && i < vocab && (v[e] > given || (v[e] == given && i < id));
+  for (int p = 0; p < E / VEC; ++p) {
+    const float than = first[p] + VEC <= id ? below(given) : given;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float y = v[p * VEC + e];
+      const float d = y - mm;  // before the change of base: m log2 e rounded would shift every weight alike
+      const float t = __builtin_amdgcn_exp2f(d * kLog2e);
+      z += t;
+      a = fmaf(t, fmaxf(d, -1000.0f), a);  // also where d is -inf; a NaN is in z
+      before += y > than;
+    }
+    if (!plain || (first[p] <= id && id < first[p] + VEC)) {  // the piece of the given token, or a given value that has no next one
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int i = first[p] + e;
+        const float y = v[p * VEC + e];
+        before -= y > than;
+        before += i >= 0 && i < vocab && (y > given || (y == given && i < id));
+      }
+    }
   }
   z = wave_sum(z);
   a = wave_sum(a);
@@ -158,27 +208,57 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const void* __restrict_
     fs[2][wave] = a;
     is[wave] = before;
   }
+  uint64_t* out = keys + (row * chunks + chunk) * top;
+  uint64_t* list = lds + kThreads;
+  if (top > 0) {
+    if (tid < top) out[tid] = 0;
+    // NaN is above everything: a thread's maximum does not show it
+    const bool odd = z != z;
+    if (mine >= bound || odd) {
+      uint32_t reach = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) reach |= (uint32_t)!(v[e] < bound) << e;
+      // (a value of the padding, -inf, reaches a bound of -inf only)
+#pragma unroll
+      for (int p = 0; p < E / VEC; ++p)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (first[p] < 0 || first[p] + VEC > vocab)
+            if (first[p] + e < 0 || first[p] + e >= vocab) reach &= ~(1u << (p * VEC + e));
+      int at = atomicAdd(&count, __popc(reach));
+      for (; reach; reach &= reach - 1, ++at) {
+        const int e = __ffs(reach) - 1, i = (int)((chunk * (E / VEC) + e / VEC) * kThreads * VEC + tid * VEC - skip) + e % VEC;
+        if (at < E * top) list[at] = full_key(load1<DT>(base, i), i);  // read again: few are
+      }
+    }
+  }
   __syncthreads();
   if (tid == 0) {
     Part p = {m, 0.0f, 0.0f, 0};
-    for (int w = 0; w < kThreads / 64; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       p.z += fs[1][w];
       p.a += fs[2][w];
       p.before += is[w];
     }
     parts[row * chunks + chunk] = p;
   }
-  if (top > 0) {
+  if (top == 0) return;
+  const int n = count;
+  if (n <= E * top) {
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t k = list[i];
+      int above = 0;
+      for (int j = 0; j < n; ++j) above += list[j] > k;
+      if (above < top) out[above] = k;
+    }
+  } else {  // uniform
     uint64_t key[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int i = first[e / VEC] + e % VEC;
       key[e] = i >= 0 && i < vocab ? full_key(v[e], i) : 0;
     }
-    uint64_t* out = keys + (row * chunks + chunk) * top;
-    if (tid < top) out[tid] = 0;
-    __syncthreads();  // before the keys that replace them
-    select_top(key, top, lds, lds + kThreads, [&](int place, uint64_t k) { out[place] = k; });
+    select_top(key, top, lds, list, [&](int place, uint64_t k) { out[place] = k; });
   }
 }
 
@@ -205,6 +285,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Part* __restrict_
       before += p[i].before;
       if (p[i].z == 0.0f) continue;  // -inf alone
       const float d = p[i].m - m, f = __expf(d);
+      if (f == 0.0f) continue;  // far below: z d may pass fp32's range
       z += p[i].z * f;
       a += (p[i].a + p[i].z * d) * f;
     }
@@ -233,36 +314,38 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Part* __restrict_
     const int64_t i = (int64_t)e * kThreads + tid;
     key[e] = i < n ? keys[row * n + i] : 0;
   }
-  // the value of a key, back from its order
   select_top(key, top, lds, lds + kThreads, [&](int place, uint64_t k) {
-    const uint32_t o = (uint32_t)(k >> 32);
-    const float v = o == 0xFFFFFFFFu ? __builtin_nanf("") : __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
-    top_logprobs[row * top + place] = v - m - lz;
+    top_logprobs[row * top + place] = value_of((uint32_t)(k >> 32)) - m - lz;
     top_ids[row * top + place] = (int32_t)(0xFFFFFFFFu - (uint32_t)k);
   });
 }
 
-constexpr int kPerThread = 32;  // values of a chunk a thread
+// values of a chunk a thread: 32, or 8 where chunks of 32 would not give every CU a workgroup
+int per_thread(int64_t rows, int64_t vocab) {
+  return rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) < gguf::device_cus() && vocab < (1 << 20) ? 8 : 32;
+}
 
-int64_t chunks_of(int64_t vocab) {  // one piece more: a row may begin inside a 16-byte piece
-  return (vocab + 7 + kThreads * kPerThread - 1) / (kThreads * kPerThread);
+int64_t chunks_of(int64_t rows, int64_t vocab) {  // one piece more: a row may begin inside a 16-byte piece
+  const int64_t size = kThreads * per_thread(rows, vocab);
+  return (vocab + 7 + size - 1) / size;
 }
 
 }  // namespace
 
 // the largest vocabulary whose chunks' best fit merge_kernel's registers
 int64_t logprobs_most_vocab(int64_t top) {
-  return top == 0 ? INT32_MAX - 65536 : (int64_t)(64 * kThreads / top) * kThreads * kPerThread - 8;
+  return top == 0 ? INT32_MAX - 65536 : (int64_t)(64 * kThreads / top) * kThreads * 32 - 8;
 }
 
 size_t logprobs_workspace(int64_t rows, int64_t vocab, int64_t top) {
-  return (size_t)rows * chunks_of(vocab) * (sizeof(Part) + top * sizeof(uint64_t));
+  return (size_t)rows * chunks_of(rows, vocab) * (sizeof(Part) + top * sizeof(uint64_t));
 }
 
 hipError_t launch_logprobs(const void* x, int dtype, int64_t stride, int64_t rows, int64_t vocab, const int64_t* ids,
                            int64_t id_stride, int top, float* logprobs, int32_t* ranks, float* entropy,
                            float* top_logprobs, int32_t* top_ids, void* ws, hipStream_t stream) {
-  const int64_t chunks = chunks_of(vocab);
+  const int64_t chunks = chunks_of(rows, vocab);
+  const int per = per_thread(rows, vocab);
   uint64_t* keys = (uint64_t*)ws;  // first: 8-byte aligned
   Part* parts = (Part*)(keys + rows * chunks * top);
   constexpr int64_t kRows = 65535;  // of a launch
@@ -273,9 +356,11 @@ hipError_t launch_logprobs(const void* x, int dtype, int64_t stride, int64_t row
     Part* pr = parts + r * chunks;
     uint64_t* kr = keys + r * chunks * top;
     const int64_t* ir = ids + r * id_stride;
-    const size_t lds = top ? (kThreads + (size_t)kPerThread * top) * 8 : 0;
-#define GGUF_DEC_CHUNK(DT) \
-  chunk_kernel<DT, kPerThread><<<dim3((unsigned)chunks, (unsigned)n), kThreads, lds, stream>>>(xr, stride, (int)vocab, ir, id_stride, top, pr, kr)
+    const size_t lds = top ? (kThreads + (size_t)per * top) * 8 : 0;
+    const dim3 grid((unsigned)chunks, (unsigned)n);
+#define GGUF_DEC_CHUNK(DT)                                                                                          \
+  if (per == 8) chunk_kernel<DT, 8><<<grid, kThreads, lds, stream>>>(xr, stride, (int)vocab, ir, id_stride, top, pr, kr); \
+  else chunk_kernel<DT, 32><<<grid, kThreads, lds, stream>>>(xr, stride, (int)vocab, ir, id_stride, top, pr, kr)
     GGUF_DEC_FLOATS(dtype, GGUF_DEC_CHUNK)
 #undef GGUF_DEC_CHUNK
     hipError_t e = hipGetLastError();
