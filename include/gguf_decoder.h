@@ -7,7 +7,8 @@
  *
  * Conventions, as in gguf_mi355x.h: plain pointers, sizes and strides; the caller gives outputs,
  * workspace and stream; the library allocates nothing, never synchronises the host and keeps no
- * state between calls. Every check that the host can make runs before any GPU access and returns
+ * state between calls. Rows that belong to no sequence (before cu_seqlens[0] or past its last offset) are left unwritten or
+ * unspecified. Every check that the host can make runs before any GPU access and returns
  * GGUF_DEC_EINVAL with a message in gguf_decoder_last_error() (per thread). What lies in device
  * memory (lengths, page numbers, slots, token ids) is checked by the kernels: a length is cut to what
  * its tensors hold, and what each entry point says happens for a page, slot or token id out of
@@ -89,7 +90,7 @@ GGUF_DEC_API int gguf_kv8_append(const gguf_kv8_cache* cache, const gguf_tensor*
 
 /* The cached values of positions starts[s] .. starts[s] + n_s - 1 of every sequence, as dense rows:
  * k_out and v_out [tokens, heads, d] (contiguous, fp32 / fp16 / bf16, 16-byte aligned). Positions
- * past the table's capacity, or in a page whose number is out of range, read as NaN.
+ * before 0 or past the table's capacity, or in a page whose number is out of range, read as NaN.
  * max_tokens: the largest n_s, a hint. */
 GGUF_DEC_API int gguf_kv8_read(const gguf_kv8_cache* cache, const gguf_tensor* block_table, const gguf_tensor* starts,
                                const gguf_tensor* cu_seqlens, int64_t max_tokens, const gguf_tensor* k_out,
@@ -120,7 +121,8 @@ GGUF_DEC_API int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cac
  * token; [seqs, m]: after each of its first m tokens, as a verify pass needs that may keep only some of
  * them; NULL: back to slots. A slot out of range keeps nothing, and a sequence of no tokens
  * copies its state to a [seqs] slot. No slot may be written twice, or written for one sequence and read
- * for another. out: [tokens, hv, dv] contiguous, in q's dtype.
+ * for another. out: [tokens, hv, dv] contiguous, in q's dtype. Token strides are at most 2^22 elements. In the
+ * chunked form a token that is not finite also makes NaN of its chunk's earlier outputs.
  * max_new: the largest n_s, a hint; the workspace is for sequences of more tokens than the recurrent form
  * takes (gguf_gated_delta_rule_workspace_bytes). */
 GGUF_DEC_API size_t gguf_gated_delta_rule_workspace_bytes(const gguf_tensor* q, const gguf_tensor* v, int64_t seqs,

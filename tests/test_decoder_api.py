@@ -167,6 +167,7 @@ def test_attention_refused(change, message):
     (dict(q=torch.zeros(3, 2, 96), k=torch.zeros(3, 2, 96)), "key head size 96"),
     (dict(v=torch.zeros(3, 4, 24), state=torch.zeros(5, 4, 24, 64)), "value head size 24"),
     (dict(v=torch.zeros(3, 3, 32)), "no multiple"),
+    (dict(v=torch.empty(2 * (1 << 23) + 128, dtype=torch.float32).as_strided((3, 4, 32), (1 << 23, 32, 1))), "2.22"),
     (dict(v=torch.zeros(3, 4, 33)[..., :32]), "16-byte aligned rows"),
     (dict(g=torch.zeros(3, 4, dtype=torch.bfloat16)), "g and beta"),
     (dict(beta=torch.zeros(3, 8)[:, ::2]), "g and beta"),

@@ -291,6 +291,8 @@ int gguf_gated_delta_rule(const gguf_tensor* q, const gguf_tensor* k, const gguf
   if (dv < 16 || dv % 16 || dv > 65536) return fail("%s: value head size %lld is not a multiple of 16", op, (long long)dv);
   if (hk < 1 || hv < 1 || hv % hk || hv > 65535) return fail("%s: %lld value heads are no multiple of %lld key heads", op, (long long)hv, (long long)hk);
   if (t > 0 && (!rows_ok(q) || !rows_ok(k) || !rows_ok(v))) return fail("%s: q, k and v need unit inner stride and 16-byte aligned rows", op);
+  if (hv * dv > (1 << 22) || (t > 1 && v->stride[0] > (1 << 22)))  // 64 rows are addressed by 32-bit byte offsets
+    return fail("%s: rows of v and out must be at most 2^22 elements apart", op);
   for (const gguf_tensor* x : {g, beta})
     if (!shaped(x, 2) || x->dtype != GGUF_DEC_F32 || x->size[0] != t || x->size[1] != hv || (hv > 1 && x->stride[1] != 1) || !aligned(x, 4))
       return fail("%s: g and beta must be fp32 [tokens, value heads] with unit inner stride", op);
