@@ -25,7 +25,7 @@ from vllm_gguf_plugin import decoder, ops  # noqa: E402,F401
 Q4_K, BLOCK = 12, 144  # ggml type id, bytes of 256 values
 HIDDEN, VOCAB = 1024, 4096
 HQ, HKV, D, PAGE = 12, 2, 128, 64          # attention layers
-HK, HV, DK, DV = 2, 6, 128, 128            # linear-attention layers
+HK, HV, DK, DV = 2, 8, 128, 128            # linear-attention layers
 
 
 class Linear:
