@@ -18,7 +18,10 @@ constexpr int kSegment = 64;  // tiles whose chunks are looked up at a time
 // that P stays within fp16's range whatever the scales are. P is rounded to fp16 (11 bits; the output
 // has 8 or 11), everything else is fp32.
 //
-// Bound: HBM for few rows. 2 bytes a (token, head, dim).
+// Bound: HBM, 2 bytes a (token, head, dim). Measured, 24 query and 4 KV heads of 256: 64 ragged sequences of up to
+// 16384 tokens 234 us (989 MB, 4.2 TB/s; before a wave's next tile was fetched ahead 444); one of 701 tokens 14 us,
+// latency. At head size 256 a workgroup takes 16 rows: 32 spill, and 8 sequences of 4 rows over up to 32768
+// tokens took 148 us with them, 104 with the cache read for two row tiles.
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   constexpr int S = D / 64, DD = D / 16;

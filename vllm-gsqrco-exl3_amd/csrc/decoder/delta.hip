@@ -37,7 +37,8 @@ __device__ __forceinline__ void load4(const void* p, int64_t i, float (&v)[4]) {
 // 64 c + 4 sub .. + 3. Rows are independent, so nothing leaves the wave. A token's two products with
 // the state, S k and S q, are summed over the 16 lanes together: S' q = S q + u (k . q), so the output need
 // not wait for the update.
-// Bound: HBM, the state in and out (2 x 64 KB a head of 128 x 128); at one sequence latency.
+// Bound: HBM, the state in and out (2 x 64 KB a head of 128 x 128); at one sequence latency. Measured, 48 heads of
+// 128 x 128: 32 sequences of 4 tokens with every state kept 104 us (508 MB, 4.9 TB/s), one token 8 us.
 template <int DT, int DK, int R>
 __global__ void __launch_bounds__(256) recurrent_kernel(DeltaArgs a, int most) {
   constexpr int P = DK / 64;
@@ -236,7 +237,7 @@ __device__ __forceinline__ void split4(const floatx4& x, uint2 (&planes)[P]) {
   }
 }
 
-// (chunk slot, v head): one workgroup
+// (chunk slot, v head): one workgroup. Measured: 168 us for the 128 chunks x 48 heads of an 8192-token prompt.
 template <int DT, int DK, int C>
 __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkWs ws) {
   typedef Layout<DT, DK, C> Lay;
@@ -445,7 +446,9 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
 // 8 consecutive values of step s of a right operand, so planes are written as they are read, 16
 // bytes a lane; only the left operands' rows are taken in that order.
 //
-// Bound: for one sequence of 48 heads, the latency of the chain S k -> X -> U -> S through a chunk.
+// Bound: for one sequence of 48 heads (192 workgroups), the fetch of a chunk's 64 KB of operands, which arrive at some
+// 25 bytes a cycle and CU, then the chain S k -> X -> U -> S. Measured: 472 us for 8192 tokens, 3.7 us a chunk; one wave
+// for 16 columns, without the barriers but with all of a chunk's work on one SIMD, took 650.
 template <int DT, int DK, int C>
 __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kernel(DeltaArgs a, int most, ChunkWs ws) {
   typedef Layout<DT, DK, C> Lay;

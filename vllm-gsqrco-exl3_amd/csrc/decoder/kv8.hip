@@ -32,7 +32,8 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
 // magnitude (as bits of |x|: unsigned order puts inf and NaN on top, so they reach the scale), then,
 // where the scale grew, the older codes, then the new ones. The second read of the values is from L2.
 //
-// Bound: HBM, 2 B in and 1 B out a value; at a token a sequence the launch's latency.
+// Bound: HBM, 2 B in and 1 B out a value; at a token a sequence the launch's latency. Measured with kv8_read:
+// 8192 tokens of 4 heads of 256 in bf16 35 us, 101 MB, 2.9 TB/s; 32 sequences of one token 13 us.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) append_kernel(Kv8 c, const void* __restrict__ key, int64_t kt, int64_t kh,
                                                           const void* __restrict__ value, int64_t vt, int64_t vh,
