@@ -46,6 +46,7 @@ struct Layout {
   static constexpr int KR = DK + 8;                                // row length of keys and queries
   // bytes: keys [NK][C][KR], queries alike; whole KB
   static constexpr int kK = 0, kQ = NK * C * KR * 2, kKq = (2 * kQ + 1023) / 1024 * 1024;
+  static constexpr int kPrep = NK * C * KR * 2 > C * (C + 4) * 4 ? NK * C * KR * 2 : C * (C + 4) * 4;  // half of prep_kernel's LDS
   // T and A in fp32, by steps of 32 columns, of which step s has the rows from 32 s on (above they are 0):
   // row i, column j lies at kTt + 4 tri(i, j)
   static constexpr int RS = 36;

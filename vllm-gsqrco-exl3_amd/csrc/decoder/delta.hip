@@ -244,10 +244,11 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
   constexpr int NK = Lay::NK, CT = C / 16;
   constexpr int KR = Lay::KR;
   extern __shared__ __align__(16) char lds[];
-  __bf16* kp = (__bf16*)lds;                 // [NK][C][KR], then q alike
-  __bf16* qp = kp + NK * C * KR;
-  float* L = (float*)(qp + NK * C * KR);     // [C][C + 4]
-  float* T = L + C * (C + 4);                // [C][C + 4]
+  // [NK][C][KR] keys, then queries; once they are multiplied, T and L [C][C + 4] in their places, so that four
+  // workgroups share a CU
+  __bf16* kp = (__bf16*)lds;
+  __bf16* qp = (__bf16*)(lds + Lay::kPrep);
+  float *T = (float*)kp, *L = (float*)qp;
   __shared__ double G[C];
   __shared__ float beta[C], rk[C], rq[C];
   constexpr int LS = C + 4;
@@ -345,12 +346,13 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
     }
   }
 
-  // k k^T and q k^T, 16 rows a wave (and turn)
+  // k k^T and q k^T, 16 rows a wave
   float* Ap = (float*)(tp + Lay::kA);
-  for (int it = wave; it < CT; it += 4) {
-    floatx4 kk[CT], qk[CT];
+  const int it = wave;
+  floatx4 kk[CT], qk[CT];
 #pragma unroll
-    for (int jt = 0; jt < CT; ++jt) kk[jt] = qk[jt] = floatx4{0, 0, 0, 0};
+  for (int jt = 0; jt < CT; ++jt) kk[jt] = qk[jt] = floatx4{0, 0, 0, 0};
+  if (it < CT) {
 #pragma unroll
     for (int s = 0; s < DK / 32; ++s) {
       bf16x8 ka[NK], qa[NK];
@@ -373,6 +375,9 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
         }
       }
     }
+  }
+  __syncthreads();
+  if (it < CT) {
 #pragma unroll
     for (int jt = 0; jt < CT; ++jt)
 #pragma unroll
@@ -656,7 +661,7 @@ hipError_t launch(const DeltaArgs& a, int64_t max_new, void* wsp, hipStream_t st
   typedef Layout<DT, DK, C> Lay;
   const int64_t slots = a.rows.tokens / C + a.rows.seqs;
   ChunkWs ws{(char*)wsp, (char*)wsp + slots * a.hk * Lay::kKq};
-  constexpr int prep_lds = Lay::NK * C * Lay::KR * 4 + 2 * C * (C + 4) * 4, scan_lds = Lay::kLds;
+  constexpr int prep_lds = 2 * Lay::kPrep, scan_lds = Lay::kLds;
   int dev = 0;
   if ((e = hipGetDevice(&dev)) != hipSuccess) return e;
   struct Tag {};
