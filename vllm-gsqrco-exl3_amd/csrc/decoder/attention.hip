@@ -29,7 +29,6 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   __shared__ float stat[kWaves][NT * 16][2];
   __shared__ Chunk chunks[4 * kSegment];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const int seqs = a.rows.seqs;
   // row tiles of one (sequence, head, split) read the same tokens: a stride of gridDim.x apart, they run on as few XCDs as
   // there are, and share their L2. Later splits, which short sequences do not have, come last.
   const int head = blockIdx.x % a.c.heads, seq = blockIdx.x / a.c.heads % a.rows.seqs;

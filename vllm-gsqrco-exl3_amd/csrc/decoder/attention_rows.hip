@@ -14,7 +14,7 @@
 // next to the matrix cores, and K needs no conversion.
 // V is converted to fp16 once a workgroup, from registers to LDS.
 //
-// Measured, 24 query and 4 KV heads of 256: 2048 rows at positions up to 8192 624 us, 578 TFLOP/s (1453 us in the
+// Measured, 24 query and 4 KV heads of 256: 2048 rows at positions up to 8192 637 us, 567 TFLOP/s (1453 us in the
 // form for few rows). A wave's turn (32 rows, 32 tokens) is some 3,100 cycles, 1,024 of them MFMAs: the softmax and
 // the operand reads are not hidden, with one wave a SIMD (D = 256: 128 accumulator and 64 query registers; two
 // workgroups a CU spill, 1,065 us).

@@ -17,7 +17,6 @@ namespace gguf_dec {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTopMax = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // order-preserving: a < b as floats <=> key(a) < key(b); -0 = +0; NaN above +inf
@@ -55,7 +54,7 @@ __device__ __forceinline__ int wave_sum(int v) {
   return v;
 }
 
-// The k (<= kTopMax) largest of the workgroup's keys, E a thread (0: none; all others distinct), as emit(place, key) for
+// The k largest of the workgroup's keys, E a thread (0: none; all others distinct), as emit(place, key) for
 // places 0 .. ; fewer where there are fewer. list: E * k keys of LDS, most: kThreads.
 template <int E, class F>
 __device__ __forceinline__ void select_top(const uint64_t (&key)[E], int k, uint64_t* most, uint64_t* list, F&& emit) {
