@@ -141,3 +141,15 @@ def test_other_stream_and_graph(dec):
     assert all(torch.equal(a, b) for a, b in zip(ref, got))
     for i in range(5):
         graph_replays_equal(lambda: dec.token_logprobs(x, ids, 20)[i], ref[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,vocab,top", [(1, 524289, 64), (1, 600000, 64), (3, 600000, 64), (1, 1048575, 33),
+                                            (1, 1040000, 16), (2, 1100000, 64)])
+def test_wide_rows_with_many_best(dec, rows, vocab, top, dtype):
+    """So many chunks that their best are more than a merge of small chunks would hold; the best tokens in the last
+    columns."""
+    g = torch.Generator().manual_seed(47)
+    x = torch.randn(rows, vocab, generator=g)
+    x[:, -top:] += 20
+    _check(dec, x.to(dtype).cuda(), torch.randint(vocab - top, vocab, (rows,), generator=g).cuda(), top)

@@ -322,32 +322,39 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Part* __restrict_
   });
 }
 
-// values of a chunk a thread: 32, or 8 where chunks of 32 would not give every CU a workgroup
-int per_thread(int64_t rows, int64_t vocab) {
-  return rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) < gguf::device_cus() && vocab < (1 << 20) ? 8 : 32;
+constexpr int kMergeMost = 64;  // keys a thread of merge_kernel, at most
+
+int64_t chunks_of(int64_t vocab, int per) {  // one piece more: a row may begin inside a 16-byte piece
+  const int64_t size = (int64_t)kThreads * per;
+  return (vocab + 7 + size - 1) / size;
 }
 
-int64_t chunks_of(int64_t rows, int64_t vocab) {  // one piece more: a row may begin inside a 16-byte piece
-  const int64_t size = kThreads * per_thread(rows, vocab);
-  return (vocab + 7 + size - 1) / size;
+// values of a chunk a thread: 32, or 8 where chunks of 32 would not give every CU a workgroup and the best of the
+// smaller ones, four times as many, still fit merge_kernel
+int per_thread(int64_t rows, int64_t vocab, int64_t top) {
+  return rows * chunks_of(vocab, 32) < gguf::device_cus() && vocab < (1 << 20) &&
+                 chunks_of(vocab, 8) * top <= kMergeMost * kThreads
+             ? 8
+             : 32;
 }
 
 }  // namespace
 
-// the largest vocabulary whose chunks' best fit merge_kernel's registers
+// the largest vocabulary whose chunks of 32 values a thread leave no more keys than merge_kernel holds
 int64_t logprobs_most_vocab(int64_t top) {
-  return top == 0 ? INT32_MAX - 65536 : (int64_t)(64 * kThreads / top) * kThreads * 32 - 8;
+  return top == 0 ? INT32_MAX - 65536 : (int64_t)(kMergeMost * kThreads / top) * kThreads * 32 - 8;
 }
 
 size_t logprobs_workspace(int64_t rows, int64_t vocab, int64_t top) {
-  return (size_t)rows * chunks_of(rows, vocab) * (sizeof(Part) + top * sizeof(uint64_t));
+  return (size_t)rows * chunks_of(vocab, per_thread(rows, vocab, top)) * (sizeof(Part) + top * sizeof(uint64_t));
 }
 
 hipError_t launch_logprobs(const void* x, int dtype, int64_t stride, int64_t rows, int64_t vocab, const int64_t* ids,
                            int64_t id_stride, int top, float* logprobs, int32_t* ranks, float* entropy,
                            float* top_logprobs, int32_t* top_ids, void* ws, hipStream_t stream) {
-  const int64_t chunks = chunks_of(rows, vocab);
-  const int per = per_thread(rows, vocab);
+  const int per = per_thread(rows, vocab, top);
+  const int64_t chunks = chunks_of(vocab, per);
+  if (chunks * top > kMergeMost * kThreads) return hipErrorInvalidValue;  // past logprobs_most_vocab
   uint64_t* keys = (uint64_t*)ws;  // first: 8-byte aligned
   Part* parts = (Part*)(keys + rows * chunks * top);
   constexpr int64_t kRows = 65535;  // of a launch
@@ -377,7 +384,7 @@ hipError_t launch_logprobs(const void* x, int dtype, int64_t stride, int64_t row
     } else if (each <= 8) {
       GGUF_DEC_MERGE(8);
     } else {
-      GGUF_DEC_MERGE(64);
+      GGUF_DEC_MERGE(kMergeMost);
     }
 #undef GGUF_DEC_MERGE
     if ((e = hipGetLastError()) != hipSuccess) return e;
