@@ -153,3 +153,24 @@ def test_wide_rows_with_many_best(dec, rows, vocab, top, dtype):
     x = torch.randn(rows, vocab, generator=g)
     x[:, -top:] += 20
     _check(dec, x.to(dtype).cuda(), torch.randint(vocab - top, vocab, (rows,), generator=g).cuda(), top)
+
+
+@pytest.mark.parametrize("rows", [2, 70])  # chunks of 2048 and of 8192 columns
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("kind", ["among masked", "chunks of NaN", "far below"])
+def test_a_nan_far_from_the_maximum(dec, kind, dtype, rows):
+    """A NaN whose chunk has nothing that counts beside the row's maximum makes the row NaN all the same."""
+    g = torch.Generator().manual_seed(48)
+    x = torch.randn(rows, 30000, generator=g)
+    first = 20000
+    if kind == "chunks of NaN":
+        first = 8000
+        x[0, first:] = torch.nan
+    else:
+        x[0, 8000:] = -torch.inf if kind == "among masked" else -200.0
+        x[0, first] = torch.nan
+    x = x.to(dtype).cuda()
+    ids = torch.full((rows,), 3).cuda()
+    lp, _, ent, tlp, tid = dec.token_logprobs(x, ids, 3)
+    assert lp[0].isnan() and ent[0].isnan() and tlp[0].isnan().all() and int(tid[0, 0]) == first
+    _check(dec, x[1:], ids[1:], 3)

@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Part* __restrict_
       before += p[i].before;
       if (p[i].z == 0.0f) continue;  // -inf alone
       const float d = p[i].m - m, f = __expf(d);
-      if (f == 0.0f) continue;  // far below: z d may pass fp32's range
+      if (f == 0.0f && p[i].z == p[i].z) continue;  // far below: z d may pass fp32's range. A NaN, which m does not show, stays
       z += p[i].z * f;
       a += (p[i].a + p[i].z * d) * f;
     }
