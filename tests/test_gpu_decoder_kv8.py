@@ -412,3 +412,17 @@ def test_append_and_read_in_a_graph(dec):
         return dec.kv8_read(cache, table, starts, cu_read, 80, 50)[1]
 
     graph_replays_equal(step, step())
+
+
+def _near(y, ref, most):
+    """_close, and no NaN (which compares as not beyond any bound)."""
+    assert not y.isnan().any()
+    _close(y, ref, most)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("news", [(2, 9), (2, 150)], ids=str)
+def test_attention_negative_scale(dec, dtype, news):
+    """A scale below 0, with scores some 50 apart, in the form for few rows and in that for many."""
+    q, cache, table, y = _run_attention(dec, (300, 400), news, 6, 2, 128, 16, dtype, 27, scale=-1.0)
+    _near(y, *_attention_ref(q, cache, table, (300, 400), news, -1.0))

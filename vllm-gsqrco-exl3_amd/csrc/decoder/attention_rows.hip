@@ -119,8 +119,9 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
       big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
       const float amax = __uint_as_float(big);  // NaN and inf on top: then the row's scores are NaN
       // a row of magnitudes below 2^-100 has scores of 0
-      const float inv = amax >= 0x1p-100f && amax < __builtin_inff() ? 16256.0f / amax : 0.0f;
-      qs = amax < __builtin_inff() ? a.scale * (amax * (1.0f / 16256.0f)) : __builtin_nanf("");
+      const float inv = amax >= 0x1p-100f && amax < __builtin_inff() ? (a.scale < 0.0f ? -16256.0f : 16256.0f) / amax : 0.0f;
+      // not negative (the scale's sign is Q's), so that the largest product is the largest score
+      qs = amax < __builtin_inff() ? fabsf(a.scale) * (amax * (1.0f / 16256.0f)) : __builtin_nanf("");
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
