@@ -223,3 +223,38 @@ def test_fake_implementations_have_the_ops_shapes():
         assert o.shape == (3, 4, 32)
         out = decoder.token_logprobs(empty(3, 100), empty(3, dtype=torch.int64), 7)
         assert [tuple(x.shape) for x in out] == [(3,), (3,), (3,), (3, 7), (3, 7)]
+
+
+@pytest.mark.parametrize("hint", [2 ** 62, 2 ** 63 - 1])
+def test_hints_beyond_every_size_are_no_trouble(hint):
+    """max_new, max_len and max_tokens may be any number: what the tensors hold bounds them before any arithmetic."""
+    c = _cache()
+    for call in (lambda: _kv(max_new=hint), lambda: _read(max_tokens=hint), lambda: _attention(max_new=hint, max_len=hint),
+                 lambda: _attention(query=torch.zeros(3, 8, 64, dtype=torch.float16), max_new=hint, max_len=6),
+                 lambda: _delta(max_new=hint)):
+        with pytest.raises(RuntimeError, match="must be CUDA tensors"):
+            call()
+
+    class T(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("ndim", ctypes.c_int32),
+                    ("size", ctypes.c_int64 * 4), ("stride", ctypes.c_int64 * 4), ("device", ctypes.c_int32)]
+
+    class Cache(ctypes.Structure):
+        _fields_ = [("k", T), ("v", T), ("k_scale", T), ("v_scale", T)]
+
+    def desc(t, dtype):
+        r = T(t.data_ptr(), dtype, t.dim())
+        r.size[:t.dim()], r.stride[:t.dim()], r.device = list(t.shape), list(t.stride()), -1
+        return r
+
+    lib = ctypes.CDLL(decoder.LIB_PATH)
+    lib.gguf_kv8_attention_workspace_bytes.restype = ctypes.c_size_t
+    cache = Cache(*(desc(t, d) for t, d in zip(c, (5, 5, 0, 0))))
+    q = desc(torch.zeros(3, 8, 64, dtype=torch.float16), 1)
+
+    def workspace(max_new, max_len):
+        return lib.gguf_kv8_attention_workspace_bytes(ctypes.byref(cache), ctypes.byref(q), ctypes.c_int64(2),
+                                                      ctypes.c_int64(max_new), ctypes.c_int64(max_len))
+
+    assert workspace(hint, 6) == workspace(3, 6)
+    assert 0 < workspace(hint, hint) == workspace(3, 2 ** 31 - 1)

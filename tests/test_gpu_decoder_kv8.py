@@ -426,3 +426,16 @@ def test_attention_negative_scale(dec, dtype, news):
     """A scale below 0, with scores some 50 apart, in the form for few rows and in that for many."""
     q, cache, table, y = _run_attention(dec, (300, 400), news, 6, 2, 128, 16, dtype, 27, scale=-1.0)
     _near(y, *_attention_ref(q, cache, table, (300, 400), news, -1.0))
+
+
+@pytest.mark.parametrize("hint", [2 ** 62, 2 ** 63 - 1])
+def test_hints_beyond_every_size(dec, hint):
+    g = torch.Generator().manual_seed(33)
+    for news in ((1, 2), (70, 3)):
+        for hq in (6, 8):
+            q, cache, table, y = _run_attention(dec, (300, 1000), news, hq, 2, 128, 16, torch.bfloat16, 14, hint, hint)
+            _near(y, *_attention_ref(q, cache, table, (300, 1000), news, 128 ** -0.5))
+    k, v = (torch.randn(5, 2, 128, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    _check_append(dec, cache, k, v, table, (300, 1000), (2, 3), max_new=hint)
+    k, _ = dec.kv8_read(cache, table, _i32(0, 0), _cu((300, 20)), 320, hint, torch.float32)
+    assert torch.equal(k[:300], _values(cache, table, 0, 300)[0].transpose(0, 1).float())

@@ -100,6 +100,9 @@ bool rows_ok(const gguf_tensor* t) {
          stride_of(t, 1) * es % 16 == 0;
 }
 
+// a hint as the launch takes it: at least 1 and at most what there can be, so that no arithmetic on it overflows
+int64_t bounded(int64_t hint, int64_t most) { return hint > most ? (most < 1 ? 1 : most) : hint < 1 ? 1 : hint; }
+
 struct DeviceScope {
   int prev = -1;
   hipError_t err = hipSuccess;
@@ -195,7 +198,7 @@ int gguf_kv8_append(const gguf_kv8_cache* cache, const gguf_tensor* key, const g
   if (scope.err != hipSuccess) return hip_fail(scope.err, op);
   const hipError_t e = gguf_dec::launch_kv8_append(c, key->dtype, key->data, stride_of(key, 0), stride_of(key, 1), value->data,
                                                    stride_of(value, 0), stride_of(value, 1), (const int32_t*)seq_lens->data, rows,
-                                                   max_new < 1 ? 1 : max_new, (hipStream_t)stream);
+                                                   bounded(max_new, key->size[0]), (hipStream_t)stream);
   return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
 }
 
@@ -220,7 +223,7 @@ int gguf_kv8_read(const gguf_kv8_cache* cache, const gguf_tensor* block_table, c
   if (k_out->size[0] == 0) return GGUF_DEC_OK;
   const DeviceScope scope(k_out->device);
   if (scope.err != hipSuccess) return hip_fail(scope.err, op);
-  const hipError_t e = gguf_dec::launch_kv8_read(c, k_out->dtype, (const int32_t*)starts->data, rows, max_tokens < 1 ? 1 : max_tokens,
+  const hipError_t e = gguf_dec::launch_kv8_read(c, k_out->dtype, (const int32_t*)starts->data, rows, bounded(max_tokens, k_out->size[0]),
                                                  k_out->data, v_out->data, (hipStream_t)stream);
   return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
 }
@@ -232,7 +235,7 @@ size_t gguf_kv8_attention_workspace_bytes(const gguf_kv8_cache* cache, const ggu
     return 0;
   const DeviceScope scope(query->device < 0 ? 0 : query->device);
   return gguf_dec::kv8_attention_workspace((int)cache->k.size[3], (int)cache->k.size[1], (int)query->size[1],
-                                           query->size[0], seqs, max_new < 1 ? 1 : max_new, max_len < 1 ? 1 : max_len);
+                                           query->size[0], seqs, bounded(max_new, query->size[0]), bounded(max_len, INT_MAX));
 }
 
 int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, const gguf_tensor* block_table,
@@ -264,7 +267,7 @@ int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, co
   if (scope.err != hipSuccess) return hip_fail(scope.err, op);
   const hipError_t e = gguf_dec::launch_kv8_attention(
       c, query->dtype, query->data, stride_of(query, 0), stride_of(query, 1), (int)query->size[1], (const int32_t*)seq_lens->data,
-      rows, max_new < 1 ? 1 : max_new, max_len < 1 ? 1 : max_len, scale, out->data, workspace, workspace ? workspace_bytes : 0,
+      rows, bounded(max_new, query->size[0]), bounded(max_len, INT_MAX), scale, out->data, workspace, workspace ? workspace_bytes : 0,
       (hipStream_t)stream);
   return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
 }
