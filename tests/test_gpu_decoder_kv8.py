@@ -439,3 +439,21 @@ def test_hints_beyond_every_size(dec, hint):
     _check_append(dec, cache, k, v, table, (300, 1000), (2, 3), max_new=hint)
     k, _ = dec.kv8_read(cache, table, _i32(0, 0), _cu((300, 20)), 320, hint, torch.float32)
     assert torch.equal(k[:300], _values(cache, table, 0, 300)[0].transpose(0, 1).float())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("hq,heads,d", [(6, 2, 128), (6, 1, 256)])
+@pytest.mark.parametrize("news", [3, 8, 70])
+def test_attention_large_v_scale_unseen(dec, news, hq, heads, d, dtype):
+    """A page of far larger values takes nothing from the rows before it, which share its tile but do not see it."""
+    g = torch.Generator().manual_seed(28)
+    end, page = 97, 16
+    cache = _random_cache(dec, 9, heads, page, d, g)
+    table = _table((end,), page, 9, g)
+    cache.v_scale[table[0, end // page].long()] = 2.0 ** 40  # the last token's page, which the last row alone sees
+    q = (torch.randn(news, hq, d, generator=g) * 0.3).to(dtype).cuda()
+    y = dec.kv8_attention(q, cache, table, _i32(end), _cu((news,)), news, end)
+    ref, most = _attention_ref(q, cache, table, (end,), (news,), d ** -0.5)
+    _near(y[:-1], ref[:-1], most[:-1])
+    if dtype == torch.bfloat16:  # (past fp16's range)
+        _near(y[-1:], ref[-1:], most[-1:])

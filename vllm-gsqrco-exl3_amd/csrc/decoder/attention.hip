@@ -14,8 +14,8 @@ constexpr int kSegment = 64;  // tiles whose chunks are looked up at a time
 // operand registers (each byte is read by one lane, so LDS would only add a hop), with statistics and
 // accumulators of their own, joined through LDS at the end. Softmax is online: a wave keeps, for each row, the maximum m so
 // far, its lanes' sums of 2^(s - m), and O scaled to m.
-// The scale of a V chunk goes into P: p * vs / ref, where ref is the largest vs the wave has met, so
-// that P stays within fp16's range whatever the scales are. P is rounded to fp16 (11 bits; the output
+// The scale of a V chunk goes into P: p * vs / ref, where ref is the largest vs of the chunks that the row has met and
+// sees, so that P stays within fp16's range whatever the scales are, and what a row does not see takes no bits from it. P is rounded to fp16 (11 bits; the output
 // has 8 or 11), everything else is fp32.
 //
 // Bound: HBM, 2 bytes a (token, head, dim). Measured, 24 query and 4 KV heads of 256: 64 ragged sequences of up to
@@ -104,12 +104,12 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
 
     floatx4 o[DD][NT];
     float m[NT], l[NT];
-    float ref = 0.0f, inv_ref = 0.0f;
+    float ref[NT], inv_ref[NT];
     int seg = tb;  // chunks[0] is of this tile
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = kNoScore;
-      l[t] = 0.0f;
+      l[t] = ref[t] = inv_ref[t] = 0.0f;
 #pragma unroll
       for (int i = 0; i < DD; ++i) o[i][t] = floatx4{0, 0, 0, 0};
     }
@@ -150,10 +150,9 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
       }
       load_k(then);
 
-      const float top = group_max(vs);
       const bool masked = kTile * tile + kTile - 1 > all;
-      float nm[NT];
-      bool grown = top > ref;
+      float nm[NT], own[NT];  // own: the V scale of the lane's chunk, if the row sees it
+      bool grown = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float f = qs[t] * ks;
@@ -171,15 +170,16 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
         // where the largest V scale grew
         mx = group_max(mx);
         nm[t] = mx > m[t] + 8.0f ? mx : m[t];
-        grown = grown || nm[t] != m[t];
+        own[t] = masked && kTile * tile + 16 * g > last[t] ? 0.0f : vs;
+        grown = grown || nm[t] != m[t] || own[t] > ref[t];
       }
       if (__any(grown)) {
-        const float nref = fmaxf(ref, top);
-        const float shrink = nref > ref ? ref / nref : 1.0f;
-        ref = nref;
-        inv_ref = ref > 0.0f ? 1.0f / ref : 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+          const float nref = fmaxf(ref[t], group_max(own[t]));
+          const float shrink = nref > ref[t] ? ref[t] / nref : 1.0f;
+          ref[t] = nref;
+          inv_ref[t] = nref > 0.0f ? 1.0f / nref : 0.0f;
           const float al = __builtin_amdgcn_exp2f(m[t] - nm[t]);
           m[t] = nm[t];
           l[t] *= al;
@@ -187,10 +187,10 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
           for (int i = 0; i < DD; ++i) o[i][t] *= al * shrink;
         }
       }
-      const float vr = vs * inv_ref;
       half8 p[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        const float vr = vs * inv_ref[t];
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < DD; ++i)
-        *(floatx4*)(lds + ((((size_t)wave * DD + i) * NT + t) * 64 + lane) * 4) = o[i][t] * ref;
+        *(floatx4*)(lds + ((((size_t)wave * DD + i) * NT + t) * 64 + lane) * 4) = o[i][t] * ref[t];
     }
     __syncthreads();
     for (int i = wave; i < DD; i += kWaves) {

@@ -253,8 +253,9 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
       // here: K of t + 1 and V of t in LDS, K of t + 2 and V of t + 1 in registers
 
       // the rows' statistics
-      const float top = fmaxf(x0.vs[0], x0.vs[1]);  // a NaN counts for nothing
       const int seen = last - (kToks * t + 8 * h);  // place 16 c + e of the lane is seen if it is at most this
+      // the largest V scale of the chunks that the row sees; a NaN counts for nothing
+      const float top = fmaxf(!kMasked || last >= kToks * t ? x0.vs[0] : 0.0f, !kMasked || last >= kToks * t + 16 ? x0.vs[1] : 0.0f);
       const float f[2] = {qs * x0.ks[0], qs * x0.ks[1]};
       float mx = kNoScore;
 #pragma unroll
