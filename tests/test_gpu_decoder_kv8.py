@@ -457,3 +457,27 @@ def test_attention_large_v_scale_unseen(dec, news, hq, heads, d, dtype):
     _near(y[:-1], ref[:-1], most[:-1])
     if dtype == torch.bfloat16:  # (past fp16's range)
         _near(y[-1:], ref[-1:], most[-1:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("news", [1, 70])
+def test_attention_many_small_weights(dec, news, dtype):
+    """Half a million tokens of 2^-26 of the first one's weight each, which together are a hundredth of the sum; the first one's
+    value is 0."""
+    n, d, page = 1 << 19, 64, 256
+    cache = dec.Kv8Cache.empty(n // page, 1, page, d)
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda")[None]
+    cache.k[0, 0, 0] = 127
+    g = torch.Generator(device="cuda").manual_seed(29)
+    cache.v.copy_(torch.randint(90, 110, cache.v.shape, device="cuda", generator=g))
+    cache.v[0, 0, :, 0] = 0
+    cache.k_scale.fill_(26 * math.log(2) / (127 * d * 0.125))
+    cache.v_scale.fill_(1 / 127)
+    q = torch.ones(news, 1, d, dtype=dtype, device="cuda")
+    y = dec.kv8_attention(q, cache, table, _i32(n), _cu((news,)), news, 1)  # (one split)
+    k, v = _values(cache, table, 0, n)
+    w = torch.exp((k[0, :, 0] - k[0, 0, 0]) * d * 0.125)  # all queries are ones, and a key's values alike
+    for i in (0, news - 1):
+        see = n - news + i + 1
+        ref = (w[:see] @ v[0, :see]) / w[:see].sum()
+        _near(y[i], ref[None], v.abs().max())

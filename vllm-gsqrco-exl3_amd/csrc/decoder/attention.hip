@@ -14,7 +14,7 @@ constexpr int kSegment = 64;  // tiles whose chunks are looked up at a time
 // operand registers (each byte is read by one lane, so LDS would only add a hop), with statistics and
 // accumulators of their own, joined through LDS at the end. Softmax is online: a wave keeps, for each row, the maximum m so
 // far, its lanes' sums of 2^(s - m), and O scaled to m.
-// The scale of a V chunk goes into P: p * vs / ref, where ref is the largest vs of the chunks that the row has met and
+// The scale of a V chunk goes into P: p * kWeight * vs / ref, where ref is the largest vs of the chunks that the row has met and
 // sees, so that P stays within fp16's range whatever the scales are, and what a row does not see takes no bits from it. P is rounded to fp16 (11 bits; the output
 // has 8 or 11), everything else is fp32.
 //
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
           const float nref = fmaxf(ref[t], group_max(own[t]));
           const float shrink = nref > ref[t] ? ref[t] / nref : 1.0f;
           ref[t] = nref;
-          inv_ref[t] = nref > 0.0f ? 1.0f / nref : 0.0f;
+          inv_ref[t] = nref > 0.0f ? kWeight / nref : 0.0f;
           const float al = __builtin_amdgcn_exp2f(m[t] - nm[t]);
           m[t] = nm[t];
           l[t] *= al;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < DD; ++i)
-        *(floatx4*)(lds + ((((size_t)wave * DD + i) * NT + t) * 64 + lane) * 4) = o[i][t] * ref[t];
+        *(floatx4*)(lds + ((((size_t)wave * DD + i) * NT + t) * 64 + lane) * 4) = o[i][t] * (ref[t] / kWeight);
     }
     __syncthreads();
     for (int i = wave; i < DD; i += kWaves) {

@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
         for (int i = 0; i < DD; ++i) o[i] *= by;
         m = nm;
         ref = nref;
-        inv_ref = ref > 0.0f ? 1.0f / ref : 0.0f;
+        inv_ref = ref > 0.0f ? kWeight / ref : 0.0f;
       }
 
       // from here on straight, for the scheduler: tile t + 1's K beside the weights
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
 
     l += __shfl_xor(l, 32, 64);
     if (orow >= 0) {
-      const float inv = splits == 1 ? (l == 0.0f ? 0.0f : ref / l) : ref;
+      const float by = ref / kWeight, inv = splits == 1 ? (l == 0.0f ? 0.0f : by / l) : by;
 #pragma unroll
       for (int i = 0; i < DD; ++i)
 #pragma unroll
