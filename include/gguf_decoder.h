@@ -67,8 +67,8 @@ typedef struct gguf_tensor {
  *   v        int8 [pages, heads, d, page]     (tokens innermost: the order in which attention's
  *                                              second product takes them)
  *   k_scale  fp32 [pages, heads], v_scale fp32 [pages, heads]      contiguous
- * d is 64, 128, 192 or 256. A sequence's tokens 0 .. len - 1 lie in the pages block_table[s, 0 ..]
- * (int32 [seqs, max_pages], unit inner stride). */
+ * A V scale below 2^-100 counts as 0 in attention. d is 64, 128, 192 or 256. A sequence's tokens
+ * 0 .. len - 1 lie in the pages block_table[s, 0 ..] (int32 [seqs, max_pages], unit inner stride). */
 typedef struct gguf_kv8_cache {
   gguf_tensor k, v, k_scale, v_scale;
 } gguf_kv8_cache;

@@ -481,3 +481,21 @@ def test_attention_many_small_weights(dec, news, dtype):
         see = n - news + i + 1
         ref = (w[:see] @ v[0, :see]) / w[:see].sum()
         _near(y[i], ref[None], v.abs().max())
+
+
+@pytest.mark.parametrize("news", [2, 70])
+def test_attention_v_scales_below_the_least(dec, news):
+    """V scales below 2^-100, which kv8_append never leaves, count as 0 here too, alone and among others."""
+    g = torch.Generator().manual_seed(34)
+    heads, page, d, end = 2, 16, 128, 200
+    cache = _random_cache(dec, 14, heads, page, d, g)
+    table = _table((end,), page, 14, g)
+    q = (torch.randn(news, 6, d, generator=g) * 0.3).to(torch.bfloat16).cuda()
+    for every in (True, False):
+        cache.v_scale[::1 if every else 2] = 1e-40
+        y = dec.kv8_attention(q, cache, table, _i32(end), _cu((news,)), news, end)
+        if every:
+            assert (y == 0).all()
+            cache.v_scale.fill_(0.01)
+        else:
+            _near(y, *_attention_ref(q, cache, table, (end,), (news,), d ** -0.5))

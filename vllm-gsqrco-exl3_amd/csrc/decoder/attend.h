@@ -79,6 +79,7 @@ __device__ __forceinline__ Chunk chunk_of(const Kv8& c, const int32_t* table, in
   r.ks = ok ? c.ks[r.ph] : none;
   r.vs = ok ? c.vs[r.ph] : none;
   if (!(r.vs <= 3.0e38f)) r.vs = __builtin_nanf("");
+  if (fabsf(r.vs) < kLeastScale) r.vs = 0.0f;
   return r;
 }
 

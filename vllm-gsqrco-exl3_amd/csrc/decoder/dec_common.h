@@ -19,6 +19,9 @@ typedef short short8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
+// scales of the 8-bit cache below this count as zero, so that 1 / s stays finite
+constexpr float kLeastScale = 0x1p-100f;
+
 // The paged 8-bit KV cache as the kernels take it.
 struct Kv8 {
   int8_t* k;       // [pages, heads, page, d]

@@ -11,9 +11,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// scales below this count as zero, so that 1 / s stays finite
-constexpr float kLeastScale = 0x1p-100f;
-
 // round to nearest even, at most 127 in magnitude; NaN (0 * inf of a page that is not finite) -> 0
 __device__ __forceinline__ int code_of(float x) {
   const float r = rintf(x);
