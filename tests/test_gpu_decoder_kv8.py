@@ -499,3 +499,19 @@ def test_attention_v_scales_below_the_least(dec, news):
             cache.v_scale.fill_(0.01)
         else:
             _near(y, *_attention_ref(q, cache, table, (end,), (news,), d ** -0.5))
+
+
+@pytest.mark.parametrize("news", [3, 70])
+def test_attention_queries_at_the_end_of_the_range(dec, news):
+    """bf16 queries of 2^127 and more, with a scale that makes ordinary scores of them."""
+    g = torch.Generator().manual_seed(30)
+    heads, page, d, end = 2, 16, 128, 200
+    cache = _random_cache(dec, 14, heads, page, d, g)
+    cache.k_scale.mul_(0.05)
+    table = _table((end,), page, 14, g)
+    q = (torch.randn(news, 6, d, generator=g).clamp(-3.9, 3.9) * 2.0 ** 125).to(torch.bfloat16)
+    q[:, :, 7] = 1.5 * 2.0 ** 127
+    q = q.cuda()
+    y = dec.kv8_attention(q, cache, table, _i32(end), _cu((news,)), news, end, 2.0 ** -126)
+    ref, most = _attention_ref(q, cache, table, (end,), (news,), 2.0 ** -126)
+    _near(y, ref, most)

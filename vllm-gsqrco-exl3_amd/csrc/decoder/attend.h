@@ -52,11 +52,11 @@ __device__ __forceinline__ float group_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// The power of two that brings a row's largest magnitude into [1, 2), so that bf16 queries of any
-// size fit fp16 exactly (but for values 2^-14 below the row's largest, rounded there); 1 for an all-zero row.
+// The power of two that brings a row's largest magnitude into [1, 2) ([2, 4) from 2^127 on), so that bf16 queries of
+// any size fit fp16 exactly (but for values 2^-14 below the row's largest, rounded there); 1 for an all-zero row.
 __device__ __forceinline__ float row_factor(float amax) {
   const int e = (int)((__float_as_uint(amax) >> 23) & 0xFF);
-  return amax > 0.0f && e >= 1 && e <= 253 ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
+  return amax > 0.0f && e >= 1 && e <= 254 ? __uint_as_float((uint32_t)max(254 - e, 1) << 23) : 1.0f;
 }
 
 // Where a 16-token chunk lies (page * heads + head, first token in the page), and its scales.
