@@ -515,3 +515,25 @@ def test_attention_queries_at_the_end_of_the_range(dec, news):
     y = dec.kv8_attention(q, cache, table, _i32(end), _cu((news,)), news, end, 2.0 ** -126)
     ref, most = _attention_ref(q, cache, table, (end,), (news,), 2.0 ** -126)
     _near(y, ref, most)
+
+
+def _far_scores(dec, news, log_k_scale):
+    """Scores of -2^(53 + log_k_scale) times whole numbers: the largest takes all."""
+    page, d, end = 16, 64, 75
+    cache = dec.Kv8Cache.empty(6, 1, page, d)
+    g = torch.Generator().manual_seed(31)
+    table = _table((end,), page, 6, g)
+    order = 20 + torch.randperm(100, generator=g)[:96].view(6, 1, page, 1)
+    cache.k.copy_(order.expand(6, 1, page, d))
+    cache.v.copy_(torch.randint(-127, 128, cache.v.shape, generator=g))
+    cache.k_scale.fill_(2.0 ** log_k_scale)
+    cache.v_scale.fill_(0.01)
+    q = torch.full((news, 1, d), -2.0 ** 50, dtype=torch.bfloat16, device="cuda")
+    y = dec.kv8_attention(q, cache, table, _i32(end), _cu((news,)), news, end)
+    _near(y, *_attention_ref(q, cache, table, (end,), (news,), d ** -0.5))
+
+
+@pytest.mark.parametrize("news", [1, 70])
+def test_attention_scores_beyond_2_to_24(dec, news):
+    """Where a score's rounding is far more than the range of a weight."""
+    _far_scores(dec, news, 10)

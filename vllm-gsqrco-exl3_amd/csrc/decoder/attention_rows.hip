@@ -290,7 +290,9 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
         const float vr = x0.vs[c] * inv_ref;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float w = __builtin_amdgcn_exp2f(fmaf((float)s[8 * c + e], f[c], -m));
+          float x = (float)s[8 * c + e] * f[c];
+          asm("" : "+v"(x));  // rounded as it was for the maximum: of scores beyond 2^24 an fma's rest would pass any weight
+          float w = __builtin_amdgcn_exp2f(x - m);
           float y = w * vr;
           if (kMasked && 16 * c + e > seen) w = y = 0.0f;  // also where the page's scale is not finite
           l += w;
