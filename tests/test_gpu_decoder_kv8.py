@@ -537,3 +537,9 @@ def _far_scores(dec, news, log_k_scale):
 def test_attention_scores_beyond_2_to_24(dec, news):
     """Where a score's rounding is far more than the range of a weight."""
     _far_scores(dec, news, 10)
+
+
+@pytest.mark.parametrize("news", [1, 70])
+def test_attention_scores_far_below_zero(dec, news):
+    """Scores below -1e30 are scores all the same."""
+    _far_scores(dec, news, 43)

@@ -20,7 +20,7 @@
 namespace gguf_dec {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoScore = -1e30f;  // the running maximum before any score
+constexpr float kNoScore = -3e38f;  // the running maximum before any score; finite, so that differences are numbers
 // Weights enter the second product in fp16, times this: the maximum lags by at most 2^8, so they end at 2^15, and keep
 // all bits down to 2^-21 of the largest, some down to 2^-32 (without it 2^-14 and 2^-25, where half a million tokens
 // of 2^-26 each, a hundredth of a row's sum, were lost).
