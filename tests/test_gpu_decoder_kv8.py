@@ -543,3 +543,22 @@ def test_attention_scores_beyond_2_to_24(dec, news):
 def test_attention_scores_far_below_zero(dec, news):
     """Scores below -1e30 are scores all the same."""
     _far_scores(dec, news, 43)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("news", [3, 70])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_attention_queries_that_are_not_finite(dec, bad, news, dtype):
+    """A query row with an infinity or a NaN is NaN, also where all of its scores are -inf; the others are as ever."""
+    g = torch.Generator().manual_seed(32)
+    heads, page, d, end = 2, 16, 64, 150
+    cache = _random_cache(dec, 12, heads, page, d, g)
+    cache.k[..., 5] = -7
+    table = _table((end,), page, 12, g)
+    q = (torch.randn(news, 6, d, generator=g) * 0.3).to(dtype).cuda()
+    ref, most = _attention_ref(q, cache, table, (end,), (news,), d ** -0.5)
+    q[1, 4, 5] = bad
+    y = dec.kv8_attention(q, cache, table, _i32(end), _cu((news,)), news, end)
+    assert y[1, 4].isnan().all()
+    y[1, 4], ref[1, 4] = 0, 0
+    _near(y, ref, most)

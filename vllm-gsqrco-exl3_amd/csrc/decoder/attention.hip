@@ -83,8 +83,9 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[2 * s + hf][e]));
         }
-      const float f = DT == kBF16 ? row_factor(group_max(amax)) : 1.0f;
-      qs[t] = a.scale / f;
+      amax = group_max(amax);
+      const float f = DT == kBF16 ? row_factor(amax) : 1.0f;
+      qs[t] = amax < __builtin_inff() ? a.scale / f : __builtin_nanf("");  // also where every score would be -inf
 #pragma unroll
       for (int s = 0; s < 2 * S; ++s)
 #pragma unroll
