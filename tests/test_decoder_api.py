@@ -225,6 +225,24 @@ def test_fake_implementations_have_the_ops_shapes():
         assert [tuple(x.shape) for x in out] == [(3,), (3,), (3,), (3, 7), (3, 7)]
 
 
+class _T(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("ndim", ctypes.c_int32),
+                ("size", ctypes.c_int64 * 4), ("stride", ctypes.c_int64 * 4), ("device", ctypes.c_int32)]
+
+
+class _CacheT(ctypes.Structure):
+    _fields_ = [("k", _T), ("v", _T), ("k_scale", _T), ("v_scale", _T)]
+
+
+_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 5, torch.int32: 6, torch.int64: 7}
+
+
+def _desc(t):
+    r = _T(t.data_ptr(), _CODES[t.dtype], t.dim())
+    r.size[:t.dim()], r.stride[:t.dim()], r.device = list(t.shape), list(t.stride()), -1
+    return r
+
+
 @pytest.mark.parametrize("hint", [2 ** 62, 2 ** 63 - 1])
 def test_hints_beyond_every_size_are_no_trouble(hint):
     """max_new, max_len and max_tokens may be any number: what the tensors hold bounds them before any arithmetic."""
@@ -235,22 +253,10 @@ def test_hints_beyond_every_size_are_no_trouble(hint):
         with pytest.raises(RuntimeError, match="must be CUDA tensors"):
             call()
 
-    class T(ctypes.Structure):
-        _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("ndim", ctypes.c_int32),
-                    ("size", ctypes.c_int64 * 4), ("stride", ctypes.c_int64 * 4), ("device", ctypes.c_int32)]
-
-    class Cache(ctypes.Structure):
-        _fields_ = [("k", T), ("v", T), ("k_scale", T), ("v_scale", T)]
-
-    def desc(t, dtype):
-        r = T(t.data_ptr(), dtype, t.dim())
-        r.size[:t.dim()], r.stride[:t.dim()], r.device = list(t.shape), list(t.stride()), -1
-        return r
-
     lib = ctypes.CDLL(decoder.LIB_PATH)
     lib.gguf_kv8_attention_workspace_bytes.restype = ctypes.c_size_t
-    cache = Cache(*(desc(t, d) for t, d in zip(c, (5, 5, 0, 0))))
-    q = desc(torch.zeros(3, 8, 64, dtype=torch.float16), 1)
+    cache = _CacheT(*(_desc(t) for t in c))
+    q = _desc(torch.zeros(3, 8, 64, dtype=torch.float16))
 
     def workspace(max_new, max_len):
         return lib.gguf_kv8_attention_workspace_bytes(ctypes.byref(cache), ctypes.byref(q), ctypes.c_int64(2),
@@ -258,3 +264,48 @@ def test_hints_beyond_every_size_are_no_trouble(hint):
 
     assert workspace(hint, 6) == workspace(3, 6)
     assert 0 < workspace(hint, hint) == workspace(3, 2 ** 31 - 1)
+
+
+def test_tensors_without_memory_are_refused():
+    """A C caller's NULL where a tensor has elements: an error, for each tensor of each entry point."""
+    lib = ctypes.CDLL(decoder.LIB_PATH)
+    lib.gguf_decoder_last_error.restype = ctypes.c_char_p
+    i64, f32, P, null = ctypes.c_int64, ctypes.c_float, ctypes.byref, ctypes.c_void_p(None)
+    c = _cache()
+    table, lens, cu, rows = torch.zeros(2, 2, dtype=torch.int32), _ints(5, 6), _ints(0, 1, 3), torch.zeros(3, 2, 64)
+    half, state = torch.zeros(3, 4, 64, dtype=torch.float16), torch.zeros(5, 4, 32, 64)
+    v, gate, ids = torch.zeros(3, 4, 32), torch.zeros(3, 4), torch.zeros(3, dtype=torch.int64)
+    f, i, ft, it = (torch.zeros(3, *s, dtype=d) for s, d in (((), torch.float32), ((), torch.int32), ((5,), torch.float32),
+                                                             ((5,), torch.int32)))
+    ws = torch.zeros(1 << 20, dtype=torch.uint8)
+    room = (ctypes.c_void_p(ws.data_ptr() + -ws.data_ptr() % 16), ctypes.c_size_t((1 << 20) - 16), null)
+    calls = {
+        "kv8_append": (["cache", rows, rows, table, lens, cu], lambda a: (*a, i64(2), null)),
+        "kv8_read": (["cache", table, lens, cu, rows, rows], lambda a: (*a[:4], i64(2), *a[4:], null)),
+        "kv8_attention": ([half, "cache", table, lens, cu, half],
+                          lambda a: (*a[:5], i64(2), i64(6), f32(1), a[5], *room)),
+        "gated_delta_rule": ([rows, rows, v, gate, gate, state, lens, lens, cu, v],
+                             lambda a: (*a[:9], i64(2), f32(1), 1, a[9], *room)),
+        "token_logprobs": ([torch.zeros(3, 100), ids, f, i, f, ft, it], lambda a: (*a[:2], i64(5), *a[2:], *room)),
+    }
+    for name, (tensors, order) in calls.items():
+        call = getattr(lib, "gguf_" + name)
+        for spoil in range(-1, len(tensors)):
+            for part in range(4 if spoil >= 0 and isinstance(tensors[spoil], str) else 1):
+                descs = [_CacheT(*map(_desc, c)) if isinstance(t, str) else _desc(t) for t in tensors]
+                if spoil >= 0:
+                    d = descs[spoil]
+                    (d if isinstance(d, _T) else getattr(d, ("k", "v", "k_scale", "v_scale")[part])).data = None
+                assert call(*order([P(d) for d in descs])) == 1
+                message = lib.gguf_decoder_last_error().decode()
+                assert ("must be CUDA tensors" if spoil < 0 else "no data") in message, (name, spoil, part, message)
+
+
+def test_no_rows_need_no_memory():
+    """Tensors without elements may have no memory: the checks end where those of other host tensors do."""
+    for call in (lambda: _kv(key=torch.zeros(0, 2, 64), value=torch.zeros(0, 2, 64)), lambda: _read(tokens=0),
+                 lambda: _attention(query=torch.zeros(0, 4, 64, dtype=torch.float16)),
+                 lambda: _logprobs(logits=torch.zeros(0, 100), token_ids=torch.zeros(0, dtype=torch.int64)),
+                 lambda: _logprobs(top=0)):
+        with pytest.raises(RuntimeError, match="must be CUDA tensors"):
+            call()

@@ -126,6 +126,14 @@ bool same_device(int dev, const T*... t) {
   return same;
 }
 
+// tensors that have elements have memory
+template <class... T>
+bool present(const T*... t) {
+  bool all = true;
+  ((all = all && (!t || t->data || numel(t) == 0)), ...);
+  return all;
+}
+
 // cu_seqlens: int32 [seqs + 1], contiguous
 int check_cu(const char* op, const gguf_tensor* cu, int64_t tokens, Ragged* out) {
   if (!shaped(cu, 1) || cu->dtype != GGUF_DEC_I32 || !contiguous(cu)) return fail("%s: cu_seqlens must be a contiguous 1-D int32 tensor", op);
@@ -162,6 +170,7 @@ int check_cache(const char* op, const gguf_kv8_cache* c, const gguf_tensor* tabl
   if (table->size[1] < 1) return fail("%s: block_table has no pages", op);
   if (table->size[1] * page > INT_MAX - 1024) return fail("%s: block_table of too many pages", op);
   if (!same_device(c->k.device, &c->v, &c->k_scale, &c->v_scale, table)) return fail("%s: tensors on different devices", op);
+  if (!present(&c->k, &c->v, &c->k_scale, &c->v_scale, table)) return fail("%s: a tensor has no data", op);
   *out = Kv8{(int8_t*)c->k.data, (int8_t*)c->v.data, (float*)c->k_scale.data, (float*)c->v_scale.data,
              (const int32_t*)table->data, stride_of(table, 0), (int)p, (int)h, (int)page, (int)d, (int)table->size[1]};
   return 0;
@@ -192,6 +201,7 @@ int gguf_kv8_append(const gguf_kv8_cache* cache, const gguf_tensor* key, const g
     return fail("%s: key and value need unit inner stride and 16-byte aligned rows", op);
   if (max_new < 0) return fail("%s: max_new must not be negative", op);
   if (!same_device(key->device, value, &cache->k, seq_lens, cu_seqlens)) return fail("%s: tensors on different devices", op);
+  if (!present(key, value, seq_lens, cu_seqlens)) return fail("%s: a tensor has no data", op);
   if (key->device < 0) return fail("%s: tensors must be CUDA tensors", op);
   if (key->size[0] == 0) return GGUF_DEC_OK;
   const DeviceScope scope(key->device);
@@ -219,6 +229,7 @@ int gguf_kv8_read(const gguf_kv8_cache* cache, const gguf_tensor* block_table, c
       return fail("%s: outputs must be contiguous, 16-byte aligned [tokens, %d, %d] for this cache", op, c.heads, c.d);
   if (max_tokens < 0) return fail("%s: max_tokens must not be negative", op);
   if (!same_device(k_out->device, v_out, &cache->k, starts, cu_seqlens)) return fail("%s: tensors on different devices", op);
+  if (!present(k_out, v_out, starts, cu_seqlens)) return fail("%s: a tensor has no data", op);
   if (k_out->device < 0) return fail("%s: tensors must be CUDA tensors", op);
   if (k_out->size[0] == 0) return GGUF_DEC_OK;
   const DeviceScope scope(k_out->device);
@@ -261,6 +272,7 @@ int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, co
   if (!std::isfinite(scale)) return fail("%s: scale must be finite", op);
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail("%s: workspace must be 16-byte aligned", op);
   if (!same_device(query->device, out, &cache->k, seq_lens, cu_seqlens)) return fail("%s: tensors on different devices", op);
+  if (!present(query, out, seq_lens, cu_seqlens)) return fail("%s: a tensor has no data", op);
   if (query->device < 0) return fail("%s: tensors must be CUDA tensors", op);
   if (query->size[0] == 0) return GGUF_DEC_OK;
   const DeviceScope scope(query->device);
@@ -325,6 +337,7 @@ int gguf_gated_delta_rule(const gguf_tensor* q, const gguf_tensor* k, const gguf
   if (max_new < 0) return fail("%s: max_new must not be negative", op);
   if (!std::isfinite(scale)) return fail("%s: scale must be finite", op);
   if (!same_device(q->device, k, v, g, beta, state, slots, out_slots, cu_seqlens, out)) return fail("%s: tensors on different devices", op);
+  if (!present(q, k, v, g, beta, state, slots, out_slots, cu_seqlens, out)) return fail("%s: a tensor has no data", op);
   if (q->device < 0) return fail("%s: tensors must be CUDA tensors", op);
   const size_t need = t ? gguf_dec::delta_workspace(q->dtype, (int)dk, (int)hk, (int)hv, t, rows.seqs, max_new, steps > 0) : 0;
   if (need > 0 && (workspace_bytes < need || !workspace)) return fail("%s: workspace of %zu bytes needed, got %zu", op, need, workspace_bytes);
@@ -363,6 +376,7 @@ int gguf_token_logprobs(const gguf_tensor* logits, const gguf_tensor* token_ids,
     if (!shaped(o.t, o.nd) || o.t->dtype != o.dt || o.t->size[0] != rows || (o.nd == 2 && o.t->size[1] != top) || !contiguous(o.t))
       return fail("%s: %s must be contiguous %s of %lld rows", op, o.name, o.dt == GGUF_DEC_F32 ? "fp32" : "int32", (long long)rows);
   if (!same_device(logits->device, token_ids, logprobs, ranks, entropy, top_logprobs, top_ids)) return fail("%s: tensors on different devices", op);
+  if (!present(logits, token_ids, logprobs, ranks, entropy, top_logprobs, top_ids)) return fail("%s: a tensor has no data", op);
   if (logits->device < 0) return fail("%s: tensors must be CUDA tensors", op);
   if (rows == 0) return GGUF_DEC_OK;
   const size_t need = gguf_dec::logprobs_workspace(rows, vocab, top);
