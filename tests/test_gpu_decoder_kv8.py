@@ -562,3 +562,17 @@ def test_attention_queries_that_are_not_finite(dec, bad, news, dtype):
     assert y[1, 4].isnan().all()
     y[1, 4], ref[1, 4] = 0, 0
     _near(y, ref, most)
+
+
+def test_attention_more_rows_than_a_join_takes(dec):
+    """2^24 rows of a hint that would split them: unsplit. (They see nothing, but for the last token's.)"""
+    hq, d, tokens = 64, 64, (1 << 18) + 3
+    g = torch.Generator().manual_seed(35)
+    cache = _random_cache(dec, 3, hq, 16, d, g)
+    table = _table((20,), 16, 3, g)
+    q = torch.zeros(tokens, hq, d, dtype=torch.bfloat16, device="cuda")
+    q[-20:] = torch.randn(20, hq, d, generator=g).cuda()
+    y = dec.kv8_attention(q, cache, table, _i32(20), _cu((tokens,)), 1, 100000)
+    ref, most = _attention_ref(q[-20:], cache, table, (20,), (20,), d ** -0.5)
+    assert (y[:-20] == 0).all()
+    _near(y[-20:], ref, most)

@@ -1,4 +1,6 @@
 // Causal attention over the 8-bit paged cache (attend.h: layouts; include/gguf_decoder.h: contract).
+#include <algorithm>
+
 #include "attend.h"
 
 namespace gguf_dec {
@@ -334,7 +336,7 @@ struct AttnPlan {
   int64_t row_tiles;
 };
 
-static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, int64_t most_splits) {
+static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, int64_t most) {
   AttnPlan p;
   p.many = rows > 64;
   p.nt = rows > 16 && d < 256 ? 2 : 1;
@@ -343,8 +345,7 @@ static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, 
   const int64_t blocks = groups * p.row_tiles, step = kTile * kWaves;
   const int64_t steps = (max_len + step - 1) / step;
   int64_t want = (2 * gguf::device_cus() + blocks - 1) / blocks;
-  if (want > 512) want = 512;
-  if (want > most_splits) want = most_splits;
+  if (want > most) want = most;
   if (want < 1) want = 1;
   const int64_t each = (steps + want - 1) / want;
   p.span = (int)(each * step < (1 << 30) ? each * step : (1 << 30));
@@ -353,9 +354,12 @@ static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, 
   return p;
 }
 
+// splits of a call of that many rows: join_kernel's grid, a workgroup a row, holds fewer than 2^32 threads
+static int64_t most_splits(int64_t rows) { return rows < (1 << 24) ? 512 : 1; }
+
 size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t seqs, int64_t max_new,
                                int64_t max_len) {
-  const AttnPlan p = attn_plan(d, max_new * (hq / heads), seqs * heads, max_len, 512);
+  const AttnPlan p = attn_plan(d, max_new * (hq / heads), seqs * heads, max_len, most_splits(tokens * hq));
   return p.splits == 1 ? 0 : (size_t)p.splits * tokens * hq * (d + 2) * sizeof(float);
 }
 
@@ -364,7 +368,8 @@ hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t 
                                 void* out, void* ws, size_t ws_bytes, hipStream_t stream) {
   const int64_t all = (int64_t)rows.tokens * hq;
   const int64_t fit = (int64_t)(ws_bytes / sizeof(float)) / (all * (c.d + 2));
-  const AttnPlan p = attn_plan(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len, fit < 2 ? 1 : fit);
+  const AttnPlan p = attn_plan(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len,
+                               fit < 2 ? 1 : std::min(fit, most_splits(all)));
   const AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, p.span, p.splits, out, (float*)ws,
                    (float*)ws + (size_t)p.splits * all * c.d};
   const dim3 grid((unsigned)(rows.seqs * c.heads * p.splits), (unsigned)(p.row_tiles < 65535 ? p.row_tiles : 65535));
