@@ -121,8 +121,9 @@ GGUF_DEC_API int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cac
  * token; [seqs, m]: after each of its first m tokens, as a verify pass needs that may keep only some of
  * them; NULL: back to slots. A slot out of range keeps nothing, and a sequence of no tokens
  * copies its state to a [seqs] slot. No slot may be written twice, or written for one sequence and read
- * for another. out: [tokens, hv, dv] contiguous, in q's dtype. Token strides are at most 2^22 elements. In the
- * chunked form a token that is not finite also makes NaN of its chunk's earlier outputs.
+ * for another. out: [tokens, hv, dv] contiguous, in q's dtype. Token strides are at most 2^22 elements. What a
+ * token that is not finite reaches (a value's column, a key's, gate's or beta's head, from that token on) is
+ * not finite, and nothing else is.
  * max_new: the largest n_s, a hint; the workspace is for sequences of more tokens than the recurrent form
  * takes (gguf_gated_delta_rule_workspace_bytes). */
 GGUF_DEC_API size_t gguf_gated_delta_rule_workspace_bytes(const gguf_tensor* q, const gguf_tensor* v, int64_t seqs,

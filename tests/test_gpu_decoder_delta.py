@@ -231,3 +231,34 @@ def test_other_stream_and_graph(dec, news):
     assert torch.equal(y, z) and torch.equal(kept, state[2:])
     graph_replays_equal(call, y)
     assert torch.equal(kept, state[2:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("what", ["q", "k", "v", "g", "beta"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [3, 84, 149])
+@pytest.mark.parametrize("max_new", [1, 150], ids=["recurrent", "chunks"])
+def test_a_token_that_is_not_finite(dec, dtype, what, bad, at, max_new):
+    """Outputs of earlier tokens, of other heads and (for a value) of other columns are as ever; from the token on nothing
+    that it reaches is finite (of a query, its own output alone)."""
+    news, hk, hv, dk, dv = (150, 40), 2, 4, 128, 48
+    q, k, v, g, beta, state = _inputs(news, hk, hv, dk, dv, dtype, 40)
+    out, last, _, size = _ref(q, k, v, g, beta, state, news, dk ** -0.5, True)
+    {"q": q[at, 1], "k": k[at, 1], "v": v[at, 3], "g": g[at, 3:], "beta": beta[at, 3:]}[what][:1 if what in "g beta" else 6] = bad
+    y = dec.gated_delta_rule(q, k, v, g, beta, state, _i32([0, 1]), _cu(news), max_new)
+    hit = torch.zeros(y.shape, dtype=torch.bool)
+    heads = [2, 3] if what in ("q", "k") else [3]
+    for h in heads:
+        hit[at:(at + 1 if what == "q" else news[0]), h, :6 if what == "v" else dv] = True
+    assert not y.cpu()[hit].isfinite().any()
+    y = torch.where(hit.cuda(), 0, y)
+    out = torch.where(hit, 0, out)
+    _check(y, out, size, dtype)
+    _check_state(state[1], last[1])
+    fine = torch.ones(hv, dv, dtype=torch.bool)
+    if what != "q":
+        fine = ~hit[-41]
+        assert not state[0].cpu()[~fine].isfinite().any()
+    for h in range(hv):
+        if fine[h].any():
+            _check_state(state[0, h:h + 1, fine[h]], [last[0][h, fine[h]]])

@@ -65,7 +65,7 @@ struct Layout {
   static constexpr int NU = DT == kF32 ? 6 : 5;     // U's planes: three for S, the others for the output
   static constexpr int kS = kKq + kT, kX = kS + ND * 3 * (DK / 32) * 1024, kU = kX + ND * 3 * (C / 32) * 1024;
   static constexpr int kLds = kU + ND * NU * (C / 32) * 1024;
-  static_assert(kLds <= 160 * 1024, "LDS");
+  static_assert(kLds + ND * 16 * 4 <= 160 * 1024, "LDS");
 };
 
 }  // namespace gguf_dec

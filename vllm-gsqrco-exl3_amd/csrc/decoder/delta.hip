@@ -146,6 +146,19 @@ __global__ void __launch_bounds__(256) recurrent_kernel(DeltaArgs a, int most) {
 // keep i + j <= 1, below 2^-16, where the output is rounded to 16 bits. Differences of G are taken in 64 bits: G
 // may reach thousands where only differences near 0 matter.
 
+// What a token that is not finite reaches: its own and later tokens, of its columns. The products meet it with the
+// zeros of T and A above the diagonal as well, where 0 NaN would reach earlier tokens; so such values are taken as 0 there,
+// and the first token of a column to have one is kept, from which on the column is NaN.
+
+// finite, and within bf16's range
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.38e38f; }
+
+// min over the four lane groups (lanes n, n + 16, n + 32, n + 48)
+__device__ __forceinline__ int groups_min(int v) {
+  v = min(v, __shfl_xor(v, 16, 64));
+  return min(v, __shfl_xor(v, 32, 64));
+}
+
 // P planes of 8 fp32 values, two a conversion
 template <int P>
 __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&planes)[P]) {
@@ -426,9 +439,23 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
         for (int s = 0; s < 4; ++s) m = __builtin_amdgcn_mfma_f32_16x16x4f32(l[s], col[y][s], m, 0, 0, 0);
       }
       const floatx4 d = *(const floatx4*)(T + (16 * I + n) * LS + 16 * I + 4 * g);
+      // rows before one that is not finite meet it with T_II's zeros, which must not make them NaN
+      int first = 16;
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (!finite(m[e])) {
+          first = 4 * g + e;
+          m[e] = 0.0f;
+        }
       floatx4 r = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < 4; ++s) r = __builtin_amdgcn_mfma_f32_16x16x4f32(-d[s], m[s], r, 0, 0, 0);
+      if (__any(first < 16)) {
+        first = groups_min(first);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * g + e >= first) r[e] = __builtin_nanf("");
+      }
       col[x] = r;
 #pragma unroll
       for (int e = 0; e < 4; ++e) T[(16 * I + 4 * g + e) * LS + 16 * J + n] = r[e];
@@ -462,6 +489,7 @@ __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kerne
   constexpr int TT = C / 16, TS = C / 32, KT = DK / 16, KS = DK / 32, KW = KT / TT;
   constexpr int MAXO = DT == kF32 ? 2 : 1;  // highest plane sum kept for the output
   extern __shared__ __align__(16) char lds[];
+  __shared__ int dead[Lay::ND][16];  // of each column: its first token that is not finite (in later chunks 0: S is NaN)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   const int wt = wave % TT, wd = wave / TT;
   const int seq = blockIdx.z, h = blockIdx.x, hk = h / a.rep;
@@ -517,6 +545,7 @@ __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kerne
   char* const xl = lds + Lay::kX + wd * 3 * TS * 1024 + 16 * lane;
   char* const ul = lds + Lay::kU + wd * Lay::NU * TS * 1024 + 16 * lane;
 
+  if (tid < 16 * Lay::ND) dead[tid / 16][n] = C;
   fetch(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
@@ -563,12 +592,17 @@ __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kerne
       f2[e] = f.w;
     }
     const float dec = F[C].x;
-    {
-      uint2 w[3];
-      split4(x, w);
+    int first = C;  // the lane's first token whose u is not finite
+    const auto clean = [&](floatx4& y) __attribute__((always_inline)) {
+      // where a branch costs less than the selects (8192 bf16 tokens, 48 heads: 605 us against 618; 2048 of fp16 263, 249)
+      if (DT == kBF16 && !__any(!finite(fabsf(y[0]) + fabsf(y[1]) + fabsf(y[2]) + fabsf(y[3])))) return;
 #pragma unroll
-      for (int p = 0; p < 3; ++p) *(uint2*)(xl + (p * TS + wt / 2) * 1024 + 8 * (wt & 1)) = w[p];
-    }
+      for (int e = 3; e >= 0; --e)
+        if (!finite(y[e])) {
+          first = min(first, tok0 + 8 * g + e);
+          y[e] = 0.0f;
+        }
+    };
     // K^T's rows are keys: the transposing read gives a lane 4 tokens of its key, from the 4 rows that its group of 16
     // lanes addresses (lane 4 r + c: 4 keys of row r)
     bf16x8 tm[TS][3], am[TS][NA], km[NK][TS][KW];
@@ -587,6 +621,13 @@ __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kerne
           km[p][s][t] = join(turned(k), turned(k + 4 * KR));
         }
     }
+    clean(x);
+    {
+      uint2 w[3];
+      split4(x, w);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *(uint2*)(xl + (p * TS + wt / 2) * 1024 + 8 * (wt & 1)) = w[p];
+    }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the chunk's operands are here
     __syncthreads();
     fetch(min(c + 1, chunks - 1));  // taken within this turn, so that its wait does not take in the stores
@@ -604,7 +645,9 @@ __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kerne
 #pragma unroll
         for (int o = 0; o + p <= 2; ++o) U[o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tm[s][p], xp[o], U[o], 0, 0, 0);
     }
-    const floatx4 u = U[0] + (U[1] + U[2]);
+    floatx4 u = U[0] + (U[1] + U[2]);
+    clean(u);
+    if (DT != kBF16 || __any(first < C)) atomicMin(&dead[wd][n], first);
     {
       uint2 w[3], o[MAXO + 1];
       split4(u * f2, w);
@@ -617,8 +660,9 @@ __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kerne
     __syncthreads();
 
     // S = e^{G_c} S + K^T (e^{G_c - G} U);   O += A U
+    first = dead[wd][n];
 #pragma unroll
-    for (int t = 0; t < KW; ++t) S[t] *= dec;
+    for (int t = 0; t < KW; ++t) S[t] *= first < C ? __builtin_nanf("") : dec;
 #pragma unroll
     for (int s = 0; s < TS; ++s) {
       bf16x8 wp[3], up[MAXO + 1];
@@ -641,7 +685,8 @@ __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kerne
     }
     const __amdgpu_buffer_rsrc_t rs = gguf::buffer_rsrc((char*)a.out + (int64_t)(r0 + c * C) * ot + (int64_t)h * a.dv * ES, (C - 1) * ot + a.dv * ES);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) Bits<DT>::store(rs, place(e, nt, ot), O[0][e] + O[1][e]);
+    for (int e = 0; e < 4; ++e)
+      Bits<DT>::store(rs, place(e, nt, ot), tok0 + 8 * g + e >= first ? __builtin_nanf("") : O[0][e] + O[1][e]);
     __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4): all but these stores
   }
   const int to = a.out_slots[(int64_t)seq * a.out_stride];
