@@ -106,7 +106,7 @@ def generate(layers=4, prompts=(300, 117), tokens=8, drafts=3, seed=0):
     n = len(prompts)
     gen = torch.Generator().manual_seed(seed + 1)
     texts = [torch.randint(VOCAB, (p,), generator=gen).tolist() for p in prompts]
-    room = -(-(max(prompts) + tokens + (drafts + 1) * tokens) // PAGE)
+    room = -(-(max(prompts) + tokens + drafts + 2) // PAGE)  # pages: the decoded tokens, a verify pass, one token more
     # slots 0 .. n - 1 hold the states, the others the states after each row of a verify pass
     m = drafts + 1
     model = Model(layers, n * room, n + n * m, seed)

@@ -42,3 +42,19 @@ def test_steps_give_what_a_prompt_gives():
     y = model(nxt, m.Batch([1] * n, [v + 1 for v in lens], table, list(range(n)), list(range(n))))
     cos = torch.nn.functional.cosine_similarity(y.float(), logits.float())
     assert (cos > 0.99).all(), cos
+
+
+@pytest.mark.parametrize("prompts,tokens,drafts", [((64, 20), 0, 3), ((63, 1), 1, 7)])
+def test_few_tokens_and_drafts(prompts, tokens, drafts, monkeypatch):
+    """No decoded tokens, and drafts that start a page: the table has room for every step."""
+    m = _example()
+
+    class Batch(m.Batch):
+        def __init__(self, *a):
+            super().__init__(*a)
+            assert self.max_len <= self.table.shape[1] * m.PAGE
+
+    monkeypatch.setattr(m, "Batch", Batch)
+    texts, logprobs, logits = m.generate(prompts=prompts, tokens=tokens, drafts=drafts)
+    assert [len(t) for t in logprobs] == [tokens] * 2 and torch.isfinite(logits).all()
+    assert all(p + tokens < len(t) <= p + tokens + 1 + drafts for p, t in zip(prompts, texts))
