@@ -132,7 +132,7 @@ def generate(layers=4, prompts=(300, 117), tokens=8, drafts=3, seed=0):
     rows = torch.cat([nxt[:, None], guess], 1)
     kept_slots = [[n + s * m + i for i in range(m)] for s in range(n)]
     logits = model(rows.flatten(), Batch([m] * n, [x + m for x in lens], table, list(range(n)), kept_slots))
-    given = torch.cat([guess, guess[:, -1:]], 1).flatten()
+    given = torch.cat([guess, nxt[:, None]], 1).flatten()  # (nothing is drafted behind the last row: any token)
     _, ranks, _, _, best = decoder.token_logprobs(logits, given, 1)
     good = (ranks.view(n, m)[:, :drafts] == 1).long().cumprod(-1).sum(-1).tolist()  # drafts that are the best tokens
     nxt = best.view(n, m)[torch.arange(n), torch.tensor(good)].long()

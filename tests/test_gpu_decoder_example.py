@@ -44,9 +44,9 @@ def test_steps_give_what_a_prompt_gives():
     assert (cos > 0.99).all(), cos
 
 
-@pytest.mark.parametrize("prompts,tokens,drafts", [((64, 20), 0, 3), ((63, 1), 1, 7)])
+@pytest.mark.parametrize("prompts,tokens,drafts", [((64, 20), 0, 3), ((63, 1), 1, 7), ((100, 30), 2, 0), ((63, 40), 0, 0)])
 def test_few_tokens_and_drafts(prompts, tokens, drafts, monkeypatch):
-    """No decoded tokens, and drafts that start a page: the table has room for every step."""
+    """No decoded tokens, no drafts, and drafts that start a page: the table has room for every step."""
     m = _example()
 
     class Batch(m.Batch):
