@@ -576,3 +576,22 @@ def test_attention_more_rows_than_a_join_takes(dec):
     ref, most = _attention_ref(q[-20:], cache, table, (20,), (20,), d ** -0.5)
     assert (y[:-20] == 0).all()
     _near(y[-20:], ref, most)
+
+
+@pytest.mark.parametrize("hq,heads,d,page", [(6, 1, 256, 64), (4, 2, 128, 16), (2, 2, 64, 144)])
+@pytest.mark.parametrize("news", [3, 70])
+@pytest.mark.parametrize("end", [4095, 4097, 4128, 8200])
+def test_attention_past_a_segment(dec, end, news, hq, heads, d, page):
+    """Contexts in one split (a hint of 1) of more tokens than either kernel looks up at a time, and of just fewer."""
+    q, cache, table, y = _run_attention(dec, (end, 70), (news, 2), hq, heads, d, page, torch.bfloat16, 36, max_len=1)
+    _near(y, *_attention_ref(q, cache, table, (end, 70), (news, 2), d ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("hq,heads,d,page", [(6, 1, 256, 16), (8, 2, 128, 32), (4, 4, 64, 144), (5, 1, 192, 64)])
+@pytest.mark.parametrize("news", [(1, 1, 1, 1), (1, 3, 0, 7), (5, 40, 2, 17), (1, 65, 200, 130)], ids=str)
+def test_attention_gives_numbers(dec, news, hq, heads, d, page, dtype):
+    """The sizes above once more, where a NaN counts."""
+    ends = (1 if news[0] == 1 else 5, 65, 200, 777)
+    q, cache, table, y = _run_attention(dec, ends, news, hq, heads, d, page, dtype, 37)
+    _near(y, *_attention_ref(q, cache, table, ends, news, d ** -0.5))
