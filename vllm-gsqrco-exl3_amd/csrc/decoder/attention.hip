@@ -22,8 +22,8 @@ constexpr int kSegment = 64;  // tiles whose chunks are looked up at a time
 //
 // Bound: HBM, 2 bytes a (token, head, dim). Measured, 24 query and 4 KV heads of 256: 64 ragged sequences of up to
 // 16384 tokens 234 us (989 MB, 4.2 TB/s; before a wave's next tile was fetched ahead 444); one of 701 tokens 14 us,
-// latency. At head size 256 a workgroup takes 16 rows: 32 spill, and 8 sequences of 4 rows over up to 32768
-// tokens took 148 us with them, 104 with the cache read for two row tiles.
+// latency. At head sizes from 128 on a workgroup takes 16 rows: of 256, 32 spill, and the kernel took 148 us for 8
+// sequences of 4 rows over up to 32768 tokens, 104 with the cache read for two row tiles; see attn_plan for the others.
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   constexpr int S = D / 64, DD = D / 16;
@@ -330,6 +330,14 @@ hipError_t launch_attend(const AttnArgs& a, dim3 grid, hipStream_t stream) {
 
 // How a call is cut: rows of a workgroup, and tokens of a split so that the CUs have two workgroups each, in
 // steps of a tile a wave.
+// Many rows: from 64 on, about where the two forms cross in long contexts. Calls in us, few / many, at up to 16384 tokens: head
+// size 256, one sequence of 24 rows 29.9 / 31.9, of 66 rows 39.8 / 34.0, eight of 24 rows 68.8 / 115, of 48 rows 114 / 120,
+// of 66 rows 158 / 120; head size 128, one of 64 rows 24.1 / 28.7, of 96 rows 39.3 / 31.8, eight of 32 rows 55.3 / 97.2, of
+// 64 rows 97.0 / 98.7, of 96 rows 116 / 101. (Over 2048 tokens one sequence stays quicker with few: of 66 rows 16.4 / 27.9.)
+// Two row tiles a workgroup (32 rows): only at head size 64 does the cache read once make up for the waves' registers.
+// Calls in us, one / two tiles, at up to 16384 tokens: head size 64, eight sequences of 64 rows 67.5 / 55.7, of 24 rows
+// 39.2 / 35.6; head size 128, eight of 32 rows 55.3 / 62.6, one of 32 rows 19.4 / 27.8; head size 192, one of 24 rows
+// 15.0 / 18.0, eight of 60 rows 37.9 / 40.4, of 36 rows 45.8 / 38.1.
 struct AttnPlan {
   bool many;
   int nt, span, splits;
@@ -339,7 +347,7 @@ struct AttnPlan {
 static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, int64_t most) {
   AttnPlan p;
   p.many = rows > 64;
-  p.nt = rows > 16 && d < 256 ? 2 : 1;
+  p.nt = rows > 16 && d < 128 ? 2 : 1;
   const int64_t tile = p.many ? kRowsTile : 16 * p.nt;
   p.row_tiles = (rows + tile - 1) / tile;
   const int64_t blocks = groups * p.row_tiles, step = kTile * kWaves;
@@ -378,7 +386,7 @@ hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t 
 #define GGUF_DEC_ATTEND(DT, D)                                                                                         \
   {                                                                                                                    \
     if (!p.many && p.nt == 1) e = launch_attend<DT, D, 1>(a, grid, stream);                                            \
-    if constexpr (D < 256)                                                                                             \
+    if constexpr (D < 128)                                                                                             \
       if (!p.many && p.nt == 2) e = launch_attend<DT, D, 2>(a, grid, stream);                                          \
     if (e == hipSuccess && p.splits > 1)                                                                               \
       join_kernel<DT, D><<<(unsigned)all, 256, 0, stream>>>(a.part, a.stat, all, p.splits, out);           \

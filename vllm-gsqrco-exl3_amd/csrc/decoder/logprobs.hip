@@ -330,7 +330,9 @@ int64_t chunks_of(int64_t vocab, int per) {  // one piece more: a row may begin 
 }
 
 // values of a chunk a thread: 32, or 8 where chunks of 32 would not give every CU a workgroup and the best of the
-// smaller ones, four times as many, still fit merge_kernel
+// smaller ones, four times as many, still fit merge_kernel. Calls in us, 32 / 8 values, 20 best of bf16 logits: of 151936
+// one row 15.5 / 14.7, 8 rows 15.9 / 16.0, 16 rows 16.5 / 17.3, 64 rows 20.1 / 29.7; of 32000 one row 15.2 / 13.9, 64 rows
+// 15.8 / 15.8, 128 rows 16.4 / 19.0.
 int per_thread(int64_t rows, int64_t vocab, int64_t top) {
   return rows * chunks_of(vocab, 32) < gguf::device_cus() && vocab < (1 << 20) &&
                  chunks_of(vocab, 8) * top <= kMergeMost * kThreads
