@@ -12,8 +12,9 @@
  * GGUF_DEC_EINVAL with a message in gguf_decoder_last_error() (per thread). What lies in device
  * memory (lengths, page numbers, slots, token ids) is checked by the kernels: a length is cut to what
  * its tensors hold, and what each entry point says happens for a page, slot or token id out of
- * range. Results do not depend on max_new and max_len (hints that size the grid) beyond the order
- * of fp32 sums. Calls are safe under stream capture.
+ * range. max_new and max_len are hints: they size the grid, and choose between forms of a call that compute the same
+ * and round differently, as its entry point says (kv8_attention up to 64 rows a KV head and above,
+ * gated_delta_rule by tokens and by chunks). Any number is allowed. Calls are safe under stream capture.
  *
  * cu_seqlens [seqs + 1] (int32) holds the offsets of each sequence's rows in the ragged tensors, and
  * sequence s has n_s = cu_seqlens[s + 1] - cu_seqlens[s] rows.
@@ -102,7 +103,12 @@ GGUF_DEC_API int gguf_kv8_read(const gguf_kv8_cache* cache, const gguf_tensor* b
  * out = softmax(scale * q k^T) v. A row that sees nothing is 0; one that sees a page whose number is
  * out of range is NaN. out: contiguous, like query. The workspace holds the partial results of a
  * cache split over workgroups; with fewer bytes than gguf_kv8_attention_workspace_bytes (0 included) the
- * call is split less. max_new, max_len: the largest n_s and seq_lens[s], hints. */
+ * call is split less. max_new, max_len: the largest n_s and seq_lens[s], hints.
+ * Precision: sums and the softmax's statistics are fp32. A weight times its page's V scale enters the second product
+ * in fp16: to 2^-12 of itself down to 2^-21 of the row's largest weight times the largest V scale that the row sees, below
+ * that to 2^-32 of these. Queries: where max_new * q_heads / heads is at most 64, exact but for bf16 elements below 2^-14
+ * of the row's largest; above, integers of 15 bits, to 2^-15 of the row's largest magnitude (0 where that is below 2^-100).
+ * A query row with an infinity or a NaN is NaN. */
 GGUF_DEC_API size_t gguf_kv8_attention_workspace_bytes(const gguf_kv8_cache* cache, const gguf_tensor* query,
                                                        int64_t seqs, int64_t max_new, int64_t max_len);
 GGUF_DEC_API int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache,
@@ -124,6 +130,8 @@ GGUF_DEC_API int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cac
  * for another. out: [tokens, hv, dv] contiguous, in q's dtype. Token strides are at most 2^22 elements. What a
  * token that is not finite reaches (a value's column, a key's, gate's or beta's head, from that token on) is
  * not finite, and nothing else is.
+ * Precision: states are fp32 throughout, products carry 24 bits. In the chunked form (more than 32 tokens) the two
+ * products that make an fp16 or bf16 output, S q and A u, keep 2^-16 of their terms.
  * max_new: the largest n_s, a hint; the workspace is for sequences of more tokens than the recurrent form
  * takes (gguf_gated_delta_rule_workspace_bytes). */
 GGUF_DEC_API size_t gguf_gated_delta_rule_workspace_bytes(const gguf_tensor* q, const gguf_tensor* v, int64_t seqs,

@@ -21,9 +21,9 @@ constexpr int kSegment = 64;  // tiles whose chunks are looked up at a time
 // has 8 or 11), everything else is fp32.
 //
 // Bound: HBM, 2 bytes a (token, head, dim). Measured, 24 query and 4 KV heads of 256: 64 ragged sequences of up to
-// 16384 tokens 234 us (989 MB, 4.2 TB/s; before a wave's next tile was fetched ahead 444); one of 701 tokens 14 us,
-// latency. At head sizes from 128 on a workgroup takes 16 rows: of 256, 32 spill, and the kernel took 148 us for 8
-// sequences of 4 rows over up to 32768 tokens, 104 with the cache read for two row tiles; see attn_plan for the others.
+// 16384 tokens 235 us a call (989 MB, 4.2 TB/s; before a wave's next tile was fetched ahead 444); one of 701 tokens 14 us,
+// of which this kernel is 12, latency. At head sizes from 128 on a workgroup takes 16 rows: of 256, 32 spill, and this kernel took 148 us for 8
+// sequences of 4 rows over up to 32768 tokens, 104 (the call 117) with the cache read for two row tiles; see attn_plan for the others.
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   constexpr int S = D / 64, DD = D / 16;

@@ -1,6 +1,6 @@
 // Causal attention over the 8-bit paged cache for many rows a sequence (a prompt's chunk): the form of
-// attention.hip with the tiles shared through LDS and 32 x 32 MFMAs, which alone reach the matrix cores' full rate here
-// (f16 32x32x16 2.45 PFLOP/s, 16x16x32 1.41).
+// attention.hip with the tiles shared through LDS and 32 x 32 MFMAs, which reach more of the matrix cores' rate here
+// (in loops without loads f16 32x32x16 1.71 PFLOP/s, 16x16x32 1.37, i8 32x32x32 4.8).
 //
 // Both products are transposed, S^T = K Q^T and O^T += V^T P^T, so that a lane keeps one query row. With lane = 32 h + n,
 // a result's element i is row 8 (i >> 2) + 4 h + (i & 3) of column n. The 32 tokens of a tile stand in K's rows in
@@ -14,10 +14,10 @@
 // next to the matrix cores, and K needs no conversion.
 // V is converted to fp16 once a workgroup, from registers to LDS.
 //
-// Measured, 24 query and 4 KV heads of 256: 2048 rows at positions up to 8192 637 us, 567 TFLOP/s (1453 us in the
-// form for few rows). A wave's turn (32 rows, 32 tokens) is some 3,100 cycles, 1,024 of them MFMAs: the softmax and
-// the operand reads are not hidden, with one wave a SIMD (D = 256: 128 accumulator and 64 query registers; two
-// workgroups a CU spill, 1,065 us).
+// Measured, 24 query and 4 KV heads of 256: a call of 2048 rows at positions up to 8192 590 us, 611 TFLOP/s (1453 us in the
+// form for few rows). By counters the matrix cores are busy for 25 % of the kernel's time and VALU instructions issue
+// for 35 %: the softmax and the operand reads are not hidden, with one wave a SIMD (D = 256: 128 accumulator and 64 query
+// registers; two workgroups a CU spill, 1,065 us).
 #include <type_traits>
 
 #include "attend.h"

@@ -250,7 +250,7 @@ __device__ __forceinline__ void split4(const floatx4& x, uint2 (&planes)[P]) {
   }
 }
 
-// (chunk slot, v head): one workgroup. Measured: 120 us for the 128 chunks x 48 heads of an 8192-token
+// (chunk slot, v head): one workgroup. Measured: 121 us for the 128 chunks x 48 heads of an 8192-token
 // prompt; with LDS of their own for T and L, two workgroups a CU, 169.
 template <int DT, int DK, int C>
 __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkWs ws) {
@@ -479,9 +479,10 @@ __global__ void __launch_bounds__(256) prep_kernel(DeltaArgs a, int most, ChunkW
 // 8 consecutive values of step s of a right operand, so planes are written as they are read, 16
 // bytes a lane; only the left operands' rows are taken in that order.
 //
-// Bound: for one sequence of 48 heads (192 workgroups), the fetch of a chunk's 64 KB of operands, which arrive at some
-// 25 bytes a cycle and CU, then the chain S k -> X -> U -> S. Measured: 472 us for 8192 tokens, 3.7 us a chunk; one wave
-// for 16 columns, without the barriers but with all of a chunk's work on one SIMD, took 650.
+// Bound: for one sequence of 48 heads (192 workgroups), latency: the chain S k -> X -> U -> S, with the fetch of a chunk's
+// 64 KB of operands beside its second half only; by counters the matrix cores of its CUs are busy for 16 % of the time.
+// Measured: 493 us for 8192 tokens, 3.9 us a chunk; one wave for 16 columns, without the barriers but with all of a chunk's
+// work on one SIMD, took 650.
 template <int DT, int DK, int C>
 __global__ void __launch_bounds__((64 * Layout<DT, DK, C>::WAVES), 1) scan_kernel(DeltaArgs a, int most, ChunkWs ws) {
   typedef Layout<DT, DK, C> Lay;

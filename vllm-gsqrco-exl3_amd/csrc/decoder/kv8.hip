@@ -29,8 +29,9 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
 // magnitude (as bits of |x|: unsigned order puts inf and NaN on top, so they reach the scale), then,
 // where the scale grew, the older codes, then the new ones. The second read of the values is from L2.
 //
-// Bound: HBM, 2 B in and 1 B out a value; at a token a sequence the launch's latency. Measured with kv8_read:
-// 8192 tokens of 4 heads of 256 in bf16 35 us, 101 MB, 2.9 TB/s; 32 sequences of one token 13 us.
+// Bound: HBM, 2 B in and 1 B out a value, and for a prompt the second pass, in which of V half of the threads have no piece
+// (pages of 64, heads of 256); at a token a sequence the launch's latency. Measured: 8192 tokens of 4 heads of 256 in bf16
+// 24 us, 50 MB, 2.1 TB/s; 32 sequences of one token 5.5 us.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) append_kernel(Kv8 c, const void* __restrict__ key, int64_t kt, int64_t kh,
                                                           const void* __restrict__ value, int64_t vt, int64_t vh,
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Kv8 c, const void* __r
 
 // One workgroup reads 64 cache positions, aligned to 16, of one (sequence, head) of K or V. A thread takes 16 positions x 8 dims: of K
 // eight bytes a position, of V sixteen a dim, turned in its registers. Bound: HBM, 1 B in, 2 B out a value (16-bit rows).
+// Measured: 8192 tokens of 4 heads of 256 as bf16 12 us, 50 MB, 4.1 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) read_kernel(Kv8 c, const int32_t* __restrict__ starts, Ragged rows,
                                                         void* __restrict__ kout, void* __restrict__ vout) {
