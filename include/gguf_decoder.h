@@ -98,8 +98,8 @@ GGUF_DEC_API int gguf_kv8_read(const gguf_kv8_cache* cache, const gguf_tensor* b
                                const gguf_tensor* v_out, void* stream);
 
 /* Causal attention of the rows of query (fp16 / bf16 [tokens, q_heads, d], unit inner stride, rows
- * 16-byte aligned; q_heads a multiple of the cache's heads) over the cache, which holds their own
- * tokens already: row i of sequence s sees positions 0 .. seq_lens[s] - n_s + i, so
+ * 16-byte aligned; q_heads a multiple of the cache's heads; sequences times heads below 2^24) over the cache, which
+ * holds their own tokens already: row i of sequence s sees positions 0 .. seq_lens[s] - n_s + i, so
  * out = softmax(scale * q k^T) v. A row that sees nothing is 0; one that sees a page whose number is
  * out of range is NaN. out: contiguous, like query. The workspace holds the partial results of a
  * cache split over workgroups; with fewer bytes than gguf_kv8_attention_workspace_bytes (0 included) the

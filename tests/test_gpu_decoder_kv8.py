@@ -595,3 +595,20 @@ def test_attention_gives_numbers(dec, news, hq, heads, d, page, dtype):
     ends = (1 if news[0] == 1 else 5, 65, 200, 777)
     q, cache, table, y = _run_attention(dec, ends, news, hq, heads, d, page, dtype, 37)
     _near(y, *_attention_ref(q, cache, table, ends, news, d ** -0.5))
+
+
+def test_attention_of_many_short_sequences(dec):
+    """More than 65,535 (sequence, head) pairs in a decode step; all sequences lie in the same pages, up to a length of their own."""
+    g = torch.Generator().manual_seed(38)
+    seqs, heads, d, page, longest = 9001, 8, 64, 16, 40
+    cache = _random_cache(dec, 3, heads, page, d, g)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda").expand(seqs, 3).contiguous()
+    lens = (torch.arange(seqs) % longest + 1).to(torch.int32).cuda()
+    q = (torch.randn(seqs, 2 * heads, d, generator=g) * 0.3).to(torch.bfloat16).cuda()
+    y = dec.kv8_attention(q, cache, table, lens, _cu((1,) * seqs), 1, longest)
+    k, v = (x.repeat_interleave(2, 0) for x in _values(cache, table, 0, longest))
+    x = torch.matmul(q.double().transpose(0, 1), k.transpose(1, 2).contiguous()) * d ** -0.5  # [heads, seqs, tokens]
+    x.masked_fill_(torch.arange(longest, device="cuda") >= lens[:, None], -math.inf)
+    ref = torch.matmul(torch.softmax(x, -1), v).transpose(0, 1)
+    seen = v.abs().amax(-1).cummax(-1).values  # [heads, tokens]
+    _near(y, ref, seen.T[lens.long() - 1][..., None])

@@ -263,7 +263,8 @@ int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, co
     return GGUF_DEC_EINVAL;
   if (query->size[2] != c.d) return fail("%s: query has head size %lld, the cache %d", op, (long long)query->size[2], c.d);
   if (query->size[1] < 1 || query->size[1] % c.heads) return fail("%s: %lld query heads are no multiple of the cache's %d", op, (long long)query->size[1], c.heads);
-  if ((int64_t)rows.seqs * c.heads > 65535) return fail("%s: sequences times heads must be at most 65535", op);
+  if ((int64_t)rows.seqs * c.heads >= (1 << 24))  // a grid holds fewer than 2^32 threads, 256 each
+    return fail("%s: sequences times heads must be below 2^24", op);
   if (query->size[0] > 0 && !rows_ok(query)) return fail("%s: query needs unit inner stride and 16-byte aligned rows", op);
   if (out->dtype != query->dtype || out->size[0] != query->size[0] || out->size[1] != query->size[1] || out->size[2] != query->size[2] ||
       !contiguous(out) || (out->size[0] > 0 && !aligned(out, 16)))
