@@ -612,3 +612,27 @@ def test_attention_of_many_short_sequences(dec):
     ref = torch.matmul(torch.softmax(x, -1), v).transpose(0, 1)
     seen = v.abs().amax(-1).cummax(-1).values  # [heads, tokens]
     _near(y, ref, seen.T[lens.long() - 1][..., None])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("news", [3, 70])
+def test_attention_queries_with_a_strong_element(dec, news, dtype):
+    """One element 300 times the others. With many rows the others keep 2^-15 of it: that much of the keys' sums of a score, and
+    twice as much of a weight, at most, on top of the usual bound."""
+    g = torch.Generator().manual_seed(39)
+    hq, heads, page, d, end = 6, 2, 16, 128, 300
+    cache = _random_cache(dec, 20, heads, page, d, g)
+    cache.k[..., 9] = torch.randint(-3, 4, (20, heads, page), generator=g).to(torch.int8)
+    table = _table((end,), page, 20, g)
+    q = torch.randn(news, hq, d, generator=g) * 0.1
+    q[..., 9] = 30.0
+    q = q.to(dtype).cuda()
+    y = dec.kv8_attention(q, cache, table, _i32(end), _cu((news,)), news, end)
+    ref, most = _attention_ref(q, cache, table, (end,), (news,), d ** -0.5)
+    room = 0.0
+    if news * hq // heads > 64:
+        sums = _values(cache, table, 0, end)[0].abs().sum(-1).amax()
+        room = 2 * 2.0 ** -15 * 30.0 * float(sums) * d ** -0.5
+    assert not y.isnan().any()
+    eps = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    assert ((y.double() - ref).abs() <= eps * ref.abs() + (2.0 ** -10 + room) * most).all()
