@@ -2,6 +2,9 @@
  * linear layers (libgguf_mi355x.so) and behind its head.
  *
  *   gguf_kv8_append, gguf_kv8_read, gguf_kv8_attention   a paged KV cache in 8 bits, and attention over it
+ *   gguf_kv8_rotary_append                               the position rotation on the way into that cache
+ *   gguf_kv8_tree_attention, gguf_kv8_keep               attention for a tree of drafts, and keeping a path of it
+ *   gguf_residual_norm                                   norms before and after a block, its gate and residual
  *   gguf_gated_delta_rule                                linear attention: recurrent and chunked
  *   gguf_token_logprobs                                  log probabilities, entropy and best tokens
  *
@@ -115,6 +118,54 @@ GGUF_DEC_API int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cac
                                     const gguf_tensor* block_table, const gguf_tensor* seq_lens,
                                     const gguf_tensor* cu_seqlens, int64_t max_new, int64_t max_len, float scale,
                                     const gguf_tensor* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* kv8_append with the position rotation of keys, and of the queries beside them, on the way, after the norms of their heads
+ * where these have weights. query [tokens, q_heads, d] (any number of heads), key, value: one float dtype, unit inner stride, rows
+ * 16-byte aligned; the sequences times the cache's heads below 2^22. For a head's row x of query (w = q_weight) or key
+ * (w = k_weight; fp32 [d], 16-byte aligned; NULL: no norm)
+ *   x = x / sqrt(mean(x^2) + eps) * w
+ *   x_i, x_j = x_i c - x_j s, x_j c + x_i s   for the pairs (i, j = i + r / 2), i < r / 2; interleaved: (2 i', j = 2 i' + 1)
+ * with c and s at cos_sin[positions[token], i] and [.., r / 2 + i] (i' where interleaved). cos_sin: fp32 [positions, r], r a
+ * multiple of 16 up to d (dims from r on do not turn), unit inner stride, rows 16-byte aligned; positions: int64 [tokens],
+ * where a tree of drafts has its depths. A position out of the table's range turns by NaN. Everything is fp32; query_out (contiguous, 16-byte
+ * aligned, like query) is rounded once, a key is rounded to its code only. All rows of query are turned,
+ * those of no sequence too. Keys and values enter the cache as by gguf_kv8_append. */
+GGUF_DEC_API int gguf_kv8_rotary_append(const gguf_kv8_cache* cache, const gguf_tensor* query, const gguf_tensor* key,
+                                        const gguf_tensor* value, const gguf_tensor* cos_sin, const gguf_tensor* positions,
+                                        const gguf_tensor* block_table, const gguf_tensor* seq_lens,
+                                        const gguf_tensor* cu_seqlens, int64_t max_new, int interleaved,
+                                        const gguf_tensor* q_weight, const gguf_tensor* k_weight, float eps,
+                                        const gguf_tensor* query_out, void* stream);
+
+/* kv8_attention for a tree of drafts: row i of sequence s sees positions 0 .. b - 1, b = seq_lens[s] - n_s, and of the sequence's
+ * own rows j (at positions b + j) those with bit j % 64 of tree_mask[row, j / 64] set (int64 [tokens, words], unit inner
+ * stride; rows past 64 * words are not seen). Usually these are a draft's ancestors and itself, but any bits are allowed. Otherwise
+ * as gguf_kv8_attention, whose workspace it takes. */
+GGUF_DEC_API int gguf_kv8_tree_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, const gguf_tensor* tree_mask,
+                                         const gguf_tensor* block_table, const gguf_tensor* seq_lens,
+                                         const gguf_tensor* cu_seqlens, int64_t max_new, int64_t max_len, float scale,
+                                         const gguf_tensor* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Keeps a path of a tree of drafts: of sequence s's n_s last positions b .. seq_lens[s] - 1, row path[s, j] moves to position
+ * b + j, in the cache alone (int32 [sequences, m], unit inner stride, m up to 1024; sequences times heads below 2^22). A path grows strictly and ends
+ * before its first entry that is out of range or does not; what lies behind its last place is no longer the sequence's (the
+ * caller's next seq_lens says so) and may have changed. Within a page codes move as they are; from another page they are rounded
+ * to the page's scale, which grows where the moved rows need it, and the page's other codes then are rounded again to it, as
+ * by gguf_kv8_append. A row from a page whose number is out of range makes the page that receives it NaN; one that would go to such a page is dropped. */
+GGUF_DEC_API int gguf_kv8_keep(const gguf_kv8_cache* cache, const gguf_tensor* path, const gguf_tensor* block_table,
+                               const gguf_tensor* seq_lens, const gguf_tensor* cu_seqlens, void* stream);
+
+/* The norm behind a block, its gate, the residual, and the next block's norm, row by row over the last dimension n of x
+ * (fp32 / fp16 / bf16 [rows, n] or [rows, heads, n], unit inner stride; any other strides, 0 included). Each part may be NULL:
+ *   u = x;   u = u / sqrt(mean(u^2) + eps) * inner_weight;   u = u * act(gate);   h = residual + scale * u
+ *   out = h / sqrt(mean(h^2) + eps) * weight
+ * act: 0 the gate itself, 1 its sigmoid, 2 silu. gate: like x (other strides); residual: x's shape, x's dtype or fp32; weights: fp32 [n].
+ * hidden (h): contiguous, residual's dtype (x's without one); out: contiguous, x's dtype, not read or written without weight. Neither
+ * overlaps an input. Everything between is fp32: out comes from h before its rounding. Squares are summed in fp32, so a row of
+ * magnitudes beyond 2^63 is taken for infinite. */
+GGUF_DEC_API int gguf_residual_norm(const gguf_tensor* x, const gguf_tensor* residual, const gguf_tensor* gate, int act,
+                                    const gguf_tensor* inner_weight, const gguf_tensor* weight, float scale, float eps,
+                                    const gguf_tensor* hidden, const gguf_tensor* out, void* stream);
 
 /* The gated delta rule over ragged sequences. q, k: [tokens, hk, dk], v: [tokens, hv, dv] of one
  * float dtype (unit inner stride, rows 16-byte aligned; hv a multiple of hk; dk 64 or 128, dv a

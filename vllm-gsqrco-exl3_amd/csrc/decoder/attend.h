@@ -103,7 +103,30 @@ struct AttnArgs {
   void* out;       // [tokens, hq, d]
   float* part;     // of a split call: [splits][tokens * hq][d] sums, then m and l: [splits][tokens * hq][2]
   float* stat;
+  const int64_t* mask;  // of a tree: [tokens][words], or null
+  int64_t mask_stride;
+  int words;
 };
+
+// What a row of a tree sees of the 16-token chunk at position `at` (a multiple of 16), a bit a token: of positions before `base` all,
+// of the sequence's own rows from there on what the row's mask says, up to `count`; nothing from the table's capacity `room` on.
+__device__ __forceinline__ uint32_t tree_bits(const int64_t* mask, int at, int64_t base, int64_t count, int64_t room) {
+  if (at >= room) return 0;
+  const int64_t from = at - base;
+  if (from >= count) return from < 0 ? (1u << (int)min(-from, (int64_t)16)) - 1 : 0;
+  if (from <= -16) return 0xFFFF;
+  uint64_t w;
+  if (from < 0) {
+    w = (uint64_t)mask[0] << -from;
+  } else {
+    const int64_t i = from >> 6;
+    const int bit = (int)(from & 63);
+    w = (uint64_t)mask[i] >> bit;
+    if (bit > 48 && 64 * (i + 1) < count) w |= (uint64_t)mask[i + 1] << (64 - bit);
+  }
+  if (count - from < 16) w &= (1u << (int)(count - from)) - 1;
+  return (uint32_t)(w | (from < 0 ? (1u << -from) - 1 : 0)) & 0xFFFF;
+}
 
 // attention_rows.hip: many rows
 constexpr int kRowsTile = 128;  // rows of a workgroup

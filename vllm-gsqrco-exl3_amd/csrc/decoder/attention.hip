@@ -24,7 +24,9 @@ constexpr int kSegment = 64;  // tiles whose chunks are looked up at a time
 // 16384 tokens 235 us a call (989 MB, 4.2 TB/s; before a wave's next tile was fetched ahead 444); one of 701 tokens 14 us,
 // of which this kernel is 12, latency. At head sizes from 128 on a workgroup takes 16 rows: of 256, 32 spill, and this kernel took 148 us for 8
 // sequences of 4 rows over up to 32768 tokens, 104 (the call 117) with the cache read for two row tiles; see attn_plan for the others.
-template <int DT, int D, int NT>
+//
+// TREE: the rows are drafts. They see the positions before the sequence's own rows, and of these what their mask says.
+template <int DT, int D, int NT, bool TREE>
 __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   constexpr int S = D / 64, DD = D / 16;
   extern __shared__ __align__(16) float lds[];  // [kWaves][DD][NT][64][4]
@@ -42,11 +44,13 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
   const int64_t room = (int64_t)a.c.max_pages * a.c.page;
   const int page16 = a.c.page / 16;
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
+  const int64_t base = (int64_t)len0 - (r1 - r0);  // position of the sequence's first row
+  const int64_t drafts = TREE ? min((int64_t)(r1 - r0), (int64_t)64 * a.words) : 0;
 
   for (int64_t tile0 = (int64_t)blockIdx.y * 16 * NT; tile0 < nrows; tile0 += (int64_t)gridDim.y * 16 * NT) {
     // what the tile's rows see at most: they are in order of their tokens
     const int64_t rlast = min(nrows, tile0 + 16 * NT) - 1;
-    const int see = (int)max(min((int64_t)len0 - (r1 - r0) + rlast / a.group, room - 1), (int64_t)-1);
+    const int see = (int)max(min(TREE ? (int64_t)len0 - 1 : (int64_t)len0 - (r1 - r0) + rlast / a.group, room - 1), (int64_t)-1);
     const int ntiles = (see + kTile) / kTile;  // see = -1: none
     const int tb = (int)min((int64_t)split * (a.span / kTile), (int64_t)ntiles);
     const int te = split == splits - 1 ? ntiles : min(ntiles, tb + a.span / kTile);
@@ -55,8 +59,9 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
         chunks[i] = chunk_of(a.c, table, page16, head, (int64_t)4 * from + i, see);
     };
     find_chunks(tb, min(tb + kSegment, te));  // (the previous rows are through: see the loop's end)
-    // rows of this tile: row -> (token, head); last: the last position that it sees
+    // rows of this tile: row -> (token, head); last: the last position that it sees (of a tree: before the mask's)
     int64_t qrow[NT];
+    const int64_t* mask[NT];
     int last[NT];
     int all = 0x7FFFFFFF;  // the last position that every row sees
     half8 q[NT][2 * S];
@@ -67,7 +72,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
       const bool ok = r < nrows;
       const int tok = ok ? (int)(r / a.group) : 0, h = head * a.group + (ok ? (int)(r % a.group) : 0);
       qrow[t] = ok ? (int64_t)(r0 + tok) * a.hq + h : -1;
-      const int64_t l = ok ? (int64_t)len0 - (r1 - r0) + tok : -1;
+      const int64_t l = ok ? (int64_t)len0 - (r1 - r0) + (TREE ? -1 : tok) : -1;
+      if constexpr (TREE) mask[t] = a.mask + (int64_t)(r0 + tok) * a.mask_stride;
       last[t] = (int)(l < room ? l : room - 1);
       if (ok) all = min(all, last[t]);
       float amax = 0.0f;
@@ -155,17 +161,19 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
 
       const bool masked = kTile * tile + kTile - 1 > all;
       float nm[NT], own[NT];  // own: the V scale of the lane's chunk, if the row sees it
+      uint32_t bits[NT];      // of a tree: the tokens of the lane's chunk that the row sees
       bool grown = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float f = qs[t] * ks;
         float mx = kNoScore;
+        if constexpr (TREE) bits[t] = masked ? tree_bits(mask[t], kTile * tile + 16 * g, base, drafts, room) : 0xFFFF;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float x = sc[tt][t][i] * f;
-            if (masked && kTile * tile + 16 * g + 4 * tt + i > last[t]) x = -__builtin_inff();
+            if (TREE ? !(bits[t] >> (4 * tt + i) & 1) : masked && kTile * tile + 16 * g + 4 * tt + i > last[t]) x = -__builtin_inff();
             sc[tt][t][i] = x;
             mx = fmaxf(mx, x);
           }
@@ -173,7 +181,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attend_kernel(AttnArgs a) {
         // where the largest V scale grew
         mx = group_max(mx);
         nm[t] = mx > m[t] + 8.0f ? mx : m[t];
-        own[t] = masked && kTile * tile + 16 * g > last[t] ? 0.0f : vs;
+        own[t] = (TREE ? bits[t] == 0 : masked && kTile * tile + 16 * g > last[t]) ? 0.0f : vs;
         grown = grown || nm[t] != m[t] || own[t] > ref[t];
       }
       if (__any(grown)) {
@@ -312,7 +320,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
   }
 }
 
-template <int DT, int D, int NT>
+template <int DT, int D, int NT, bool TREE>
 hipError_t launch_attend(const AttnArgs& a, dim3 grid, hipStream_t stream) {
   constexpr int lds = kWaves * D * 16 * NT * 4;
   int dev = 0;
@@ -320,9 +328,9 @@ hipError_t launch_attend(const AttnArgs& a, dim3 grid, hipStream_t stream) {
   if (e != hipSuccess) return e;
   struct Tag {};
   gguf::once_per_device<Tag>(dev, [&] {
-    (void)hipFuncSetAttribute((const void*)attend_kernel<DT, D, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    (void)hipFuncSetAttribute((const void*)attend_kernel<DT, D, NT, TREE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   });
-  attend_kernel<DT, D, NT><<<grid, 64 * kWaves, lds, stream>>>(a);
+  attend_kernel<DT, D, NT, TREE><<<grid, 64 * kWaves, lds, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -373,21 +381,22 @@ size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t
 
 hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t qt, int64_t qh, int hq,
                                 const int32_t* lens, const Ragged& rows, int64_t max_new, int64_t max_len, float scale,
-                                void* out, void* ws, size_t ws_bytes, hipStream_t stream) {
+                                const int64_t* mask, int64_t mask_stride, int words, void* out, void* ws, size_t ws_bytes,
+                                hipStream_t stream) {
   const int64_t all = (int64_t)rows.tokens * hq;
   const int64_t fit = (int64_t)(ws_bytes / sizeof(float)) / (all * (c.d + 2));
   const AttnPlan p = attn_plan(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len,
                                fit < 2 ? 1 : std::min(fit, most_splits(all)));
   const AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, p.span, p.splits, out, (float*)ws,
-                   (float*)ws + (size_t)p.splits * all * c.d};
+                   (float*)ws + (size_t)p.splits * all * c.d, mask, mask_stride, words};
   const dim3 grid((unsigned)(rows.seqs * c.heads * p.splits), (unsigned)(p.row_tiles < 65535 ? p.row_tiles : 65535));
   hipError_t e = hipSuccess;
   if (p.many) e = launch_attend_rows(a, dtype, p.row_tiles, stream);
 #define GGUF_DEC_ATTEND(DT, D)                                                                                         \
   {                                                                                                                    \
-    if (!p.many && p.nt == 1) e = launch_attend<DT, D, 1>(a, grid, stream);                                            \
+    if (!p.many && p.nt == 1) e = mask ? launch_attend<DT, D, 1, true>(a, grid, stream) : launch_attend<DT, D, 1, false>(a, grid, stream); \
     if constexpr (D < 128)                                                                                             \
-      if (!p.many && p.nt == 2) e = launch_attend<DT, D, 2>(a, grid, stream);                                          \
+      if (!p.many && p.nt == 2) e = mask ? launch_attend<DT, D, 2, true>(a, grid, stream) : launch_attend<DT, D, 2, false>(a, grid, stream); \
     if (e == hipSuccess && p.splits > 1)                                                                               \
       join_kernel<DT, D><<<(unsigned)all, 256, 0, stream>>>(a.part, a.stat, all, p.splits, out);           \
   }

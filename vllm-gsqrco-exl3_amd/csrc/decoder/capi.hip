@@ -8,6 +8,8 @@
 
 #include "../../../include/gguf_decoder.h"
 #include "delta.h"
+#include "norm.h"
+#include "rotary.h"
 
 namespace gguf_dec {
 hipError_t launch_kv8_append(const Kv8& c, int dtype, const void* key, int64_t kt, int64_t kh, const void* value,
@@ -19,7 +21,12 @@ size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t
                                int64_t max_len);
 hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t qt, int64_t qh, int hq,
                                 const int32_t* lens, const Ragged& rows, int64_t max_new, int64_t max_len, float scale,
-                                void* out, void* ws, size_t ws_bytes, hipStream_t stream);
+                                const int64_t* mask, int64_t mask_stride, int words, void* out, void* ws, size_t ws_bytes,
+                                hipStream_t stream);
+hipError_t launch_kv8_rotary(const RotaryArgs& a, int dtype, int64_t max_new, hipStream_t stream);
+hipError_t launch_kv8_keep(const Kv8& c, const int32_t* path, int64_t path_stride, int m, const int32_t* lens,
+                           const Ragged& rows, hipStream_t stream);
+hipError_t launch_norm(const NormArgs& a, int dtype, int residual_dtype, bool wide, hipStream_t stream);
 size_t delta_workspace(int dtype, int dk, int hk, int hv, int64_t tokens, int64_t seqs, int64_t max_new, bool steps);
 hipError_t launch_delta(const DeltaArgs& a, int dtype, int dk, int64_t max_new, void* ws, hipStream_t stream);
 int64_t logprobs_most_vocab(int64_t top);
@@ -249,11 +256,12 @@ size_t gguf_kv8_attention_workspace_bytes(const gguf_kv8_cache* cache, const ggu
                                            query->size[0], seqs, bounded(max_new, query->size[0]), bounded(max_len, INT_MAX));
 }
 
-int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, const gguf_tensor* block_table,
-                       const gguf_tensor* seq_lens, const gguf_tensor* cu_seqlens, int64_t max_new, int64_t max_len,
-                       float scale, const gguf_tensor* out, void* workspace, size_t workspace_bytes, void* stream) {
+// kv8_attention, or with a mask kv8_tree_attention
+static int attention(const char* op, const gguf_tensor* query, const gguf_kv8_cache* cache, const gguf_tensor* mask, bool tree,
+                     const gguf_tensor* block_table, const gguf_tensor* seq_lens, const gguf_tensor* cu_seqlens, int64_t max_new,
+                     int64_t max_len, float scale, const gguf_tensor* out, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   begin();
-  const char* op = "kv8_attention";
   if (!shaped(query, 3) || !shaped(out, 3)) return fail("%s: query and out must be [tokens, heads, head size]", op);
   if (!is_half(query->dtype)) return fail("%s: query must be fp16 or bf16", op);
   Ragged rows;
@@ -266,22 +274,173 @@ int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, co
   if ((int64_t)rows.seqs * c.heads >= (1 << 24))  // a grid holds fewer than 2^32 threads, 256 each
     return fail("%s: sequences times heads must be below 2^24", op);
   if (query->size[0] > 0 && !rows_ok(query)) return fail("%s: query needs unit inner stride and 16-byte aligned rows", op);
+  if (tree && (!shaped(mask, 2) || mask->dtype != GGUF_DEC_I64 || mask->size[0] != query->size[0] || mask->size[1] < 1 ||
+               mask->size[1] > (1 << 24) || (mask->size[1] > 1 && mask->stride[1] != 1)))
+    return fail("%s: tree_mask must be int64 [tokens, words] with unit inner stride", op);
+  if (tree && !aligned(mask, 8)) return fail("%s: tree_mask must be 8-byte aligned", op);
   if (out->dtype != query->dtype || out->size[0] != query->size[0] || out->size[1] != query->size[1] || out->size[2] != query->size[2] ||
       !contiguous(out) || (out->size[0] > 0 && !aligned(out, 16)))
     return fail("%s: out must be contiguous, 16-byte aligned, with query's shape and dtype", op);
   if (max_new < 0 || max_len < 0) return fail("%s: max_new and max_len must not be negative", op);
   if (!std::isfinite(scale)) return fail("%s: scale must be finite", op);
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail("%s: workspace must be 16-byte aligned", op);
-  if (!same_device(query->device, out, &cache->k, seq_lens, cu_seqlens)) return fail("%s: tensors on different devices", op);
-  if (!present(query, out, seq_lens, cu_seqlens)) return fail("%s: a tensor has no data", op);
+  if (!same_device(query->device, out, &cache->k, seq_lens, cu_seqlens, mask)) return fail("%s: tensors on different devices", op);
+  if (!present(query, out, seq_lens, cu_seqlens, mask)) return fail("%s: a tensor has no data", op);
   if (query->device < 0) return fail("%s: tensors must be CUDA tensors", op);
   if (query->size[0] == 0) return GGUF_DEC_OK;
   const DeviceScope scope(query->device);
   if (scope.err != hipSuccess) return hip_fail(scope.err, op);
   const hipError_t e = gguf_dec::launch_kv8_attention(
       c, query->dtype, query->data, stride_of(query, 0), stride_of(query, 1), (int)query->size[1], (const int32_t*)seq_lens->data,
-      rows, bounded(max_new, query->size[0]), bounded(max_len, INT_MAX), scale, out->data, workspace, workspace ? workspace_bytes : 0,
+      rows, bounded(max_new, query->size[0]), bounded(max_len, INT_MAX), scale, tree ? (const int64_t*)mask->data : nullptr,
+      tree ? stride_of(mask, 0) : 0, tree ? (int)mask->size[1] : 0, out->data, workspace, workspace ? workspace_bytes : 0,
       (hipStream_t)stream);
+  return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
+}
+
+int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, const gguf_tensor* block_table,
+                       const gguf_tensor* seq_lens, const gguf_tensor* cu_seqlens, int64_t max_new, int64_t max_len,
+                       float scale, const gguf_tensor* out, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention("kv8_attention", query, cache, nullptr, false, block_table, seq_lens, cu_seqlens, max_new, max_len, scale, out,
+                   workspace, workspace_bytes, stream);
+}
+
+int gguf_kv8_tree_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, const gguf_tensor* tree_mask,
+                            const gguf_tensor* block_table, const gguf_tensor* seq_lens, const gguf_tensor* cu_seqlens,
+                            int64_t max_new, int64_t max_len, float scale, const gguf_tensor* out, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  return attention("kv8_tree_attention", query, cache, tree_mask, true, block_table, seq_lens, cu_seqlens, max_new, max_len, scale,
+                   out, workspace, workspace_bytes, stream);
+}
+
+int gguf_kv8_rotary_append(const gguf_kv8_cache* cache, const gguf_tensor* query, const gguf_tensor* key,
+                           const gguf_tensor* value, const gguf_tensor* cos_sin, const gguf_tensor* positions,
+                           const gguf_tensor* block_table, const gguf_tensor* seq_lens, const gguf_tensor* cu_seqlens,
+                           int64_t max_new, int interleaved, const gguf_tensor* q_weight, const gguf_tensor* k_weight, float eps,
+                           const gguf_tensor* query_out, void* stream) {
+  begin();
+  const char* op = "kv8_rotary_append";
+  if (!shaped(query, 3) || !shaped(key, 3) || !shaped(value, 3)) return fail("%s: query, key and value must be [tokens, heads, head size]", op);
+  if (!is_float(key->dtype) || value->dtype != key->dtype || query->dtype != key->dtype) return fail("%s: query, key and value must share one float dtype", op);
+  const int64_t t = key->size[0];
+  Ragged rows;
+  Kv8 c;
+  if (check_cu(op, cu_seqlens, t, &rows) || check_cache(op, cache, block_table, rows.seqs, &c) ||
+      check_seq_ints(op, "seq_lens", seq_lens, rows.seqs))
+    return GGUF_DEC_EINVAL;
+  for (const gguf_tensor* x : {key, value})
+    if (x->size[0] != t || x->size[1] != c.heads || x->size[2] != c.d)
+      return fail("%s: key and value must be [tokens, %d, %d] for this cache", op, c.heads, c.d);
+  if (query->size[0] != t || query->size[1] < 1 || query->size[2] != c.d) return fail("%s: query must be [tokens, heads, %d] with key's tokens", op, c.d);
+  if (t > 0 && (!rows_ok(query) || !rows_ok(key) || !rows_ok(value)))
+    return fail("%s: query, key and value need unit inner stride and 16-byte aligned rows", op);
+  if ((int64_t)rows.seqs * c.heads >= (1 << 22)) return fail("%s: sequences times heads must be below 2^22", op);
+  if (!shaped(cos_sin, 2) || cos_sin->dtype != GGUF_DEC_F32 || cos_sin->size[0] < 1 || cos_sin->size[1] < 16 || cos_sin->size[1] % 16 ||
+      cos_sin->size[1] > c.d || cos_sin->stride[1] != 1 || !aligned(cos_sin, 16) || stride_of(cos_sin, 0) % 4)
+    return fail("%s: cos_sin must be fp32 [positions, 16 .. %d in steps of 16] with unit inner stride and 16-byte aligned rows", op, c.d);
+  if (!shaped(positions, 1) || positions->dtype != GGUF_DEC_I64 || positions->size[0] != t || !contiguous(positions) || !aligned(positions, 8))
+    return fail("%s: positions must be a contiguous int64 [tokens]", op);
+  for (const gguf_tensor* w : {q_weight, k_weight})
+    if (w && (!shaped(w, 1) || w->dtype != GGUF_DEC_F32 || w->size[0] != c.d || !contiguous(w) || !aligned(w, 16)))
+      return fail("%s: q_weight and k_weight must be contiguous, 16-byte aligned fp32 of %d values", op, c.d);
+  if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail("%s: eps must be finite and not negative", op);
+  if (!shaped(query_out, 3) || query_out->dtype != query->dtype || query_out->size[0] != t || query_out->size[1] != query->size[1] ||
+      query_out->size[2] != c.d || !contiguous(query_out) || (t > 0 && !aligned(query_out, 16)))
+    return fail("%s: query_out must be contiguous, 16-byte aligned, with query's shape and dtype", op);
+  if (max_new < 0) return fail("%s: max_new must not be negative", op);
+  if (!same_device(key->device, query, value, cos_sin, positions, &cache->k, seq_lens, cu_seqlens, q_weight, k_weight, query_out))
+    return fail("%s: tensors on different devices", op);
+  if (!present(query, key, value, cos_sin, positions, seq_lens, cu_seqlens, q_weight, k_weight, query_out)) return fail("%s: a tensor has no data", op);
+  if (key->device < 0) return fail("%s: tensors must be CUDA tensors", op);
+  if (t == 0) return GGUF_DEC_OK;
+  const DeviceScope scope(key->device);
+  if (scope.err != hipSuccess) return hip_fail(scope.err, op);
+  const gguf_dec::RotaryArgs a{c, query->data, key->data, value->data, stride_of(query, 0), stride_of(query, 1), stride_of(key, 0),
+                               stride_of(key, 1), stride_of(value, 0), stride_of(value, 1), q_weight ? (const float*)q_weight->data : nullptr,
+                               k_weight ? (const float*)k_weight->data : nullptr, eps, (const float*)cos_sin->data, stride_of(cos_sin, 0),
+                               cos_sin->size[0], (const int64_t*)positions->data, (int)cos_sin->size[1], interleaved != 0,
+                               (const int32_t*)seq_lens->data, rows, (int)query->size[1], query_out->data};
+  const hipError_t e = gguf_dec::launch_kv8_rotary(a, key->dtype, bounded(max_new, t), (hipStream_t)stream);
+  return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
+}
+
+int gguf_kv8_keep(const gguf_kv8_cache* cache, const gguf_tensor* path, const gguf_tensor* block_table, const gguf_tensor* seq_lens,
+                  const gguf_tensor* cu_seqlens, void* stream) {
+  begin();
+  const char* op = "kv8_keep";
+  Ragged rows;
+  Kv8 c;
+  if (check_cu(op, cu_seqlens, INT_MAX, &rows) || check_cache(op, cache, block_table, rows.seqs, &c) ||
+      check_seq_ints(op, "seq_lens", seq_lens, rows.seqs))
+    return GGUF_DEC_EINVAL;
+  if (!shaped(path, 2) || path->dtype != GGUF_DEC_I32 || path->size[0] != rows.seqs || (path->size[1] > 1 && path->stride[1] != 1))
+    return fail("%s: path must be int32 [sequences, rows] with unit inner stride", op);
+  if (path->size[1] > gguf_dec::kMostKept) return fail("%s: a path of %lld rows is longer than %d", op, (long long)path->size[1], gguf_dec::kMostKept);
+  if ((int64_t)rows.seqs * c.heads >= (1 << 22)) return fail("%s: sequences times heads must be below 2^22", op);
+  if (!same_device(cache->k.device, path, seq_lens, cu_seqlens)) return fail("%s: tensors on different devices", op);
+  if (!present(path, seq_lens, cu_seqlens)) return fail("%s: a tensor has no data", op);
+  if (cache->k.device < 0) return fail("%s: tensors must be CUDA tensors", op);
+  if (path->size[1] == 0) return GGUF_DEC_OK;
+  const DeviceScope scope(cache->k.device);
+  if (scope.err != hipSuccess) return hip_fail(scope.err, op);
+  const hipError_t e = gguf_dec::launch_kv8_keep(c, (const int32_t*)path->data, stride_of(path, 0), (int)path->size[1],
+                                                 (const int32_t*)seq_lens->data, rows, (hipStream_t)stream);
+  return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
+}
+
+int gguf_residual_norm(const gguf_tensor* x, const gguf_tensor* residual, const gguf_tensor* gate, int act,
+                       const gguf_tensor* inner_weight, const gguf_tensor* weight, float scale, float eps, const gguf_tensor* hidden,
+                       const gguf_tensor* out, void* stream) {
+  begin();
+  const char* op = "residual_norm";
+  const int nd = x && x->ndim == 3 ? 3 : 2;
+  if (!shaped(x, nd) || !is_float(x->dtype)) return fail("%s: x must be a float [rows, n] or [rows, heads, n]", op);
+  const int64_t n = x->size[nd - 1], heads = nd == 3 ? x->size[1] : 1, rows = x->size[0] * heads;
+  if (n < 1 || heads < 1) return fail("%s: x has no columns", op);
+  if (rows > INT_MAX) return fail("%s: x has too many rows", op);
+  const auto like = [&](const gguf_tensor* t) {
+    if (!shaped(t, nd)) return false;
+    for (int i = 0; i < nd; ++i)
+      if (t->size[i] != x->size[i]) return false;
+    return true;
+  };
+  if (gate && (!like(gate) || gate->dtype != x->dtype)) return fail("%s: gate must have x's shape and dtype", op);
+  if (act < 0 || act > 2) return fail("%s: act=%d is not 0 (none), 1 (sigmoid) or 2 (silu)", op, act);
+  if (residual && (!like(residual) || (residual->dtype != x->dtype && residual->dtype != GGUF_DEC_F32)))
+    return fail("%s: residual must have x's shape, and its dtype or fp32", op);
+  for (const gguf_tensor* w : {inner_weight, weight})
+    if (w && (!shaped(w, 1) || w->dtype != GGUF_DEC_F32 || w->size[0] != n || !contiguous(w) || !aligned(w, 4)))
+      return fail("%s: weights must be contiguous fp32 of %lld values", op, (long long)n);
+  const int rdt = residual ? residual->dtype : x->dtype;
+  if (!like(hidden) || hidden->dtype != rdt || !contiguous(hidden) || !aligned(hidden, size_of(rdt)))
+    return fail("%s: hidden must be contiguous, with x's shape and residual's dtype", op);
+  if (weight && (!like(out) || out->dtype != x->dtype || !contiguous(out) || !aligned(out, size_of(x->dtype))))
+    return fail("%s: out must be contiguous, with x's shape and dtype", op);
+  for (const gguf_tensor* t : {x, residual, gate})
+    if (t && ((n > 1 && t->stride[nd - 1] != 1) || !aligned(t, size_of(t->dtype))))
+      return fail("%s: x, residual and gate need unit inner stride and alignment to their elements", op);
+  if (!std::isfinite(scale) || !(eps >= 0.0f) || !std::isfinite(eps)) return fail("%s: scale must be finite, eps finite and not negative", op);
+  if (!weight) out = nullptr;
+  if (!same_device(x->device, residual, gate, inner_weight, weight, hidden, out)) return fail("%s: tensors on different devices", op);
+  if (!present(x, residual, gate, inner_weight, weight, hidden, out)) return fail("%s: a tensor has no data", op);
+  if (x->device < 0) return fail("%s: tensors must be CUDA tensors", op);
+  if (rows == 0) return GGUF_DEC_OK;
+  bool wide = n % 8 == 0;
+  for (const gguf_tensor* t : {x, residual, gate, inner_weight, weight, hidden, out}) {
+    if (!t) continue;
+    wide = wide && aligned(t, 16);
+    for (int i = 0; i + 1 < t->ndim; ++i) wide = wide && stride_of(t, i) * size_of(t->dtype) % 16 == 0;
+  }
+  const auto strides = [&](const gguf_tensor* t) {
+    return t ? gguf_dec::RowStride{stride_of(t, 0), nd == 3 ? stride_of(t, 1) : 0} : gguf_dec::RowStride{0, 0};
+  };
+  const auto data = [](const gguf_tensor* t) { return t ? t->data : nullptr; };
+  const DeviceScope scope(x->device);
+  if (scope.err != hipSuccess) return hip_fail(scope.err, op);
+  const gguf_dec::NormArgs a{x->data, data(residual), data(gate), (const float*)data(inner_weight), (const float*)data(weight),
+                             hidden->data, data(out), strides(x), strides(residual), strides(gate), rows, (int)heads, (int)n,
+                             act, scale, eps};
+  const hipError_t e = gguf_dec::launch_norm(a, x->dtype, rdt, wide, (hipStream_t)stream);
   return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
 }
 

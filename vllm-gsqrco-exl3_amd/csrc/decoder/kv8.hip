@@ -3,26 +3,13 @@
 // A (page, head) of K or of V has one scale s = amax / 127 and codes round(x / s). A page that is
 // filled over several calls keeps s >= every earlier scale, so older codes are only ever rounded
 // again to a coarser step: round(code * s_old / s_new).
-#include "dec_common.h"
+#include "kv8_codes.h"
 
 namespace gguf_dec {
 
 namespace {
 
 constexpr int kThreads = 256;
-
-// round to nearest even, at most 127 in magnitude; NaN (0 * inf of a page that is not finite) -> 0
-__device__ __forceinline__ int code_of(float x) {
-  const float r = rintf(x);
-  return r != r ? 0 : (int)fminf(fmaxf(r, -127.0f), 127.0f);
-}
-
-__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
-  uint32_t out = 0;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) out |= (uint32_t)(code_of((float)(int8_t)(w >> 8 * b) * ratio) & 0xFF) << 8 * b;
-  return out;
-}
 
 // One workgroup writes the new tokens of one (sequence, page, head) of K (blockIdx.y even) or of V
 // (odd), so no two workgroups share a scale and nothing is atomic. First the new values' largest

@@ -1,0 +1,198 @@
+// The norm behind a block, its gate and residual scale, and the next block's norm, in one pass:
+//   u = x;  u = u rsqrt(mean u^2 + eps) w_in;  u = u act(gate);  h = residual + scale u;
+//   out = h rsqrt(mean h^2 + eps) w_out
+// (every part but x optional). A row's values stay in registers from the loads to the stores, so each input is read and
+// each output written once; sums of squares are fp32, and only h and out are rounded.
+#include <algorithm>
+
+#include "norm.h"
+
+namespace gguf_dec {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float act_of(float g, int act) {
+  const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));  // of -inf: 1 / inf
+  return act == kActSilu ? g * s : act == kActSigmoid ? s : g;
+}
+
+// sum over the row's lanes (a power of two up to 64, aligned) or over the workgroup
+template <bool WG>
+__device__ __forceinline__ float row_sum(float v, int lanes, float* part) {
+  if constexpr (!WG) {
+    for (int off = 1; off < lanes; off <<= 1) v += __shfl_xor(v, off, 64);
+    return v;
+  } else {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+    const int waves = blockDim.x >> 6;
+    __syncthreads();  // the last sum's parts have been read
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+    for (int w = 1; w < waves; ++w) v += part[w];
+    return v;
+  }
+}
+
+__device__ __forceinline__ void at_row(const RowStride& s, int64_t token, int head, int64_t& at) {
+  at = token * s.t + head * s.h;
+}
+
+// A row is ITEMS pieces of 8 values a lane: `lanes` lanes of a wave take it, or (WG) the whole workgroup. Weights are held over
+// the rows that a lane takes.
+template <int DT, int RT, int ITEMS, bool WG>
+__global__ void __launch_bounds__(WG ? 1024 : 256) norm_kernel(NormArgs a, int lanes) {
+  __shared__ float part[16];
+  const int per = WG ? 1 : blockDim.x / lanes;  // rows a workgroup at a time
+  const int lane = WG ? threadIdx.x : threadIdx.x % lanes, width = WG ? blockDim.x : lanes;
+  const int mine = WG ? 0 : threadIdx.x / lanes;
+  const float over = 1.0f / (float)a.n;
+  float wi[ITEMS][8], wo[ITEMS][8];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = 8 * (lane + i * width);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) wi[i][e] = wo[i][e] = 0.0f;
+    if (c < a.n) {
+      if (a.inner) load8<kF32>(a.inner, c, wi[i]);
+      if (a.outer) load8<kF32>(a.outer, c, wo[i]);
+    }
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < a.rows; r0 += (int64_t)gridDim.x * per) {
+    const bool ok = r0 + mine < a.rows;
+    const int64_t row = ok ? r0 + mine : a.rows - 1;  // lanes past the last row take it again, and store nothing
+    const int64_t token = a.heads == 1 ? row : row / a.heads;
+    const int head = a.heads == 1 ? 0 : (int)(row - token * a.heads);
+    int64_t xa, ra, ga;
+    at_row(a.xs, token, head, xa);
+    at_row(a.rs, token, head, ra);
+    at_row(a.gs, token, head, ga);
+    float u[ITEMS][8], g[ITEMS][8], h[ITEMS][8];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = 8 * (lane + i * width);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[i][e] = h[i][e] = 0.0f, g[i][e] = 1.0f;
+      if (c < a.n) {
+        load8<DT>(a.x, xa + c, u[i]);
+        if (a.gate) load8<DT>(a.gate, ga + c, g[i]);
+        if (a.residual) load8<RT>(a.residual, ra + c, h[i]);
+      }
+    }
+    if (a.inner) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += u[i][e] * u[i][e];
+      const float by = rsqrtf(row_sum<WG>(sum, lanes, part) * over + a.eps);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[i][e] *= by * wi[i][e];
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = 8 * (lane + i * width);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (a.gate) u[i][e] *= act_of(g[i][e], a.act);
+        h[i][e] += a.scale * u[i][e];
+        if (c < a.n) sum += h[i][e] * h[i][e];
+      }
+      if (c < a.n && ok) store8<RT>(a.hidden, row * a.n + c, h[i]);
+    }
+    if (a.outer) {
+      const float by = rsqrtf(row_sum<WG>(sum, lanes, part) * over + a.eps);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = 8 * (lane + i * width);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] *= by * wo[i][e];
+        if (c < a.n && ok) store8<DT>(a.out, row * a.n + c, h[i]);
+      }
+    }
+  }
+}
+
+// Rows of any length and alignment, value by value, read again for each sum: a workgroup a row.
+template <int DT, int RT>
+__global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
+  __shared__ float part[16];
+  const float over = 1.0f / (float)a.n;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t token = row / a.heads;
+    const int head = (int)(row - token * a.heads);
+    int64_t xa, ra, ga;
+    at_row(a.xs, token, head, xa);
+    at_row(a.rs, token, head, ra);
+    at_row(a.gs, token, head, ga);
+    float by = 1.0f, sum = 0.0f;
+    if (a.inner) {
+      for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
+        const float v = load1<DT>(a.x, xa + c);
+        sum += v * v;
+      }
+      by = rsqrtf(row_sum<true>(sum, 64, part) * over + a.eps);
+    }
+    const auto hidden = [&](int c) __attribute__((always_inline)) {
+      float u = load1<DT>(a.x, xa + c);
+      if (a.inner) u *= by * a.inner[c];
+      if (a.gate) u *= act_of(load1<DT>(a.gate, ga + c), a.act);
+      return (a.residual ? load1<RT>(a.residual, ra + c) : 0.0f) + a.scale * u;
+    };
+    sum = 0.0f;
+    for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
+      const float h = hidden(c);
+      sum += h * h;
+      store1<RT>(a.hidden, row * a.n + c, h);
+    }
+    if (a.outer) {
+      const float f = rsqrtf(row_sum<true>(sum, 64, part) * over + a.eps);
+      for (int c = threadIdx.x; c < a.n; c += blockDim.x) store1<DT>(a.out, row * a.n + c, hidden(c) * (f * a.outer[c]));
+    }
+  }
+}
+
+template <int DT, int RT>
+hipError_t launch(const NormArgs& a, bool wide, hipStream_t stream) {
+  const int64_t most = 1 << 22;  // workgroups: a grid holds fewer than 2^32 threads
+  const int pieces = (a.n + 7) / 8;
+  if (!wide || pieces > 4 * 1024) {
+    norm_any_kernel<DT, RT><<<(unsigned)std::min(a.rows, most), 256, 0, stream>>>(a);
+    return hipGetLastError();
+  }
+  if (pieces <= 64) {  // a row is at most one piece of each lane of a wave
+    int lanes = 8;
+    while (lanes < pieces) lanes *= 2;
+    const int64_t blocks = (a.rows * lanes + 255) / 256;
+    norm_kernel<DT, RT, 1, false><<<(unsigned)std::min(blocks, most), 256, 0, stream>>>(a, lanes);
+    return hipGetLastError();
+  }
+  const int64_t rows = std::min(a.rows, most / 4);
+  const auto threads = [&](int items) { return 64 * ((pieces + 64 * items - 1) / (64 * items)); };
+  if (pieces <= 1024) norm_kernel<DT, RT, 1, true><<<(unsigned)rows, threads(1), 0, stream>>>(a, 64);
+  else if (pieces <= 2048) norm_kernel<DT, RT, 2, true><<<(unsigned)rows, threads(2), 0, stream>>>(a, 64);
+  else norm_kernel<DT, RT, 4, true><<<(unsigned)rows, threads(4), 0, stream>>>(a, 64);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// wide: rows are a multiple of 8 long and 16-byte aligned, as are the weights
+hipError_t launch_norm(const NormArgs& a, int dtype, int residual_dtype, bool wide, hipStream_t stream) {
+  if (residual_dtype == kF32) {
+    switch (dtype) {
+      case kF32: return launch<kF32, kF32>(a, wide, stream);
+      case kF16: return launch<kF16, kF32>(a, wide, stream);
+      default: return launch<kBF16, kF32>(a, wide, stream);
+    }
+  }
+  return dtype == kF16 ? launch<kF16, kF16>(a, wide, stream) : launch<kBF16, kBF16>(a, wide, stream);
+}
+
+}  // namespace gguf_dec

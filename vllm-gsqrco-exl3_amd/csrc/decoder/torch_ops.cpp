@@ -90,6 +90,64 @@ Tensor kv8_attention(const Tensor& query, const Tensor& k, const Tensor& v, cons
   return out;
 }
 
+Tensor kv8_tree_attention(const Tensor& query, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs,
+                          const Tensor& tree_mask, const Tensor& block_table, const Tensor& seq_lens, const Tensor& cu_seqlens,
+                          int64_t max_new, int64_t max_len, double scale) {
+  const gguf_kv8_cache c = cache_of(k, v, ks, vs);
+  Tensor out = at::empty(query.sizes(), query.options());
+  const gguf_tensor q = desc(query), m = desc(tree_mask), t = desc(block_table), l = desc(seq_lens), cu = desc(cu_seqlens),
+                    o = desc(out);
+  const size_t bytes = gguf_kv8_attention_workspace_bytes(&c, &q, cu_seqlens.numel() - 1, max_new, max_len);
+  const Tensor ws = workspace(query, bytes);
+  check(gguf_kv8_tree_attention(&q, &c, &m, &t, &l, &cu, max_new, max_len, (float)scale, &o, data_of(ws), bytes, stream_of(query)));
+  return out;
+}
+
+// a tensor that may be missing, as the library takes it
+struct Maybe {
+  gguf_tensor t{};
+  const gguf_tensor* p = nullptr;
+  explicit Maybe(const std::optional<Tensor>& x) {
+    if (x) {
+      t = desc(*x);
+      p = &t;
+    }
+  }
+};
+
+Tensor kv8_rotary_append(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& k, const Tensor& v,
+                         const Tensor& ks, const Tensor& vs, const Tensor& cos_sin, const Tensor& positions,
+                         const Tensor& block_table, const Tensor& seq_lens, const Tensor& cu_seqlens, int64_t max_new,
+                         bool interleaved, const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight,
+                         double eps) {
+  const gguf_kv8_cache c = cache_of(k, v, ks, vs);
+  Tensor out = at::empty(query.sizes(), query.options());
+  const gguf_tensor a = desc(query), b = desc(key), x = desc(value), cs = desc(cos_sin), p = desc(positions), t = desc(block_table),
+                    l = desc(seq_lens), cu = desc(cu_seqlens), o = desc(out);
+  const Maybe qw(q_weight), kw(k_weight);
+  check(gguf_kv8_rotary_append(&c, &a, &b, &x, &cs, &p, &t, &l, &cu, max_new, interleaved, qw.p, kw.p, (float)eps, &o, stream_of(key)));
+  return out;
+}
+
+void kv8_keep(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& path,
+              const Tensor& block_table, const Tensor& seq_lens, const Tensor& cu_seqlens) {
+  const gguf_kv8_cache c = cache_of(k, v, ks, vs);
+  const gguf_tensor p = desc(path), t = desc(block_table), l = desc(seq_lens), cu = desc(cu_seqlens);
+  check(gguf_kv8_keep(&c, &p, &t, &l, &cu, stream_of(k)));
+}
+
+std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const std::optional<Tensor>& residual, const std::optional<Tensor>& gate,
+                                         int64_t act, const std::optional<Tensor>& inner_weight,
+                                         const std::optional<Tensor>& weight, double scale, double eps) {
+  Tensor hidden = at::empty(x.sizes(), residual ? x.options().dtype(residual->dtype()) : x.options());
+  Tensor out = weight ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  const gguf_tensor a = desc(x), h = desc(hidden), o = desc(out);
+  const Maybe r(residual), g(gate), wi(inner_weight), w(weight);
+  check(gguf_residual_norm(&a, r.p, g.p, act < 0 || act > 2 ? -1 : (int)act, wi.p, w.p, (float)scale, (float)eps, &h, w.p ? &o : nullptr,
+                           stream_of(x)));
+  return {out, hidden};
+}
+
 Tensor gated_delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                         const Tensor& state, const Tensor& slots, const Tensor& cu_seqlens, int64_t max_new,
                         const std::optional<Tensor>& out_slots, double scale, bool l2norm) {
@@ -131,6 +189,15 @@ TORCH_LIBRARY_FRAGMENT(_C_gguf, m) {
         "Tensor cu_seqlens, int tokens, int max_tokens, ScalarType dtype) -> (Tensor, Tensor)");
   m.def("kv8_attention(Tensor query, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, "
         "Tensor block_table, Tensor seq_lens, Tensor cu_seqlens, int max_new, int max_len, float scale) -> Tensor");
+  m.def("kv8_tree_attention(Tensor query, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor tree_mask, "
+        "Tensor block_table, Tensor seq_lens, Tensor cu_seqlens, int max_new, int max_len, float scale) -> Tensor");
+  m.def("kv8_rotary_append(Tensor query, Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+        "Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor cos_sin, Tensor positions, Tensor block_table, Tensor seq_lens, "
+        "Tensor cu_seqlens, int max_new, bool interleaved, Tensor? q_weight, Tensor? k_weight, float eps) -> Tensor");
+  m.def("kv8_keep(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor path, "
+        "Tensor block_table, Tensor seq_lens, Tensor cu_seqlens) -> ()");
+  m.def("residual_norm(Tensor x, Tensor? residual, Tensor? gate, int act, Tensor? inner_weight, Tensor? weight, float scale, "
+        "float eps) -> (Tensor, Tensor)");
   m.def("gated_delta_rule(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor(a!) state, Tensor slots, "
         "Tensor cu_seqlens, int max_new, Tensor? out_slots, float scale, bool l2norm) -> Tensor");
   m.def("token_logprobs(Tensor logits, Tensor token_ids, int top) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
@@ -141,6 +208,10 @@ TORCH_LIBRARY_FRAGMENT(_C_gguf, m) {
     m.impl("kv8_append", &kv8_append);                \
     m.impl("kv8_read", &kv8_read);                    \
     m.impl("kv8_attention", &kv8_attention);          \
+    m.impl("kv8_tree_attention", &kv8_tree_attention); \
+    m.impl("kv8_rotary_append", &kv8_rotary_append);  \
+    m.impl("kv8_keep", &kv8_keep);                    \
+    m.impl("residual_norm", &residual_norm);          \
     m.impl("gated_delta_rule", &gated_delta_rule);    \
     m.impl("token_logprobs", &token_logprobs);        \
   }

@@ -1,5 +1,6 @@
 """Operators of a decoder between its GGUF linear layers, and behind its head: the 8-bit paged KV
-cache and its attention, the gated delta rule (linear attention) and token log probabilities.
+cache, the position rotation on the way into it and its attention, also for trees of drafted tokens, block norms with
+their gates and residuals, the gated delta rule (linear attention) and token log probabilities.
 
 They are torch.ops._C_gguf.<name>, served by the HIP kernels of libgguf_decoder.so
 (include/gguf_decoder.h states what each does with every argument); the functions here are the same
@@ -13,7 +14,12 @@ first row.
     cache = Kv8Cache.empty(pages=512, heads=4, page=64, head_size=256)
     kv8_append(cache, k, v, block_table, seq_lens, cu_seqlens, max_new)
     y = kv8_attention(q, cache, block_table, seq_lens, cu_seqlens, max_new, max_len)
+    normed, residual = residual_norm(y, residual, weight)
+    q = kv8_rotary_append(cache, q, k, v, cos_sin, positions, block_table, seq_lens, cu_seqlens, max_new)
+    y = kv8_tree_attention(q, cache, tree_mask, block_table, seq_lens, cu_seqlens, max_new, max_len)
+    kv8_keep(cache, path, block_table, seq_lens, cu_seqlens)
     o = gated_delta_rule(q, k, v, g, beta, state, slots, cu_seqlens, max_new)
+    o = gated_norm(o, gate, weight)
     logprobs, ranks, entropy, top_logprobs, top_ids = token_logprobs(logits, token_ids, top=20)
 """
 
@@ -55,6 +61,24 @@ def register() -> None:
     @torch.library.register_fake("_C_gguf::kv8_attention")
     def _(query, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, max_new, max_len, scale):
         return query.new_empty(query.shape)
+
+    @torch.library.register_fake("_C_gguf::kv8_tree_attention")
+    def _(query, k_cache, v_cache, k_scale, v_scale, tree_mask, block_table, seq_lens, cu_seqlens, max_new, max_len, scale):
+        return query.new_empty(query.shape)
+
+    @torch.library.register_fake("_C_gguf::kv8_rotary_append")
+    def _(query, key, value, k_cache, v_cache, k_scale, v_scale, cos_sin, positions, block_table, seq_lens, cu_seqlens,
+          max_new, interleaved, q_weight, k_weight, eps):
+        return query.new_empty(query.shape)
+
+    @torch.library.register_fake("_C_gguf::kv8_keep")
+    def _(k_cache, v_cache, k_scale, v_scale, path, block_table, seq_lens, cu_seqlens):
+        return None
+
+    @torch.library.register_fake("_C_gguf::residual_norm")
+    def _(x, residual, gate, act, inner_weight, weight, scale, eps):
+        return (x.new_empty(x.shape if weight is not None else (0,)),
+                x.new_empty(x.shape, dtype=x.dtype if residual is None else residual.dtype))
 
     @torch.library.register_fake("_C_gguf::gated_delta_rule")
     def _(q, k, v, g, beta, state, slots, cu_seqlens, max_new, out_slots, scale, l2norm):
@@ -116,6 +140,71 @@ def kv8_attention(query, cache: Kv8Cache, block_table, seq_lens, cu_seqlens, max
     if scale is None:
         scale = query.shape[-1] ** -0.5
     return _ops.kv8_attention(query, *cache, block_table, seq_lens, cu_seqlens, max_new, max_len, scale)
+
+
+def kv8_rotary_append(cache: Kv8Cache, query, key, value, cos_sin, positions, block_table, seq_lens, cu_seqlens,
+                      max_new: int, interleaved: bool = False, q_weight=None, k_weight=None, eps: float = 1e-6):
+    """kv8_append of the keys turned by their positions, and the queries [tokens, q_heads, head_size] turned: returned in their
+    dtype. cos_sin fp32 [positions, r] holds the cosines and then the sines of r / 2 angles a position; dims i and i + r / 2
+    of a head turn together (interleaved: 2i and 2i + 1), those from r on stay. positions int64 [tokens]: a draft's is
+    its depth's. q_weight, k_weight fp32 [head_size]: the heads are normed by their root mean square first."""
+    return _ops.kv8_rotary_append(query, key, value, *cache, cos_sin, positions, block_table, seq_lens, cu_seqlens, max_new,
+                                  interleaved, q_weight, k_weight, eps)
+
+
+def tree_mask(parents):
+    """The int64 [tokens, words] mask of kv8_tree_attention, on the host, for a batch of trees: each a list of its rows' parents (row
+    numbers before the row's own, -1 for none). A row sees itself and its ancestors."""
+    words = max(1, -(-max((len(t) for t in parents), default=0) // 64))
+    out = []
+    for tree in parents:
+        rows = []
+        for i, p in enumerate(tree):
+            if not -1 <= p < i:
+                raise ValueError(f"row {i} cannot have parent {p}")
+            rows.append((rows[p] if p >= 0 else 0) | 1 << i)
+        for r in rows:
+            w = [r >> 64 * j & (1 << 64) - 1 for j in range(words)]
+            out.append([x - (1 << 64) if x >> 63 else x for x in w])
+    return torch.tensor(out, dtype=torch.int64).view(-1, words)
+
+
+def kv8_tree_attention(query, cache: Kv8Cache, tree_mask, block_table, seq_lens, cu_seqlens, max_new: int, max_len: int,
+                       scale: float | None = None):
+    """Attention of a tree of drafts, query [tokens, q_heads, head_size] (fp16 or bf16): a row sees all of its sequence's
+    positions before the sequence's own rows, and of these row j where bit j % 64 of tree_mask[row, j // 64] is set. The
+    cache holds the drafts' keys and values as the sequence's last positions, in the rows' order."""
+    if scale is None:
+        scale = query.shape[-1] ** -0.5
+    return _ops.kv8_tree_attention(query, *cache, tree_mask, block_table, seq_lens, cu_seqlens, max_new, max_len, scale)
+
+
+def kv8_keep(cache: Kv8Cache, path, block_table, seq_lens, cu_seqlens) -> None:
+    """Move row path[s, j] (int32 [seqs, m]) of each sequence's last rows, its drafts, to their j-th place in the cache: a
+    path grows strictly and ends at its first entry that does not (or is out of range, as -1). The arguments are those the drafts were
+    appended with; afterwards the sequence is as long as its older tokens and the path."""
+    _ops.kv8_keep(*cache, path, block_table, seq_lens, cu_seqlens)
+
+
+_ACTS = {"none": 0, "sigmoid": 1, "silu": 2}
+
+
+def residual_norm(x, residual=None, weight=None, *, inner_weight=None, gate=None, act: str = "none", scale: float = 1.0,
+                  eps: float = 1e-6):
+    """Norms before and after a block with its gate and residual, over the last dimension of x [rows, n] or [rows, heads, n]:
+        u = x, normed by inner_weight, times act(gate);  h = residual + scale * u;  out = h, normed by weight
+    with RMS norms (weights fp32 [n]); every part may be missing. act: "none", "sigmoid" or "silu" of a gate like x. Returns (out,
+    h): out in x's dtype (None without weight), h in residual's (x's dtype or fp32)."""
+    if act not in _ACTS:
+        raise RuntimeError(f"residual_norm: act={act!r} is not one of {', '.join(_ACTS)}")
+    out, hidden = _ops.residual_norm(x, residual, gate, _ACTS[act], inner_weight, weight, scale, eps)
+    return (None if weight is None else out), hidden
+
+
+def gated_norm(x, gate, weight, *, act: str = "silu", eps: float = 1e-6):
+    """x [rows, n] or [rows, heads, n] normed over its last dimension by weight (fp32 [n]), times act(gate): the norm behind
+    linear attention's heads."""
+    return residual_norm(x, inner_weight=weight, gate=gate, act=act, eps=eps)[1]
 
 
 def gated_delta_rule(q, k, v, g, beta, state, slots, cu_seqlens, max_new: int, out_slots=None,
