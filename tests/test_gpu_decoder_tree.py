@@ -75,36 +75,77 @@ def _run(dec, ends, news, hq, heads, d, page, dtype, seed, words=1, mask=None, m
     return q, cache, table, mask, y
 
 
+# max_len hints: the contexts' own, and one that asks for the forms for many rows wherever more than 32 rows share a KV head
+HINTS = [None, 1 << 24]
+
+
+@pytest.mark.parametrize("hint", HINTS)
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
-@pytest.mark.parametrize("hq,heads,d,page", [(6, 1, 256, 16), (8, 2, 128, 32), (4, 4, 64, 144), (5, 1, 192, 64)])
+@pytest.mark.parametrize("hq,heads,d,page", [(6, 1, 256, 16), (8, 2, 128, 32), (4, 4, 64, 144), (5, 1, 192, 64), (16, 2, 256, 144), (3, 1, 192, 16)])
 @pytest.mark.parametrize("news", [(1, 1, 1, 1), (1, 3, 0, 7), (2, 9, 8, 5), (5, 40, 2, 17), (64, 63, 1, 30)], ids=str)
-def test_tree(dec, dtype, hq, heads, d, page, news):
+def test_tree(dec, dtype, hq, heads, d, page, news, hint):
     """Any bits, a root alone to a whole mask word, behind contexts of none to several splits."""
-    _run(dec, (news[0], 65, 200, 777), news, hq, heads, d, page, dtype, 21)
+    _run(dec, (news[0], 65, 200, 777), news, hq, heads, d, page, dtype, 21, max_len=hint)
 
 
 @pytest.mark.parametrize("hq,heads,d,page,dtype", [(6, 1, 256, 16, BF16), (1, 1, 128, 16, F16), (8, 1, 64, 32, BF16)])
 @pytest.mark.parametrize("words", [1, 2, 3])
-def test_masks_of_several_words(dec, hq, heads, d, page, dtype, words):
+@pytest.mark.parametrize("hint", HINTS)
+def test_masks_of_several_words(dec, hq, heads, d, page, dtype, words, hint):
     """Trees that end inside, at and beyond their masks: rows past them are not seen. Tiles that straddle words."""
-    _run(dec, (130, 400, 71 + 64 * words, 191), (130, 100, 64 * words, 191), hq, heads, d, page, dtype, 22, words)
+    _run(dec, (130, 400, 71 + 64 * words, 191), (130, 100, 64 * words, 191), hq, heads, d, page, dtype, 22, words, max_len=hint)
 
 
 @pytest.mark.parametrize("base", [0, 1, 15, 16, 31, 33, 63, 64, 65, 100])
 @pytest.mark.parametrize("hq,news", [(2, 11), (2, 37)])
-def test_where_the_drafts_begin(dec, base, hq, news):
+@pytest.mark.parametrize("d,hint", [(128, None), (128, 1 << 24), (256, 1 << 24)])
+def test_where_the_drafts_begin(dec, base, hq, news, d, hint):
     """The first draft at every place of a chunk, tile and page; ancestors as a tree has them."""
     parents = [[-1] + [(i * 7) % i for i in range(1, news)]]
-    _run(dec, (base + news,), (news,), 2 * hq, 2, 128, 16, BF16, 23, mask=dec.tree_mask(parents))
+    _run(dec, (base + news,), (news,), 2 * hq, 2, d, 16, BF16, 23, mask=dec.tree_mask(parents), max_len=hint)
+
+
+@pytest.mark.parametrize("d,hq", [(256, 6), (192, 3), (128, 6)])
+def test_long_contexts(dec, d, hq):
+    """Contexts that shares of the work begin and end in, beyond the chunks that are looked up at a time (2048 tokens, and 4096), beside
+    short ones and empty sequences; one sequence alone; many short ones in a share."""
+    _run(dec, (9000, 40, 5, 2600, 0, 4177), (30, 33, 5, 1, 0, 64), hq, 1, d, 64, BF16, 31, max_len=1 << 24)
+    _run(dec, (20011,), (24,), hq, 1, d, 16, BF16, 32, max_len=1 << 24)
+    ends = tuple(3 + 17 * i % 150 for i in range(300))
+    _run(dec, ends, tuple(min(e, 1 + i % 4) for i, e in enumerate(ends)), 3 * hq, 3, d, 32, F16, 33, max_new=20, max_len=1 << 24)
+
+
+@pytest.mark.parametrize("scale", [-0.5, 0.0, 3e4, 1e-30])
+@pytest.mark.parametrize("hint", HINTS)
+def test_scales_and_maxima_that_move(dec, scale, hint):
+    """Any scale; scores that rise and fall by hundreds from tile to tile, in one half of a tile and the other."""
+    g = torch.Generator().manual_seed(34)
+    ends, news, page = (700,), (40,), 16
+    cache = _random_cache(dec, 46, 1, page, 256, g)
+    cache.k_scale.copy_(torch.exp2(12 * torch.rand(46, 1, generator=g) - 8))
+    table = _table(ends, page, 46, g)
+    q = (torch.randn(40, 4, 256, generator=g) * (1 if abs(scale) > 1 else 0.3)).to(BF16).cuda()
+    mask = _random_mask(40, 1, g).cuda()
+    y = dec.kv8_tree_attention(q, cache, mask, table, _i32(*ends), _cu(news), 40, hint or 700, scale)
+    # the form for many rows takes queries as integers of the row's largest / 16256: half a step of these times keys of some hundreds
+    # is up to 5 here, so the reference has them too (the form for few rows has these queries exactly)
+    amax = q.double().abs().amax(-1, keepdim=True)
+    ref, most = _tree_ref(torch.round(q.double() * 16256 / amax) * amax / 16256 if hint else q, cache, table, mask, ends, news, scale)
+    assert torch.isfinite(y).all()
+    if abs(scale) < 1:
+        _close(y, ref, most)
+    else:  # one token takes all, but where two are within the queries' last bits
+        assert ((y.double() - ref).abs() <= 2.0 ** -6 * most).float().mean() > 0.98
 
 
 @pytest.mark.parametrize("news", [(3, 4, 2, 5), (3, 90, 2, 80)], ids=str)
-def test_rows_that_see_nothing(dec, news):
+@pytest.mark.parametrize("d,hint", [(128, None), (128, 1 << 24), (256, 1 << 24)])
+def test_rows_that_see_nothing(dec, news, d, hint):
     """No bits and no context, a length below the rows, a negative one: zeros. And no bits over a context."""
     mask = torch.zeros(sum(news), 1, dtype=I64)
     mask[news[0] + 3] = 0b1010
     ends = (news[0], 3, -3, news[3] + 50)
-    y = _run(dec, ends, news, 6, 2, 128, 16, BF16, 24, mask=mask)[-1]
+    y = _run(dec, ends, news, 6, 2, d, 16, BF16, 24, mask=mask, max_len=hint)[-1]
     assert (y[:news[0]] == 0).all() and (y[news[0]:news[0] + 3] == 0).all() and (y[-news[3] - news[2]:-news[3]] == 0).all()
     assert (y[-news[3]:] != 0).any(-1).all()
 
@@ -124,24 +165,26 @@ def test_hints_only_size_the_launch(dec, news, max_new, max_len):
 
 
 @pytest.mark.parametrize("news", [5, 70])
-def test_drafts_past_the_table(dec, news):
+@pytest.mark.parametrize("d,hint", [(64, None), (64, 1 << 24), (192, 1 << 24)])
+def test_drafts_past_the_table(dec, news, d, hint):
     """A table that holds some of the drafts, none of them, or not the whole context: what it lacks is not seen."""
     for pages in (1, 3, 6, 7):
-        _run(dec, (100 + news,), (news,), 4, 2, 64, 16, F16, 27, change=lambda c, t: t[:, :pages].contiguous())
+        _run(dec, (100 + news,), (news,), 4, 2, d, 16, F16, 27, max_len=hint, change=lambda c, t: t[:, :pages].contiguous())
 
 
 @pytest.mark.parametrize("news", [4, 50])
-def test_what_a_row_does_not_see_does_not_touch_it(dec, news):
+@pytest.mark.parametrize("d,hint", [(128, None), (128, 1 << 24), (256, 1 << 24)])
+def test_what_a_row_does_not_see_does_not_touch_it(dec, news, d, hint):
     """A draft page that is not finite, far larger, or out of range: NaN for the rows that see one of its rows, and others keep
     their bits."""
     ends, page = (32 + news,), 16
     mask = torch.zeros(news, 1, dtype=I64)
     mask[1::2] = 1  # odd rows see the first draft, in page 2
-    q, cache, table, mask, y = _run(dec, ends, (news,), 4, 2, 128, page, BF16, 28, mask=mask)
+    q, cache, table, mask, y = _run(dec, ends, (news,), 4, 2, d, page, BF16, 28, mask=mask, max_len=hint)
 
     def again(t):
         poison_allocator()
-        return dec.kv8_tree_attention(q, cache, mask, t, _i32(*ends), _cu((news,)), news, ends[0])
+        return dec.kv8_tree_attention(q, cache, mask, t, _i32(*ends), _cu((news,)), news, hint or ends[0])
 
     at = int(table[0, 2])
     was = cache.v_scale[at].clone()
@@ -158,31 +201,48 @@ def test_what_a_row_does_not_see_does_not_touch_it(dec, news):
         assert torch.equal(x[::2], y[::2]) and torch.isnan(x[1::2]).all()
 
 
-def test_rows_behind_the_last_sequence_and_strides(dec):
+@pytest.mark.parametrize("d,hint", [(128, 70), (128, 1 << 24), (256, 1 << 24)])
+def test_rows_behind_the_last_sequence_and_strides(dec, d, hint):
     """A padded batch: rows past the last offset cost nothing and touch nobody; queries and masks are views of wider tensors."""
     g = torch.Generator().manual_seed(29)
-    cache = _random_cache(dec, 12, 2, 16, 128, g)
+    cache = _random_cache(dec, 12, 2, 16, d, g)
     ends, news = (70, 50), (6, 20)
     table = _table(ends, 16, 12, g)
-    wide = (torch.randn(40, 9, 128, generator=g) * 0.3).to(BF16).cuda()
+    wide = (torch.randn(40, 9, d, generator=g) * 0.3).to(BF16).cuda()
     q, m = wide[:, 2:8], torch.stack([_random_mask(40, 1, g)[:, 0]] * 3, 1).cuda()[:, 1:2]
-    y = dec.kv8_tree_attention(q, cache, m, table, _i32(*ends), _cu(news), 20, 70)
-    ref, most = _tree_ref(q[:26], cache, table, m, ends, news, 128 ** -0.5)
+    y = dec.kv8_tree_attention(q, cache, m, table, _i32(*ends), _cu(news), 20, hint)
+    ref, most = _tree_ref(q[:26], cache, table, m, ends, news, d ** -0.5)
     _close(y[:26], ref, most)
-    x = dec.kv8_tree_attention(q[:26], cache, m[:26], table, _i32(*ends), _cu(news), 20, 70)
+    x = dec.kv8_tree_attention(q[:26], cache, m[:26], table, _i32(*ends), _cu(news), 20, hint)
     assert torch.equal(x, y[:26])
 
 
 @pytest.mark.parametrize("news", [3, 40])
-def test_tree_repeats_and_replays(dec, news):
-    q, cache, table, mask, y = _run(dec, (900, 2000), (news, news), 12, 2, 256, 64, BF16, 30)
+@pytest.mark.parametrize("d,hint", [(256, 2000), (128, 1 << 24), (256, 1 << 24)])
+def test_tree_repeats_and_replays(dec, news, d, hint):
+    """The same bits every time, in a graph too; and a graph replayed with other lengths, offsets, masks and pages, which are cut into
+    other shares."""
+    q, cache, table, mask, y = _run(dec, (900, 2000), (news, news), 12, 2, d, 64, BF16, 30, max_len=hint)
+    lens, cu = _i32(900, 2000), _cu((news, news))
 
     def call():
-        return dec.kv8_tree_attention(q, cache, mask, table, _i900, _cu2, news, 2000)
+        return dec.kv8_tree_attention(q, cache, mask, table, lens, cu, news, hint)
 
-    _i900, _cu2 = _i32(900, 2000), _cu((news, news))
     assert torch.equal(call(), y)
     graph_replays_equal(call, y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for ends, at in (((70, 1900), (0, 1, 1 + news)), ((2000, 2000), (0, news, 2 * news)), ((0, 3), (0, 0, news))):
+        lens.copy_(_i32(*ends))
+        cu.copy_(_i32(*at))
+        table.copy_(table.flip(1))
+        mask.copy_(mask.flip(0))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out[:at[-1]].clone()
+        assert torch.equal(got.nan_to_num(7), call()[:at[-1]].nan_to_num(7))
+        # (a table turned round has pages that are not there: NaN, in the same places)
 
 
 # ------------------------------------------------------------------------------------------ keep

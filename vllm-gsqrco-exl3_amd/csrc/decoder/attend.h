@@ -106,6 +106,7 @@ struct AttnArgs {
   const int64_t* mask;  // of a tree: [tokens][words], or null
   int64_t mask_stride;
   int words;
+  int dtype;            // of q and out, where a kernel is not made for one
 };
 
 // What a row of a tree sees of the 16-token chunk at position `at` (a multiple of 16), a bit a token: of positions before `base` all,
@@ -131,5 +132,9 @@ __device__ __forceinline__ uint32_t tree_bits(const int64_t* mask, int at, int64
 // attention_rows.hip: many rows
 constexpr int kRowsTile = 128;  // rows of a workgroup
 hipError_t launch_attend_rows(const AttnArgs& a, int dtype, int64_t row_tiles, hipStream_t stream);
+
+// attention_tree.hip: many rows of a tree; `rows`: of a KV head, a hint
+size_t tree_workspace(int d, int64_t rows, int64_t tokens, int hq, int64_t seqs, int heads, int64_t max_len);
+hipError_t launch_attend_tree(AttnArgs a, int64_t rows, int64_t max_len, void* ws, hipStream_t stream);
 
 }  // namespace gguf_dec

@@ -346,15 +346,26 @@ hipError_t launch_attend(const AttnArgs& a, dim3 grid, hipStream_t stream) {
 // Calls in us, one / two tiles, at up to 16384 tokens: head size 64, eight sequences of 64 rows 67.5 / 55.7, of 24 rows
 // 39.2 / 35.6; head size 128, eight of 32 rows 55.3 / 62.6, one of 32 rows 19.4 / 27.8; head size 192, one of 24 rows
 // 15.0 / 18.0, eight of 60 rows 37.9 / 40.4, of 36 rows 45.8 / 38.1.
+// A tree takes its form for many rows (of heads up to 128 attention_rows.hip, beyond attention_tree.hip) by its work, since that form's
+// fixed costs are larger: from 33 rows of a (sequence, KV head) on, and 2^23 of rows times tokens over all of them (3 * 2^23 of heads up
+// to 128). Calls in us, few / many: head size 256, four KV heads, 96 rows of one sequence of 16000 tokens 45.8 / 57.6, of four of 4000
+// 60.3 / 53.0, of eight 75.0 / 53.0; 48 rows of four of 4000 36.7 / 42.9, of eight of 16000 132 / 100, of 32 of 2000 87.8 / 67.6; 24 rows of
+// eight of 16000 92.3 / 98.0; 384 rows of one of 2000 37.5 / 53.5. Head size 192, one KV head, 96 rows of eight of 16000 61.3 / 48.9,
+// 48 rows of these 37.0 / 41.9. Head size 128, eight KV heads, 256 rows of one of 2000 21.6 / 26.5; 64 rows of eight of 4000 38.6 / 42.3,
+// of 32 of 2000 78.3 / 67.5; 32 rows of eight of 16000 86.3 / 102, 48 rows 117 / 105.
+static bool tree_many(int d, int64_t rows, int64_t groups, int64_t max_len) {
+  return rows > 32 && (double)rows * (double)groups * (double)max_len >= (d > 128 ? 1 : 3) * 8388608.0;
+}
+
 struct AttnPlan {
   bool many;
   int nt, span, splits;
   int64_t row_tiles;
 };
 
-static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, int64_t most) {
+static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, int64_t most, bool tree) {
   AttnPlan p;
-  p.many = rows > 64;
+  p.many = tree ? tree_many(d, rows, groups, max_len) : rows > 64;
   p.nt = rows > 16 && d < 128 ? 2 : 1;
   const int64_t tile = p.many ? kRowsTile : 16 * p.nt;
   p.row_tiles = (rows + tile - 1) / tile;
@@ -374,8 +385,10 @@ static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, 
 static int64_t most_splits(int64_t rows) { return rows < (1 << 24) ? 512 : 1; }
 
 size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t seqs, int64_t max_new,
-                               int64_t max_len) {
-  const AttnPlan p = attn_plan(d, max_new * (hq / heads), seqs * heads, max_len, most_splits(tokens * hq));
+                               int64_t max_len, bool tree) {
+  if (tree && d > 128 && tree_many(d, max_new * (hq / heads), seqs * heads, max_len))
+    return tree_workspace(d, max_new * (hq / heads), tokens, hq, seqs, heads, max_len);
+  const AttnPlan p = attn_plan(d, max_new * (hq / heads), seqs * heads, max_len, most_splits(tokens * hq), tree);
   return p.splits == 1 ? 0 : (size_t)p.splits * tokens * hq * (d + 2) * sizeof(float);
 }
 
@@ -383,12 +396,16 @@ hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t 
                                 const int32_t* lens, const Ragged& rows, int64_t max_new, int64_t max_len, float scale,
                                 const int64_t* mask, int64_t mask_stride, int words, void* out, void* ws, size_t ws_bytes,
                                 hipStream_t stream) {
+  if (mask && c.d > 128 && tree_many(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len)) {
+    const AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, 0, 0, out, nullptr, nullptr, mask, mask_stride, words, dtype};
+    return launch_attend_tree(a, max_new * (hq / c.heads), max_len, ws, stream);
+  }
   const int64_t all = (int64_t)rows.tokens * hq;
   const int64_t fit = (int64_t)(ws_bytes / sizeof(float)) / (all * (c.d + 2));
   const AttnPlan p = attn_plan(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len,
-                               fit < 2 ? 1 : std::min(fit, most_splits(all)));
+                               fit < 2 ? 1 : std::min(fit, most_splits(all)), mask != nullptr);
   const AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, p.span, p.splits, out, (float*)ws,
-                   (float*)ws + (size_t)p.splits * all * c.d, mask, mask_stride, words};
+                   (float*)ws + (size_t)p.splits * all * c.d, mask, mask_stride, words, dtype};
   const dim3 grid((unsigned)(rows.seqs * c.heads * p.splits), (unsigned)(p.row_tiles < 65535 ? p.row_tiles : 65535));
   hipError_t e = hipSuccess;
   if (p.many) e = launch_attend_rows(a, dtype, p.row_tiles, stream);

@@ -361,9 +361,9 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
 
 hipError_t launch_attend_rows(const AttnArgs& a, int dtype, int64_t row_tiles, hipStream_t stream) {
   const dim3 grid((unsigned)(a.rows.seqs * a.c.heads * a.splits), (unsigned)(row_tiles < 65535 ? row_tiles : 65535));
-#define GGUF_DEC_ROWS_D(DT, D)                                                                    \
-  if (a.mask) attend_rows_kernel<DT, D, true><<<grid, 64 * kRowWaves, 0, stream>>>(a);            \
-  else attend_rows_kernel<DT, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a);
+#define GGUF_DEC_ROWS_D(DT, D)                                                                                  \
+  if (D > 128 || !a.mask) attend_rows_kernel<DT, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a);             \
+  else attend_rows_kernel<DT, D, D <= 128><<<grid, 64 * kRowWaves, 0, stream>>>(a);  // (larger heads: attention_tree.hip)
 #define GGUF_DEC_ROWS(DT)                            \
   switch (a.c.d) {                                   \
     case 64: GGUF_DEC_ROWS_D(DT, 64) break;          \

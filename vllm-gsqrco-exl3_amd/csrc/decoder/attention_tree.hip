@@ -1,0 +1,625 @@
+// Attention for trees of drafts over the 8-bit paged cache, for many rows a KV head: some ten to some hundred rows that
+// all see a long context, and of each other what their masks say (attend.h: tree_bits).
+//
+// Products and operands are those of attention_rows.hip: S^T = K Q^T in int8 with Q as two planes, O^T += V^T P^T in fp16,
+// 32 x 32 MFMAs, a lane keeps its query rows. What differs:
+//   - Two waves share 32 NR rows, so that either holds half of the output's dims and two waves fit a SIMD: one's softmax runs
+//     beside the other's products. Of a tile of 64 tokens each takes 32 scores a row; weights go to the partner through LDS.
+//   - The row maximum lags behind: weights are taken against the maximum before the tile, and only where a score passes it by
+//     2^8 (the workgroup sees a flag behind the tile's barrier) do the partners agree on a new one and take them again. So a
+//     tile costs one barrier.
+//   - The tiles of all (sequence, head, row tile)s in a line are cut into equal shares, one a workgroup, whatever the lengths
+//     are. A workgroup whose share begins or ends inside a group leaves its sums to join_tree_kernel; a group that lies in one share is
+//     written at once.
+#include <algorithm>
+#include <type_traits>
+
+#include "attend.h"
+
+namespace gguf_dec {
+
+namespace {
+
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+constexpr int kToks = 64;                // tokens of a tile
+constexpr int kVRow = 2 * kToks + 16;    // bytes of a dim's row of V in LDS; 16 more than its values, for the banks
+constexpr int kAhead = 32;               // tiles whose chunks are looked up at a time
+constexpr int kPlaces = 4 * 2 * kAhead;  // places of chunks that are held: those of tile t at 4 (t % (2 kAhead))
+constexpr int kLeastTiles = 4;           // of a workgroup's share
+
+// v, made again where it is needed: what comes of a thread's number (its places in LDS and memory) would otherwise be kept over the
+// tiles, in registers that the products need
+__device__ __forceinline__ int again(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// Where a chunk's K and V lie, and its scales.
+struct Place {
+  int64_t k, v;
+  float ks, vs;
+};
+
+// A group of tiles that lies in several shares, from share `first` on (it begins there) to `last`.
+struct Cut {
+  int seq, first, last, own;  // own: it is the first of share `first`
+  int64_t group;              // among its sequence's
+};
+
+// Queries as the products take them, and the line of all tiles, cut: what prep_tree_kernel leaves.
+struct Prep {
+  int8_t* q;       // [tokens * hq][2][d]: integers of 15 bits, in two planes
+  float* qs;       // [tokens * hq]: what they are multiplied by, with the call's scale
+  int64_t* line;   // [seqs + 1]: tiles before a sequence's
+  int* begins;     // [shares]: the sequence in which a share begins
+  int* cuts;       // how many groups are cut
+  Cut* cut;        // [shares]
+};
+
+template <int D, int NG>
+struct Lay {
+  static constexpr int kThreads = 128 * NG, kRows = 32 * NG;
+  static constexpr int kKRow = D + 16;                           // bytes of a token's row of K
+  static constexpr int kK = 0;                                   // [2][64][kKRow]
+  static constexpr int kV = kK + 2 * kToks * kKRow;              // [2][D][kVRow]
+  static constexpr int kP = kV + 2 * D * kVRow;                  // [waves][2][64] x 16 bytes
+  static constexpr int kPlace = kP + 2 * NG * 2048;              // Place [kPlaces]
+  static constexpr int kStat = kPlace + 24 * kPlaces;            // float [waves][32]
+  static constexpr int kBytes = kStat + 2 * NG * 128;
+};
+
+// tiles of a sequence's rows: 0 without rows, at least one with them (it writes the zeros of rows that see nothing)
+struct Seq {
+  int r0, n, tiles, row_tiles;
+  int64_t len;
+};
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s, int rows) {
+  Seq q;
+  int r1;
+  rows_of(a.rows, s, q.r0, r1);
+  q.n = r1 - q.r0;
+  q.len = a.lens[s];
+  const int64_t room = (int64_t)a.c.max_pages * a.c.page;
+  const int64_t see = min(q.len, room);
+  q.tiles = q.n == 0 ? 0 : (int)max((see + kToks - 1) / kToks, (int64_t)1);
+  q.row_tiles = (int)(((int64_t)q.n * a.group + rows - 1) / rows);
+  return q;
+}
+
+// How the line of all tiles is cut: share w of `shares` is [w total / shares, (w + 1) total / shares).
+struct Line {
+  int64_t total, shares;
+  __device__ Line(const AttnArgs& a, const Prep& p, int64_t most) : total(p.line[a.rows.seqs]) {
+    shares = min(most, max((total + kLeastTiles - 1) / kLeastTiles, (int64_t)1));
+  }
+  __device__ int64_t begin(int64_t w) const { return w * total / shares; }
+};
+
+// Queries as integers (attention_rows.hip), a wave a row; and, by the last workgroup, the tiles before each sequence's, where the
+// shares begin, and which groups they cut.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int rows, int64_t most) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (blockIdx.x + 1 == gridDim.x) {
+    __shared__ int64_t part[4];
+    int64_t total = 0;
+    for (int s0 = 0; s0 < a.rows.seqs; s0 += 256) {
+      const int s = s0 + tid;
+      int64_t cost = 0;
+      if (s < a.rows.seqs) {
+        const Seq q = seq_of(a, s, rows);
+        cost = (int64_t)a.c.heads * q.row_tiles * q.tiles;
+      }
+      int64_t x = cost;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int64_t y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+      }
+      __syncthreads();
+      if (lane == 63) part[wave] = x;
+      __syncthreads();
+      int64_t before = total;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += part[w];
+        total += part[w];
+      }
+      if (s < a.rows.seqs) p.line[s] = before + x - cost;
+    }
+    if (tid == 0) p.line[a.rows.seqs] = total, *p.cuts = 0;
+    __syncthreads();
+    const Line line(a, p, most);
+    for (int64_t w = tid; w < line.shares && total > 0; w += 256) {
+      const int64_t at = line.begin(w);
+      int s = 0;  // the last sequence with line[s] <= at: one that has tiles
+      for (int lo = 0, hi = a.rows.seqs - 1; lo <= hi;) {
+        const int mid = lo + (hi - lo) / 2;
+        if (p.line[mid] <= at) s = mid, lo = mid + 1;
+        else hi = mid - 1;
+      }
+      p.begins[w] = s;
+      if (w == 0) continue;
+      const int tiles = seq_of(a, s, rows).tiles;
+      const int64_t group = (at - p.line[s]) / tiles, lo = p.line[s] + group * tiles, hi = lo + tiles;
+      if (at == lo || line.begin(w - 1) > lo) continue;  // it begins with the group, or an earlier share's begin lies inside it
+      int64_t last = w;
+      while (line.begin(last + 1) < hi) ++last;
+      p.cut[atomicAdd(p.cuts, 1)] = Cut{s, (int)w - 1, (int)last, line.begin(w - 1) == lo, group};
+    }
+    return;
+  }
+  const int64_t all = (int64_t)a.rows.tokens * a.hq;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < all; r += (int64_t)(gridDim.x - 1) * 4) {
+    const int64_t tok = r / a.hq;
+    const int at = min(4 * lane, D - 4);  // four values a lane
+    const uint2 w = *(const uint2*)((const uint16_t*)a.q + tok * a.qt + (r - tok * a.hq) * a.qh + at);
+    const uint32_t bits[4] = {w.x & 0xFFFF, w.x >> 16, w.y & 0xFFFF, w.y >> 16};
+    float v[4];
+    uint32_t big = 0;  // NaN and inf on top: then the row's scores are NaN
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = DT == kF16 ? gguf::half_bits_to_float(bits[e]) : __uint_as_float(bits[e] << 16);
+      big = max(big, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off, 64));
+    const float amax = __uint_as_float(big);
+    // a row of magnitudes below 2^-100 has scores of 0
+    const float inv = amax >= 0x1p-100f && amax < __builtin_inff() ? (a.scale < 0.0f ? -16256.0f : 16256.0f) / amax : 0.0f;
+    uint32_t hi = 0, lo = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int x = (int)rintf(v[e] * inv), top = (x + 64) >> 7;
+      hi |= (uint32_t)(top & 0xFF) << 8 * e;
+      lo |= (uint32_t)((x - 128 * top) & 0xFF) << 8 * e;
+    }
+    if (4 * lane < D) {
+      *(uint32_t*)(p.q + r * 2 * D + at) = hi;
+      *(uint32_t*)(p.q + r * 2 * D + D + at) = lo;
+    }
+    // not negative: the scale's sign is the integers'
+    if (lane == 0) p.qs[r] = amax < __builtin_inff() ? fabsf(a.scale) * (amax * (1.0f / 16256.0f)) : __builtin_nanf("");
+  }
+}
+
+// A workgroup's share. Sums of a group that it does not have alone: slot 2 w of one in which share w begins, 2 w + 1 of a later one.
+//
+// A tile is two steps of a wave: products (the tile before's O^T += V^T P^T, then S^T = K Q^T), and weights (softmax, and the tiles' way
+// to LDS), with a barrier behind each. The first four waves, one a SIMD, and the others (LAG: there are others) are a step apart,
+// so that on a SIMD one wave's products run beside the other's weights. The first bring V: tile t's in the step of its weights, over
+// tile t - 2's, which the others have read a step before. The others bring K: tile t + 2's in the step of tile t's weights, over tile t's.
+template <int D, int NG>
+__global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(NG > 2 ? 2 : 1, NG > 2 ? 2 : 1))) attend_tree_kernel(AttnArgs a, Prep prep, int64_t most) {
+  using L = Lay<D, NG>;
+  constexpr bool LAG = NG > 2;
+  constexpr int KS = D / 32, DD = D / 64;       // steps of the first product; 32-dim tiles of the wave's half of the dims
+  constexpr int PIECES = 4 * D;                 // 16-byte pieces of a tile's K, and of its V
+  constexpr int FIRST = LAG ? 256 : L::kThreads / 2;  // threads that bring V, and as many K
+  constexpr int NP = PIECES / FIRST;
+  static_assert(PIECES % FIRST == 0 && L::kThreads == 2 * FIRST, "whole turns");
+  extern __shared__ __align__(16) char lds[];
+  Place* places = (Place*)(lds + L::kPlace);
+  float* stat = (float*)(lds + L::kStat);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
+  const int rg = wave >> 1, half = wave & 1;
+  const bool brings_v = wave < FIRST / 64, late = LAG && !brings_v;
+  const int room = (int)min((int64_t)a.c.max_pages * a.c.page, (int64_t)INT32_MAX);
+
+  const Line line(a, prep, most);
+  if ((int64_t)blockIdx.x >= line.shares || line.total == 0) return;
+  const int64_t begin = line.begin(blockIdx.x), end = line.begin((int64_t)blockIdx.x + 1);
+  int seq = prep.begins[blockIdx.x];
+
+  for (int64_t pos = begin; pos < end;) {
+    while (pos >= prep.line[seq + 1]) ++seq;  // (sequences without rows cost nothing)
+    const Seq q = seq_of(a, seq, L::kRows);
+    const int64_t in_seq = pos - prep.line[seq], group = in_seq / q.tiles;
+    const int tb = (int)(in_seq - group * q.tiles), te = (int)min((int64_t)q.tiles, tb + (end - pos));
+    const int head = (int)(group / q.row_tiles), rt = (int)(group - (int64_t)head * q.row_tiles);
+    const bool whole = tb == 0 && te == q.tiles, first = pos == begin;
+    pos += te - tb;
+
+    const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
+    const int see = (int)min(q.len, (int64_t)room) - 1;
+    // position of the sequence's first row; below -2^30 no position is one of its rows (their masks hold 2^30 bits at most)
+    const int base = (int)max(q.len - q.n, -((int64_t)1 << 30));
+    const int drafts = (int)min((int64_t)q.n, (int64_t)64 * a.words);
+    const int open = min(base, room);  // positions that every row sees
+    const int tlast = te - 1;
+    const auto places_of = [&](int t) __attribute__((always_inline)) { return places + 4 * (t & (2 * kAhead - 1)); };
+    const auto find_places = [&](int from, int tiles, int threads) __attribute__((always_inline)) {
+      for (int i = again(tid); i < 4 * tiles; i += threads) {
+        const Chunk c = chunk_of(a.c, table, a.c.page / 16, head, (int64_t)4 * from + i, see);
+        places_of(from + (i >> 2))[i & 3] =
+            Place{((int64_t)c.ph * a.c.page + c.off) * D, (int64_t)c.ph * a.c.page * D + c.off, c.ks, c.vs};
+      }
+    };
+
+    // A thread's pieces, j * FIRST + me, of V (chunk p & 3 of dim p >> 2) or of K (row p / (D / 16)), on their way.
+    uintx4 raw[NP];
+    const auto load_v = [&](int t) __attribute__((always_inline)) {
+      const int me = again(tid);
+      const int8_t* from = a.c.v + places_of(t)[me & 3].v;
+#pragma unroll
+      for (int j = 0; j < NP; ++j) raw[j] = *(const uintx4*)(from + (uint32_t)((j * (FIRST / 4) + (me >> 2)) * a.c.page));
+    };
+    const auto load_k = [&](int t) __attribute__((always_inline)) {
+      const int me = again(tid - FIRST);
+      const Place* at = places_of(t);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const uint32_t p = j * FIRST + me, row = p / (D / 16);
+        raw[j] = *(const uintx4*)(a.c.k + at[row >> 4].k + (row & 15) * D + 16 * (p % (D / 16)));
+      }
+    };
+    const auto put_v = [&](int t) __attribute__((always_inline)) {
+      const int me = again(tid);
+      char* to = lds + L::kV + (t & 1) * D * kVRow + (me >> 2) * kVRow + 32 * (me & 3);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        *(half8*)(to + j * (FIRST / 4) * kVRow) = codes8(raw[j][0], raw[j][1]);
+        *(half8*)(to + j * (FIRST / 4) * kVRow + 16) = codes8(raw[j][2], raw[j][3]);
+      }
+    };
+    const auto put_k = [&](int t) __attribute__((always_inline)) {
+      const int me = again(tid - FIRST);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const uint32_t p = j * FIRST + me;
+        *(uintx4*)(lds + L::kK + (t & 1) * kToks * L::kKRow + p / (D / 16) * L::kKRow + 16 * (p % (D / 16))) = raw[j];
+      }
+    };
+    __syncthreads();  // what the last piece left in LDS has been read
+    find_places(tb, 2 * kAhead, L::kThreads);
+    __syncthreads();
+
+    const int64_t row0 = (int64_t)rt * L::kRows;
+    const int tok0 = (int)(row0 / a.group), head0 = (int)(row0 - (int64_t)tok0 * a.group);
+    const int left = (int)min((int64_t)q.n * a.group - row0, (int64_t)L::kRows);
+    // the lane's row: its token (of the first row if it is none), and its place among all rows
+    struct Row {
+      bool ok;
+      int tok;
+      int64_t at;
+    };
+    const auto row_of = [&]() __attribute__((always_inline)) {
+      const int r = 32 * rg + (again(lane) & 31);
+      Row x;
+      x.ok = r < left;
+      const uint32_t y = head0 + (x.ok ? r : 0), z = y / (uint32_t)a.group;
+      x.tok = q.r0 + tok0 + (int)z;
+      x.at = (int64_t)x.tok * a.hq + head * a.group + (int)(y - z * a.group);
+      return x;
+    };
+
+    intx4 qhi[KS], qlo[KS];
+    const Row row = row_of();
+    const float qs = prep.qs[row.at];
+    const int8_t* qp = prep.q + row.at * 2 * D + 16 * h;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      qhi[i] = *(const intx4*)(qp + 32 * i);
+      qlo[i] = *(const intx4*)(qp + D + 32 * i);
+    }
+    if (brings_v) {
+      load_v(tb);
+    } else {
+      load_k(tb);
+      put_k(tb);
+      load_k(min(tb + 1, tlast));
+      put_k(tb + 1);
+      load_k(min(tb + 2, tlast));
+    }
+    floatx16 o[DD];
+    float m = kNoScore, l = 0.0f, ref = 0.0f, inv_ref = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DD; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) asm volatile("" : "+v"(qhi[i]), "+v"(qlo[i]));  // here: not waited for with the tiles' loads
+
+    half8* const weights = (half8*)(lds + L::kP);  // [waves][2][64]: for the waves' partners
+    const int krow = 32 * half + 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);  // token of K's row n
+    const char* const k0 = lds + L::kK + krow * L::kKRow + 16 * h;
+    const char* const v0 = lds + L::kV + (half * (D / 2) + n) * kVRow + 16 * h;
+    half8 p[2], pp[2];  // the weights of a tile, the wave's own and its partner's
+    // The products of a step, two MFMAs at a time: O^T of tile t - 1 (the wave's half of the dims; its own tokens' weights, then its
+    // partner's), then S^T of the wave's 32 tokens of tile t. Operands are read two pairs ahead.
+    // BACK: the first, FRONT: the second.
+    intx16 hi, lo;
+    const auto products = [&](int t, auto back, auto front) __attribute__((always_inline)) {
+      constexpr bool BACK = decltype(back)::value, FRONT = decltype(front)::value;
+      constexpr int P2 = BACK ? 2 * DD : 0, PAIRS = P2 + (FRONT ? KS : 0);
+      const char* const vt = v0 + ((t - 1) & 1) * D * kVRow;
+      const char* const kt = k0 + (t & 1) * kToks * L::kKRow;
+      half8 v[BACK ? 4 * DD : 1];
+      intx4 k[KS];
+      const auto fetch = [&](int r) __attribute__((always_inline)) {  // the operands of pair r
+        if (r < P2) {
+#pragma unroll
+          for (int f = 2 * r; f < 2 * r + 2; ++f)
+            v[f] = *(const half8*)(vt + 64 * (half ^ (f / DD >> 1)) + 32 * (f / DD & 1) + 32 * (f % DD) * kVRow);
+        } else if (r < PAIRS) {
+          k[r - P2] = *(const intx4*)(kt + 32 * (r - P2));
+        }
+      };
+      if constexpr (BACK) {
+        const int me = again(lane);
+        const float other = stat[32 * (wave ^ 1) + (me & 31)];
+        const half8* const theirs = weights + 64 * 2 * (wave ^ 1) + me;
+        pp[0] = theirs[0];
+        pp[1] = theirs[64];
+        fetch(0);
+        fetch(1);
+        if (__any(other != m)) {  // one of the partners has raised its maximum: both go on with the larger
+          const float nm = fmaxf(m, other), al = __builtin_amdgcn_exp2f(m - nm), be = __builtin_amdgcn_exp2f(other - nm);
+          m = nm;
+          l *= al;
+#pragma unroll
+          for (int i = 0; i < DD; ++i) o[i] *= al;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {  // by powers of two: the maxima are whole numbers
+            p[c] *= (_Float16)al;
+            pp[c] *= (_Float16)be;
+          }
+        }
+      } else {
+        fetch(0);
+        fetch(1);
+      }
+      if constexpr (FRONT) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) hi[e] = lo[e] = 0;
+      }
+#pragma unroll
+      for (int r = 0; r < PAIRS; ++r) {
+        fetch(r + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        if (r < P2) {
+#pragma unroll
+          for (int f = 2 * r; f < 2 * r + 2; ++f)
+            o[f % DD] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[f], f / DD < 2 ? p[f / DD] : pp[f / DD - 2], o[f % DD], 0, 0, 0);
+        } else {
+          hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[r - P2], qhi[r - P2], hi, 0, 0, 0);
+          lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[r - P2], qlo[r - P2], lo, 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+
+    __syncthreads();
+    if (late) __syncthreads();
+    for (int t = tb; t < te; ++t) {
+      if (t > tb) products(t, std::true_type(), std::true_type());
+      else products(t, std::false_type(), std::true_type());
+      const Place* at = places_of(t);
+      float own[2] = {at[2 * half].vs, at[2 * half + 1].vs};
+      const float f[2] = {qs * at[2 * half].ks, qs * at[2 * half + 1].ks};
+      // the largest V scale of the chunks that the row sees (a NaN counts for nothing)
+      float highest = fmaxf(fmaxf(at[0].vs, at[1].vs), fmaxf(at[2].vs, at[3].vs));
+      __syncthreads();
+
+      if (brings_v) {
+        put_v(t);
+        load_v(min(t + 1, tlast));
+        if (((t - tb) & (kAhead - 1)) == 0 && t != tb && t + kAhead <= tlast) find_places(t + kAhead, kAhead, FIRST);
+      } else {
+        put_k(t);  // tile t + 2's, in tile t's place
+        load_k(min(t + 3, tlast));
+      }
+      floatx16 s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float x = (float)((hi[e] << 7) + lo[e]) * f[e >> 3];
+        asm("" : "+v"(x));  // rounded here: of scores beyond 2^24 an fma's rest would pass any weight
+        s[e] = x;
+      }
+      if (kToks * t + kToks > open) {
+        highest = 0.0f;
+        const int64_t* mask = a.mask + row_of().tok * a.mask_stride;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c)
+          if (tree_bits(mask, kToks * t + 16 * c, base, drafts, room)) highest = fmaxf(highest, at[c].vs);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t bits = tree_bits(mask, kToks * t + 32 * half + 16 * c, base, drafts, room);
+          if (bits == 0) own[c] = 0.0f;  // also where the page's scale is not finite
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (!(bits >> (8 * h + e) & 1)) s[8 * c + e] = -__builtin_inff();
+        }
+      }
+      float mx = kNoScore;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
+      mx = half_max(mx);
+      // the maximum may lag: weights stay below 2^8, and the sums are scaled again only where it does not do, or
+      // where the largest V scale grew
+      const bool raise = mx > m + 8.0f;
+      if (__any(raise || highest > ref)) {
+        const float nref = fmaxf(ref, highest), nm = raise ? ceilf(mx) : m, al = __builtin_amdgcn_exp2f(m - nm);
+        const float by = nref > ref ? al * (ref / nref) : al;
+        l *= al;
+#pragma unroll
+        for (int i = 0; i < DD; ++i) o[i] *= by;
+        m = nm;
+        ref = nref;
+        inv_ref = nref > 0.0f ? kWeight / nref : 0.0f;
+      }
+      const int me = again(lane);
+      half8* const ours = weights + 64 * 2 * wave + me;
+      stat[32 * wave + (me & 31)] = m;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float vr = own[c] * inv_ref;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float w = __builtin_amdgcn_exp2f(s[8 * c + e] - m);
+          l += w;
+          p[c][e] = (_Float16)(w * vr);
+        }
+        ours[64 * c] = p[c];
+      }
+      __syncthreads();
+    }
+    products(te, std::true_type(), std::false_type());
+    __syncthreads();
+    if (LAG && !late) __syncthreads();
+
+    // the rows' sums over both halves of the tokens
+    l += __shfl_xor(l, 32, 64);
+    if (h == 0) stat[32 * wave + n] = l;
+    __syncthreads();
+    const Row mine = row_of();
+    if (!mine.ok) continue;
+    const float all = l + stat[32 * (wave ^ 1) + n], by = ref / kWeight;
+    if (whole) {
+      const float inv = all == 0.0f ? 0.0f : by / all;
+#pragma unroll
+      for (int i = 0; i < DD; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int64_t to = mine.at * D + half * (D / 2) + 32 * i + 2 * e + 4 * h;
+          const float y[4] = {o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv};
+          if (a.dtype == kF16) store4<kF16>(a.out, to, y);
+          else store4<kBF16>(a.out, to, y);
+        }
+    } else {
+      const int64_t r = (2 * (int64_t)blockIdx.x + !first) * L::kRows + 32 * rg + n;
+#pragma unroll
+      for (int i = 0; i < DD; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *(floatx4*)(a.part + r * D + half * (D / 2) + 32 * i + 2 * e + 4 * h) =
+              floatx4{o[i][e] * by, o[i][e + 1] * by, o[i][e + 2] * by, o[i][e + 3] * by};
+      if (h == 0 && half == 0) *(float2*)(a.stat + r * 2) = make_float2(m, all);
+    }
+  }
+}
+
+// Joins the rows of the groups that are cut, one at a time: its waves take the parts in turn, D / 64 dims a lane, and join through LDS.
+template <int D>
+__global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, int rows) {
+  constexpr int E = D / 64;
+  __shared__ float sums[4][64][E];
+  __shared__ float ls[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int cuts = *prep.cuts;
+  for (int i = blockIdx.y; i < cuts; i += gridDim.y) {
+    const Cut cut = prep.cut[i];
+    const Seq q = seq_of(a, cut.seq, rows);
+    const int head = (int)(cut.group / q.row_tiles), rt = (int)(cut.group - (int64_t)head * q.row_tiles);
+    const int64_t nrows = min((int64_t)rows, (int64_t)q.n * a.group - (int64_t)rt * rows);
+    for (int64_t r = blockIdx.x; r < nrows; r += gridDim.x) {
+      const int64_t row = (int64_t)rt * rows + r;
+      const auto slot = [&](int w) { return (2 * (int64_t)w + (w == cut.first && !cut.own)) * rows + r; };
+      float mx = kNoScore;
+      for (int w = cut.first + lane; w <= cut.last; w += 64) mx = fmaxf(mx, a.stat[slot(w) * 2]);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+      float sum = 0.0f, acc[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+      for (int w = cut.first + wave; w <= cut.last; w += 4) {
+        const float2 ml = *(const float2*)(a.stat + slot(w) * 2);
+        const float f = __builtin_amdgcn_exp2f(ml.x - mx);
+        sum += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += a.part[slot(w) * D + E * lane + e] * f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) sums[wave][lane][e] = acc[e];
+      if (lane == 0) ls[wave] = sum;
+      __syncthreads();
+      if (wave == 0) {
+        sum = ls[0] + ls[1] + ls[2] + ls[3];
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t to = ((int64_t)(q.r0 + row / a.group) * a.hq + head * a.group + row % a.group) * D + E * lane;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float y = (sums[0][lane][e] + sums[1][lane][e] + sums[2][lane][e] + sums[3][lane][e]) * inv;
+          if (a.dtype == kF16) store1<kF16>(a.out, to + e, y);
+          else store1<kBF16>(a.out, to + e, y);
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+struct Plan {
+  int groups;        // row groups of 32 a workgroup
+  int64_t shares;
+  int64_t heads;     // (sequence, head, row tile)s, at most a workgroup's share each
+  size_t q, qs, line, begins, cuts, cut, part, stat, bytes;  // parts of the workspace, and its size
+};
+
+size_t padded(size_t n) { return (n + 255) / 256 * 256; }
+
+// `rows`: of a KV head. As few workgroups a KV head as there can be, of as few rows; shares of a workgroup a CU.
+Plan plan_of(int d, int64_t rows, int64_t tokens, int hq, int64_t seqs, int heads, int64_t max_len) {
+  Plan p;
+  const int64_t units = std::max<int64_t>(1, (rows + 31) / 32), row_tiles = (units + 3) / 4;
+  p.groups = (units + row_tiles - 1) / row_tiles <= 2 ? 2 : 4;
+  const int64_t tiles = std::max<int64_t>(1, (max_len + kToks - 1) / kToks);
+  // (each factor is capped where the product is beyond every number of workgroups)
+  const int64_t work = std::min<int64_t>(seqs * heads, 1 << 20) * std::min<int64_t>(row_tiles, 1 << 20) * std::min<int64_t>(tiles, 1 << 20);
+  p.shares = std::max<int64_t>(1, std::min<int64_t>(gguf::device_cus(), (work + kLeastTiles - 1) / kLeastTiles));
+  p.q = 0;
+  p.qs = p.q + padded((size_t)tokens * hq * 2 * d);
+  p.line = p.qs + padded((size_t)tokens * hq * sizeof(float));
+  p.heads = std::min<int64_t>(std::min<int64_t>(seqs * heads, 1 << 20) * std::min<int64_t>(row_tiles, 1 << 20), p.shares);
+  p.begins = p.line + padded((size_t)(seqs + 1) * sizeof(int64_t));
+  p.cuts = p.begins + padded((size_t)p.shares * sizeof(int));
+  p.cut = p.cuts + 256;
+  p.part = p.cut + padded((size_t)p.shares * sizeof(Cut));
+  const size_t slots = p.shares == 1 ? 0 : 2 * (size_t)p.shares * 32 * p.groups;
+  p.stat = p.part + slots * d * sizeof(float);
+  p.bytes = p.stat + slots * 2 * sizeof(float);
+  return p;
+}
+
+template <int D, int NG>
+hipError_t launch(const AttnArgs& a, const Prep& prep, const Plan& p, hipStream_t stream) {
+  using L = Lay<D, NG>;
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  struct Tag {};
+  gguf::once_per_device<Tag>(dev, [&] {
+    (void)hipFuncSetAttribute((const void*)attend_tree_kernel<D, NG>, hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  });
+  const int64_t rows = ((int64_t)a.rows.tokens * a.hq + 3) / 4;
+  const unsigned blocks = (unsigned)std::min<int64_t>(rows, 1 << 20) + 1;
+  if (a.dtype == kF16) prep_tree_kernel<kF16, D><<<blocks, 256, 0, stream>>>(a, prep, L::kRows, p.shares);
+  else prep_tree_kernel<kBF16, D><<<blocks, 256, 0, stream>>>(a, prep, L::kRows, p.shares);
+  attend_tree_kernel<D, NG><<<(unsigned)p.shares, L::kThreads, L::kBytes, stream>>>(a, prep, p.shares);
+  if (p.shares > 1)  // a row a workgroup, or four where there are many
+    join_tree_kernel<D><<<dim3(p.heads <= 32 ? L::kRows : L::kRows / 4, (unsigned)p.heads), 256, 0, stream>>>(a, prep, L::kRows);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t tree_workspace(int d, int64_t rows, int64_t tokens, int hq, int64_t seqs, int heads, int64_t max_len) {
+  return plan_of(d, rows, tokens, hq, seqs, heads, max_len).bytes;
+}
+
+hipError_t launch_attend_tree(AttnArgs a, int64_t rows, int64_t max_len, void* ws, hipStream_t stream) {
+  const Plan p = plan_of(a.c.d, rows, a.rows.tokens, a.hq, a.rows.seqs, a.c.heads, max_len);
+  char* w = (char*)ws;
+  const Prep prep{(int8_t*)w, (float*)(w + p.qs), (int64_t*)(w + p.line), (int*)(w + p.begins), (int*)(w + p.cuts), (Cut*)(w + p.cut)};
+  a.part = (float*)(w + p.part);
+  a.stat = (float*)(w + p.stat);
+  if (a.c.d == 192) return p.groups == 2 ? launch<192, 2>(a, prep, p, stream) : launch<192, 4>(a, prep, p, stream);
+  return p.groups == 2 ? launch<256, 2>(a, prep, p, stream) : launch<256, 4>(a, prep, p, stream);
+}
+
+}  // namespace gguf_dec

@@ -18,7 +18,7 @@ hipError_t launch_kv8_append(const Kv8& c, int dtype, const void* key, int64_t k
 hipError_t launch_kv8_read(const Kv8& c, int dtype, const int32_t* starts, const Ragged& rows, int64_t max_tokens,
                            void* kout, void* vout, hipStream_t stream);
 size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t seqs, int64_t max_new,
-                               int64_t max_len);
+                               int64_t max_len, bool tree);
 hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t qt, int64_t qh, int hq,
                                 const int32_t* lens, const Ragged& rows, int64_t max_new, int64_t max_len, float scale,
                                 const int64_t* mask, int64_t mask_stride, int words, void* out, void* ws, size_t ws_bytes,
@@ -246,14 +246,24 @@ int gguf_kv8_read(const gguf_kv8_cache* cache, const gguf_tensor* block_table, c
   return e == hipSuccess ? GGUF_DEC_OK : hip_fail(e, op);
 }
 
-size_t gguf_kv8_attention_workspace_bytes(const gguf_kv8_cache* cache, const gguf_tensor* query, int64_t seqs,
-                                          int64_t max_new, int64_t max_len) {
+static size_t attention_workspace(const gguf_kv8_cache* cache, const gguf_tensor* query, int64_t seqs, int64_t max_new,
+                                  int64_t max_len, bool tree) {
   if (!cache || cache->k.ndim != 4 || !query || query->ndim != 3 || seqs < 1 || cache->k.size[1] < 1 || query->size[0] < 1 ||
       query->size[1] % cache->k.size[1] || query->size[1] < 1)
     return 0;
   const DeviceScope scope(query->device < 0 ? 0 : query->device);
   return gguf_dec::kv8_attention_workspace((int)cache->k.size[3], (int)cache->k.size[1], (int)query->size[1],
-                                           query->size[0], seqs, bounded(max_new, query->size[0]), bounded(max_len, INT_MAX));
+                                           query->size[0], seqs, bounded(max_new, query->size[0]), bounded(max_len, INT_MAX), tree);
+}
+
+size_t gguf_kv8_attention_workspace_bytes(const gguf_kv8_cache* cache, const gguf_tensor* query, int64_t seqs,
+                                          int64_t max_new, int64_t max_len) {
+  return attention_workspace(cache, query, seqs, max_new, max_len, false);
+}
+
+size_t gguf_kv8_tree_attention_workspace_bytes(const gguf_kv8_cache* cache, const gguf_tensor* query, int64_t seqs,
+                                               int64_t max_new, int64_t max_len) {
+  return attention_workspace(cache, query, seqs, max_new, max_len, true);
 }
 
 // kv8_attention, or with a mask kv8_tree_attention
@@ -288,6 +298,8 @@ static int attention(const char* op, const gguf_tensor* query, const gguf_kv8_ca
   if (!present(query, out, seq_lens, cu_seqlens, mask)) return fail("%s: a tensor has no data", op);
   if (query->device < 0) return fail("%s: tensors must be CUDA tensors", op);
   if (query->size[0] == 0) return GGUF_DEC_OK;
+  const size_t need = tree ? gguf_kv8_tree_attention_workspace_bytes(cache, query, rows.seqs, max_new, max_len) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes needed, got %zu", op, need, workspace_bytes);
   const DeviceScope scope(query->device);
   if (scope.err != hipSuccess) return hip_fail(scope.err, op);
   const hipError_t e = gguf_dec::launch_kv8_attention(

@@ -97,7 +97,7 @@ Tensor kv8_tree_attention(const Tensor& query, const Tensor& k, const Tensor& v,
   Tensor out = at::empty(query.sizes(), query.options());
   const gguf_tensor q = desc(query), m = desc(tree_mask), t = desc(block_table), l = desc(seq_lens), cu = desc(cu_seqlens),
                     o = desc(out);
-  const size_t bytes = gguf_kv8_attention_workspace_bytes(&c, &q, cu_seqlens.numel() - 1, max_new, max_len);
+  const size_t bytes = gguf_kv8_tree_attention_workspace_bytes(&c, &q, cu_seqlens.numel() - 1, max_new, max_len);
   const Tensor ws = workspace(query, bytes);
   check(gguf_kv8_tree_attention(&q, &c, &m, &t, &l, &cu, max_new, max_len, (float)scale, &o, data_of(ws), bytes, stream_of(query)));
   return out;
