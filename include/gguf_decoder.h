@@ -121,7 +121,7 @@ GGUF_DEC_API int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cac
 
 /* kv8_append with the position rotation of keys, and of the queries beside them, on the way, after the norms of their heads
  * where these have weights. query [tokens, q_heads, d] (any number of heads), key, value: one float dtype, unit inner stride, rows
- * 16-byte aligned; the sequences times the cache's heads below 2^22. For a head's row x of query (w = q_weight) or key
+ * 16-byte aligned; the sequences times the cache's heads below 2^21. For a head's row x of query (w = q_weight) or key
  * (w = k_weight; fp32 [d], 16-byte aligned; NULL: no norm)
  *   x = x / sqrt(mean(x^2) + eps) * w
  *   x_i, x_j = x_i c - x_j s, x_j c + x_i s   for the pairs (i, j = i + r / 2), i < r / 2; interleaved: (2 i', j = 2 i' + 1)

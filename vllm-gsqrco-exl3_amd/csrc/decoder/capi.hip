@@ -346,7 +346,7 @@ int gguf_kv8_rotary_append(const gguf_kv8_cache* cache, const gguf_tensor* query
   if (query->size[0] != t || query->size[1] < 1 || query->size[2] != c.d) return fail("%s: query must be [tokens, heads, %d] with key's tokens", op, c.d);
   if (t > 0 && (!rows_ok(query) || !rows_ok(key) || !rows_ok(value)))
     return fail("%s: query, key and value need unit inner stride and 16-byte aligned rows", op);
-  if ((int64_t)rows.seqs * c.heads >= (1 << 22)) return fail("%s: sequences times heads must be below 2^22", op);
+  if ((int64_t)rows.seqs * c.heads >= (1 << 21)) return fail("%s: sequences times heads must be below 2^21", op);
   if (!shaped(cos_sin, 2) || cos_sin->dtype != GGUF_DEC_F32 || cos_sin->size[0] < 1 || cos_sin->size[1] < 16 || cos_sin->size[1] % 16 ||
       cos_sin->size[1] > c.d || cos_sin->stride[1] != 1 || !aligned(cos_sin, 16) || stride_of(cos_sin, 0) % 4)
     return fail("%s: cos_sin must be fp32 [positions, 16 .. %d in steps of 16] with unit inner stride and 16-byte aligned rows", op, c.d);

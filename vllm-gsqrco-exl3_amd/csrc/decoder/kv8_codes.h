@@ -41,41 +41,4 @@ __device__ __forceinline__ Rescale rescale_of(float was, float amax) {
   return grown(was, fresh < kLeastScale ? 0.0f : fresh);
 }
 
-// Writes tokens [lo, hi) of a (page, head) of V, whose tokens are innermost: a thread turns 16 tokens x 8 dims in its registers.
-// `base`: where the page's token 0 would lie in x. 16-token groups without new tokens are touched only where the scale grew.
-template <int DT, int D, int THREADS>
-__device__ __forceinline__ void put_v(int8_t* codes, int page, int lo, int hi, int older, const void* x, int64_t base,
-                                      int64_t stride, const Rescale& s) {
-  constexpr int per = D / 8;
-  const bool shrink = older > 0 && s.shrink;
-  const int g0 = shrink ? 0 : lo / 16, g1 = (hi + 15) / 16;
-  for (int i = threadIdx.x; i < (g1 - g0) * per; i += THREADS) {
-    const int t0 = 16 * (g0 + i / per), at = 8 * (i % per);
-    uint32_t w[8][4];
-    const bool whole = lo <= t0 && t0 + 16 <= hi;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      uint4 o = make_uint4(0, 0, 0, 0);
-      if (!whole) o = *(const uint4*)(codes + (int64_t)(at + e) * page + t0);
-      w[e][0] = o.x; w[e][1] = o.y; w[e][2] = o.z; w[e][3] = o.w;
-    }
-#pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      float v[8];
-      const bool is_new = t0 + t >= lo && t0 + t < hi;
-      const bool is_old = shrink && t0 + t < older;
-      if (is_new) load8<DT>(x, base + (t0 + t) * stride + at, v);
-      if (is_new || is_old) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = is_new ? v[e] * s.inv : (float)(int8_t)(w[e][t >> 2] >> 8 * (t & 3)) * s.ratio;
-          w[e][t >> 2] = (w[e][t >> 2] & ~(0xFFu << 8 * (t & 3))) | (uint32_t)(code_of(y) & 0xFF) << 8 * (t & 3);
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) *(uint4*)(codes + (int64_t)(at + e) * page + t0) = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
-  }
-}
-
 }  // namespace gguf_dec
