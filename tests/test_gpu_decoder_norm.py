@@ -112,6 +112,19 @@ def test_many_rows(dec):
             assert torch.equal(c, a[lo:hi]) and torch.equal(d, b[lo:hi])
 
 
+@pytest.mark.parametrize("n", [4096, 4104, 5120, 8192, 12296, 16384, 20000])
+def test_many_long_rows(dec, n):
+    """Rows of many a workgroup's pieces, alone and among more than a thousand: the same bits."""
+    g = torch.Generator().manual_seed(8)
+    x, r, w = torch.randn(1100, n, generator=g).bfloat16().cuda(), torch.randn(1100, n, generator=g).bfloat16().cuda(), torch.randn(n, generator=g).cuda()
+    kw = dict(inner_weight=w, act="silu", scale=0.7)
+    a, b = dec.residual_norm(x, r, w, gate=r, **kw)
+    for lo, hi in ((0, 1), (511, 540), (1099, 1100)):
+        c, d = dec.residual_norm(x[lo:hi], r[lo:hi], w, gate=r[lo:hi], **kw)
+        assert torch.equal(c, a[lo:hi]) and torch.equal(d, b[lo:hi])
+    _run(dec, (1030, n), BF16, F32, 9, True, True, "sigmoid", True, 0.5)
+
+
 def test_broadcast_gate_and_residual(dec):
     """Strides of 0: one gate, one residual row for all rows."""
     g = torch.Generator().manual_seed(7)

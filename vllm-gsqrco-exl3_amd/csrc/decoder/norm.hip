@@ -3,6 +3,10 @@
 //   out = h rsqrt(mean h^2 + eps) w_out
 // (every part but x optional). A row's values stay in registers from the loads to the stores, so each input is read and
 // each output written once; sums of squares are fp32, and only h and out are rounded.
+//
+// Bound by memory for many rows, by the launch and a row's chain of loads, sums and stores for few: 8192 rows of 5120 values, all
+// bf16, both norms: 76 us (4.4 TB/s; a copy reaches 4.9 to 5.2); 8192 x 48 heads of 128 with a gate: 56 us (5.3
+// TB/s); 4 rows of 5120: 3.4 us in a graph, 6.7 by itself, where the host takes the time.
 #include <algorithm>
 
 #include "norm.h"
@@ -18,21 +22,37 @@ __device__ __forceinline__ float act_of(float g, int act) {
   return act == kActSilu ? g * s : act == kActSigmoid ? s : g;
 }
 
-// sum over the row's lanes (a power of two up to 64, aligned) or over the workgroup
-template <bool WG>
-__device__ __forceinline__ float row_sum(float v, int lanes, float* part) {
+// Sum over the row's lanes (a power of two up to 64, aligned) or over the workgroup, of whose waves each holds ITEMS parts. Each
+// 64 pieces are summed for themselves, then these sums, in one order, so that a row has the same bits in every form that takes it.
+template <bool WG, int ITEMS>
+__device__ __forceinline__ float row_sum(const float (&sums)[ITEMS], int lanes, float* part) {
   if constexpr (!WG) {
+    float v = sums[0];
     for (int off = 1; off < lanes; off <<= 1) v += __shfl_xor(v, off, 64);
     return v;
   } else {
+    const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // the sums of ITEMS values together: after the first steps lane l holds a part of the (l % ITEMS)-th alone
+    float s[ITEMS];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
-    const int waves = blockDim.x >> 6;
+    for (int i = 0; i < ITEMS; ++i) s[i] = sums[i];
+#pragma unroll
+    for (int left = ITEMS; left > 1; left /= 2) {
+      const int off = ITEMS / left;
+      const bool odd = lane & off;
+#pragma unroll
+      for (int i = 0; i < left / 2; ++i) {
+        const float mine = odd ? s[2 * i + 1] : s[2 * i], other = odd ? s[2 * i] : s[2 * i + 1];
+        s[i] = mine + __shfl_xor(other, off, 64);
+      }
+    }
+#pragma unroll
+    for (int off = ITEMS; off < 64; off <<= 1) s[0] += __shfl_xor(s[0], off, 64);
     __syncthreads();  // the last sum's parts have been read
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    if (lane < ITEMS) part[lane * waves + wave] = s[0];
     __syncthreads();
-    v = part[0];
-    for (int w = 1; w < waves; ++w) v += part[w];
+    float v = part[0];
+    for (int g = 1; g < ITEMS * waves; ++g) v += part[g];
     return v;
   }
 }
@@ -42,23 +62,26 @@ __device__ __forceinline__ void at_row(const RowStride& s, int64_t token, int he
 }
 
 // A row is ITEMS pieces of 8 values a lane: `lanes` lanes of a wave take it, or (WG) the whole workgroup. Weights are held over
-// the rows that a lane takes.
+// the rows that a lane takes; of four pieces a lane, weights and gates are read as they are needed, for the registers.
 template <int DT, int RT, int ITEMS, bool WG>
 __global__ void __launch_bounds__(WG ? 1024 : 256) norm_kernel(NormArgs a, int lanes) {
-  __shared__ float part[16];
+  __shared__ float part[64];
   const int per = WG ? 1 : blockDim.x / lanes;  // rows a workgroup at a time
   const int lane = WG ? threadIdx.x : threadIdx.x % lanes, width = WG ? blockDim.x : lanes;
   const int mine = WG ? 0 : threadIdx.x / lanes;
   const float over = 1.0f / (float)a.n;
-  float wi[ITEMS][8], wo[ITEMS][8];
+  constexpr bool HELD = ITEMS < 4;
+  float wi[HELD ? ITEMS : 1][8], wo[HELD ? ITEMS : 1][8];
+  const auto weight = [&](const float* from, int c, float (&w)[8]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int c = 8 * (lane + i * width);
+    for (int e = 0; e < 8; ++e) w[e] = 0.0f;
+    if (from && c < a.n) load8<kF32>(from, c, w);
+  };
+  if constexpr (HELD) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) wi[i][e] = wo[i][e] = 0.0f;
-    if (c < a.n) {
-      if (a.inner) load8<kF32>(a.inner, c, wi[i]);
-      if (a.outer) load8<kF32>(a.outer, c, wo[i]);
+    for (int i = 0; i < ITEMS; ++i) {
+      weight(a.inner, 8 * (lane + i * width), wi[i]);
+      weight(a.outer, 8 * (lane + i * width), wo[i]);
     }
   }
   for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < a.rows; r0 += (int64_t)gridDim.x * per) {
@@ -70,39 +93,47 @@ __global__ void __launch_bounds__(WG ? 1024 : 256) norm_kernel(NormArgs a, int l
     at_row(a.xs, token, head, xa);
     at_row(a.rs, token, head, ra);
     at_row(a.gs, token, head, ga);
-    float u[ITEMS][8], g[ITEMS][8], h[ITEMS][8];
+    float u[ITEMS][8], g[HELD ? ITEMS : 1][8], h[ITEMS][8];
+    const auto gate = [&](int c, float (&to)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] = 1.0f;
+      if (a.gate && c < a.n) load8<DT>(a.gate, ga + c, to);
+    };
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int c = 8 * (lane + i * width);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[i][e] = h[i][e] = 0.0f, g[i][e] = 1.0f;
+      for (int e = 0; e < 8; ++e) u[i][e] = h[i][e] = 0.0f;
+      if constexpr (HELD) gate(c, g[i]);
       if (c < a.n) {
         load8<DT>(a.x, xa + c, u[i]);
-        if (a.gate) load8<DT>(a.gate, ga + c, g[i]);
         if (a.residual) load8<RT>(a.residual, ra + c, h[i]);
       }
     }
     if (a.inner) {
-      float sum = 0.0f;
+      float sum[ITEMS] = {};
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += u[i][e] * u[i][e];
+        for (int e = 0; e < 8; ++e) sum[i] += u[i][e] * u[i][e];
       const float by = rsqrtf(row_sum<WG>(sum, lanes, part) * over + a.eps);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
+      for (int i = 0; i < ITEMS; ++i) {
+        if constexpr (!HELD) weight(a.inner, 8 * (lane + i * width), wi[0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[i][e] *= by * wi[i][e];
+        for (int e = 0; e < 8; ++e) u[i][e] *= by * wi[HELD ? i : 0][e];
+      }
     }
-    float sum = 0.0f;
+    float sum[ITEMS] = {};
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int c = 8 * (lane + i * width);
+      if constexpr (!HELD) gate(c, g[0]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (a.gate) u[i][e] *= act_of(g[i][e], a.act);
+        if (a.gate) u[i][e] *= act_of(g[HELD ? i : 0][e], a.act);
         h[i][e] += a.scale * u[i][e];
-        if (c < a.n) sum += h[i][e] * h[i][e];
+        if (c < a.n) sum[i] += h[i][e] * h[i][e];
       }
       if (c < a.n && ok) store8<RT>(a.hidden, row * a.n + c, h[i]);
     }
@@ -111,8 +142,9 @@ __global__ void __launch_bounds__(WG ? 1024 : 256) norm_kernel(NormArgs a, int l
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         const int c = 8 * (lane + i * width);
+        if constexpr (!HELD) weight(a.outer, c, wo[0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[i][e] *= by * wo[i][e];
+        for (int e = 0; e < 8; ++e) h[i][e] *= by * wo[HELD ? i : 0][e];
         if (c < a.n && ok) store8<DT>(a.out, row * a.n + c, h[i]);
       }
     }
@@ -131,11 +163,11 @@ __global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
     at_row(a.xs, token, head, xa);
     at_row(a.rs, token, head, ra);
     at_row(a.gs, token, head, ga);
-    float by = 1.0f, sum = 0.0f;
+    float by = 1.0f, sum[1] = {};
     if (a.inner) {
       for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
         const float v = load1<DT>(a.x, xa + c);
-        sum += v * v;
+        sum[0] += v * v;
       }
       by = rsqrtf(row_sum<true>(sum, 64, part) * over + a.eps);
     }
@@ -145,10 +177,10 @@ __global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
       if (a.gate) u *= act_of(load1<DT>(a.gate, ga + c), a.act);
       return (a.residual ? load1<RT>(a.residual, ra + c) : 0.0f) + a.scale * u;
     };
-    sum = 0.0f;
+    sum[0] = 0.0f;
     for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
       const float h = hidden(c);
-      sum += h * h;
+      sum[0] += h * h;
       store1<RT>(a.hidden, row * a.n + c, h);
     }
     if (a.outer) {
@@ -175,9 +207,15 @@ hipError_t launch(const NormArgs& a, bool wide, hipStream_t stream) {
   }
   const int64_t rows = std::min(a.rows, most / 4);
   const auto threads = [&](int items) { return 64 * ((pieces + 64 * items - 1) / (64 * items)); };
-  if (pieces <= 1024) norm_kernel<DT, RT, 1, true><<<(unsigned)rows, threads(1), 0, stream>>>(a, 64);
-  else if (pieces <= 2048) norm_kernel<DT, RT, 2, true><<<(unsigned)rows, threads(2), 0, stream>>>(a, 64);
-  else norm_kernel<DT, RT, 4, true><<<(unsigned)rows, threads(4), 0, stream>>>(a, 64);
+  // Few rows take as many waves as there are, for the latency; of many rows smaller workgroups keep the loads of one under way while
+  // another waits for its sum. Four pieces a lane against one or two, in us, with the gate and both norms (with one norm), bf16:
+  //   rows of 5120 values:  512: 8.6 : 7.3 (6.5 : 5.5), 1024: 11.3 : 14.1 (8.8 : 9.9), 4096: 36.8 : 41.0 (30.7 : 28.2)
+  //   rows of 8192 values:  512: 10.3 : 11.2 (8.0 : 7.9), 1024: 15.9 : 20.7 (12.6 : 15.5), 4096: 50.9 : 71.8 (43.9 : 47.4)
+  //   rows of 16384 values: 4: 7.9 : 7.1 (5.5 : 4.8), 1024: 30.3 : 36.5 (23.9 : 27.8), 4096: 123 : 152 (104 : 104)
+  // and 4096 rows of 4096 values: 28.7 : 27.3 (24.1 : 22.5).
+  if (pieces > 2048 || (pieces > 512 && a.rows >= 1024)) norm_kernel<DT, RT, 4, true><<<(unsigned)rows, threads(4), 0, stream>>>(a, 64);
+  else if (pieces <= 1024) norm_kernel<DT, RT, 1, true><<<(unsigned)rows, threads(1), 0, stream>>>(a, 64);
+  else norm_kernel<DT, RT, 2, true><<<(unsigned)rows, threads(2), 0, stream>>>(a, 64);
   return hipGetLastError();
 }
 
