@@ -2,12 +2,13 @@
 refuse what they cannot take, with a message, before any GPU access: host tensors here, where a call that passes all
 checks ends with "must be CUDA tensors". And the mask of a batch of trees, which is made on the host."""
 
+import ctypes
 import random
 
 import pytest
 import torch
 
-from test_decoder_api import _cache, _ints
+from test_decoder_api import _cache, _CacheT, _desc, _ints, _T
 
 from vllm_gguf_plugin import decoder
 
@@ -179,3 +180,59 @@ def test_tree_masks():
     for bad in ([0], [-1, 1], [-2], [-1, 0, 5]):
         with pytest.raises(ValueError, match="parent"):
             decoder.tree_mask([bad])
+
+
+def test_tensors_without_memory_are_refused():
+    """A C caller's NULL where a tensor has elements: an error, for each tensor of each entry point. Optional ones may be NULL
+    themselves."""
+    lib = ctypes.CDLL(decoder.LIB_PATH)
+    lib.gguf_decoder_last_error.restype = ctypes.c_char_p
+    i64, f32, P, null = ctypes.c_int64, ctypes.c_float, ctypes.byref, ctypes.c_void_p(None)
+    c = _cache()
+    table, lens, cu, rows, w = torch.zeros(2, 2, dtype=I32), _ints(5, 6), _ints(0, 1, 3), torch.zeros(3, 2, 64), torch.zeros(64)
+    half, mask, x = torch.zeros(3, 4, 64, dtype=F16), torch.zeros(3, 1, dtype=I64), torch.zeros(3, 64)
+    ws = torch.zeros(1 << 20, dtype=torch.uint8)
+    room = (ctypes.c_void_p(ws.data_ptr() + -ws.data_ptr() % 16), ctypes.c_size_t((1 << 20) - 16), null)
+    calls = {
+        "kv8_rotary_append": (["cache", rows, rows, rows, torch.zeros(9, 32), torch.zeros(3, dtype=I64), table, lens, cu, w, w, rows],
+                              lambda a: (*a[:9], i64(2), 0, *a[9:11], f32(1e-6), a[11], null), (9, 10)),
+        "kv8_tree_attention": ([half, "cache", mask, table, lens, cu, half],
+                               lambda a: (*a[:6], i64(2), i64(6), f32(1), a[6], *room), ()),
+        "kv8_keep": (["cache", torch.zeros(2, 4, dtype=I32), table, lens, cu], lambda a: (*a, null), ()),
+        "residual_norm": ([x, x, x, w, w, x, x], lambda a: (*a[:3], 2, *a[3:5], f32(1), f32(1e-6), *a[5:], null), (1, 2, 3)),
+    }
+    for name, (tensors, order, optional) in calls.items():
+        call = getattr(lib, "gguf_" + name)
+
+        def refused(descs, message):
+            assert call(*order([d if d is None else P(d) for d in descs])) == 1
+            assert message in lib.gguf_decoder_last_error().decode(), (name, lib.gguf_decoder_last_error())
+
+        for spoil in range(-1, len(tensors)):
+            for part in range(4 if spoil >= 0 and isinstance(tensors[spoil], str) else 1):
+                descs = [_CacheT(*map(_desc, c)) if isinstance(t, str) else _desc(t) for t in tensors]
+                if spoil >= 0:
+                    d = descs[spoil]
+                    (d if isinstance(d, _T) else getattr(d, ("k", "v", "k_scale", "v_scale")[part])).data = None
+                refused(descs, "must be CUDA tensors" if spoil < 0 else "no data")
+        for spoil in range(len(tensors)):
+            descs = [_CacheT(*map(_desc, c)) if isinstance(t, str) else _desc(t) for t in tensors]
+            descs[spoil] = None
+            refused(descs, "must be CUDA tensors" if spoil in optional else "")
+
+
+def test_tree_workspaces():
+    """Hints beyond every size count as what the tensors hold."""
+    lib = ctypes.CDLL(decoder.LIB_PATH)
+    lib.gguf_kv8_tree_attention_workspace_bytes.restype = ctypes.c_size_t
+    i64, P = ctypes.c_int64, ctypes.byref
+    for d, q_heads, tokens in ((64, 4, 3), (256, 8, 50), (192, 64, 100)):
+        c = _cache(d=d)
+        cache, q = _CacheT(*map(_desc, c)), _desc(torch.zeros(tokens, q_heads, d, dtype=F16))
+
+        def bytes_of(max_new, max_len):
+            return lib.gguf_kv8_tree_attention_workspace_bytes(P(cache), P(q), i64(2), i64(max_new), i64(max_len))
+
+        for hint in (2 ** 62, 2 ** 63 - 1):
+            assert bytes_of(hint, 6) == bytes_of(tokens, 6)
+            assert 0 < bytes_of(hint, hint) == bytes_of(tokens, 2 ** 31 - 1)
