@@ -140,9 +140,8 @@ GGUF_DEC_API int gguf_kv8_rotary_append(const gguf_kv8_cache* cache, const gguf_
 /* kv8_attention for a tree of drafts: row i of sequence s sees positions 0 .. b - 1, b = seq_lens[s] - n_s, and of the sequence's
  * own rows j (at positions b + j) those with bit j % 64 of tree_mask[row, j / 64] set (int64 [tokens, words], unit inner
  * stride; rows past 64 * words are not seen). Usually these are a draft's ancestors and itself, but any bits are allowed. Otherwise
- * as gguf_kv8_attention, but for the workspace, which is needed whole, and for where queries become integers of 15 bits: of
- * R = max_new * q_heads / heads where R is above 32 and R * max_len * sequences * heads at least 2^23 (heads of 192 and 256) or
- * 3 * 2^23 (of 64 and 128). */
+ * as gguf_kv8_attention, but for the workspace, which is needed whole, and for queries, which never become integers: bf16 elements
+ * below 2^-14 of the row's largest alone are rounded. */
 GGUF_DEC_API size_t gguf_kv8_tree_attention_workspace_bytes(const gguf_kv8_cache* cache, const gguf_tensor* query,
                                                             int64_t seqs, int64_t max_new, int64_t max_len);
 GGUF_DEC_API int gguf_kv8_tree_attention(const gguf_tensor* query, const gguf_kv8_cache* cache, const gguf_tensor* tree_mask,

@@ -127,10 +127,7 @@ def test_scales_and_maxima_that_move(dec, scale, hint):
     q = (torch.randn(40, 4, 256, generator=g) * (1 if abs(scale) > 1 else 0.3)).to(BF16).cuda()
     mask = _random_mask(40, 1, g).cuda()
     y = dec.kv8_tree_attention(q, cache, mask, table, _i32(*ends), _cu(news), 40, hint or 700, scale)
-    # the form for many rows takes queries as integers of the row's largest / 16256: half a step of these times keys of some hundreds
-    # is up to 5 here, so the reference has them too (the form for few rows has these queries exactly)
-    amax = q.double().abs().amax(-1, keepdim=True)
-    ref, most = _tree_ref(torch.round(q.double() * 16256 / amax) * amax / 16256 if hint else q, cache, table, mask, ends, news, scale)
+    ref, most = _tree_ref(q, cache, table, mask, ends, news, scale)
     assert torch.isfinite(y).all()
     if abs(scale) < 1:
         _close(y, ref, most)

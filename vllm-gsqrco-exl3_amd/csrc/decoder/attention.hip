@@ -346,15 +346,16 @@ hipError_t launch_attend(const AttnArgs& a, dim3 grid, hipStream_t stream) {
 // Calls in us, one / two tiles, at up to 16384 tokens: head size 64, eight sequences of 64 rows 67.5 / 55.7, of 24 rows
 // 39.2 / 35.6; head size 128, eight of 32 rows 55.3 / 62.6, one of 32 rows 19.4 / 27.8; head size 192, one of 24 rows
 // 15.0 / 18.0, eight of 60 rows 37.9 / 40.4, of 36 rows 45.8 / 38.1.
-// A tree takes its form for many rows (of heads up to 128 attention_rows.hip, beyond attention_tree.hip) by its work, since that form's
-// fixed costs are larger: from 33 rows of a (sequence, KV head) on, and 2^23 of rows times tokens over all of them (3 * 2^23 of heads up
-// to 128). Calls in us, few / many: head size 256, four KV heads, 96 rows of one sequence of 16000 tokens 45.8 / 57.6, of four of 4000
-// 60.3 / 53.0, of eight 75.0 / 53.0; 48 rows of four of 4000 36.7 / 42.9, of eight of 16000 132 / 100, of 32 of 2000 87.8 / 67.6; 24 rows of
-// eight of 16000 92.3 / 98.0; 384 rows of one of 2000 37.5 / 53.5. Head size 192, one KV head, 96 rows of eight of 16000 61.3 / 48.9,
-// 48 rows of these 37.0 / 41.9. Head size 128, eight KV heads, 256 rows of one of 2000 21.6 / 26.5; 64 rows of eight of 4000 38.6 / 42.3,
-// of 32 of 2000 78.3 / 67.5; 32 rows of eight of 16000 86.3 / 102, 48 rows 117 / 105.
+// A tree takes its form for many rows (attention_tree.hip) by its work, since that form's fixed costs are larger: from 33 rows of a
+// (sequence, KV head) on (65 of heads of 64), and 2^23 of rows times tokens over all of them (3 * 2^23 of heads up to 128). Calls in us,
+// few / many: head size 256, four KV heads, 96 rows of one sequence of 16000 tokens 45.2 / 56.8, of four of 4000 59.9 / 52.3, of
+// eight 74.2 / 56.1; 48 rows of four of 4000 36.6 / 43.7, of eight of 16000 129 / 102; 24 rows of eight of 16000 93.3 / 98.1, of 32 of 8000
+// 201 / 182; 384 rows of one of 2000 38.2 / 50.5. Head size 192, one KV head, 96 rows of eight of 16000 60.1 / 48.9, 192 of four of 4000
+// 28.6 / 41.8. Head size 128, eight KV heads, 128 rows of two of 8000 40.1 / 59.6, of four 67.0 / 63.0, of eight of 4000 62.4 / 64.4, of
+// 32 of 4000 303 / 126; 48 rows of eight of 16000 118 / 110, 32 rows 83.8 / 109. Head size 64, eight KV heads, 128 rows of two of 8000
+// 32.3 / 48.7, of 32 of 4000 140 / 84.3; 64 rows of 32 of 2000 43.4 / 52.6, of 16 of 16000 137 / 138.
 static bool tree_many(int d, int64_t rows, int64_t groups, int64_t max_len) {
-  return rows > 32 && (double)rows * (double)groups * (double)max_len >= (d > 128 ? 1 : 3) * 8388608.0;
+  return rows > (d == 64 ? 64 : 32) && (double)rows * (double)groups * (double)max_len >= (d > 128 ? 1 : 3) * 8388608.0;
 }
 
 struct AttnPlan {
@@ -365,7 +366,7 @@ struct AttnPlan {
 
 static AttnPlan attn_plan(int d, int64_t rows, int64_t groups, int64_t max_len, int64_t most, bool tree) {
   AttnPlan p;
-  p.many = tree ? tree_many(d, rows, groups, max_len) : rows > 64;
+  p.many = !tree && rows > 64;
   p.nt = rows > 16 && d < 128 ? 2 : 1;
   const int64_t tile = p.many ? kRowsTile : 16 * p.nt;
   p.row_tiles = (rows + tile - 1) / tile;
@@ -386,7 +387,7 @@ static int64_t most_splits(int64_t rows) { return rows < (1 << 24) ? 512 : 1; }
 
 size_t kv8_attention_workspace(int d, int heads, int hq, int64_t tokens, int64_t seqs, int64_t max_new,
                                int64_t max_len, bool tree) {
-  if (tree && d > 128 && tree_many(d, max_new * (hq / heads), seqs * heads, max_len))
+  if (tree && tree_many(d, max_new * (hq / heads), seqs * heads, max_len))
     return tree_workspace(d, max_new * (hq / heads), tokens, hq, seqs, heads, max_len);
   const AttnPlan p = attn_plan(d, max_new * (hq / heads), seqs * heads, max_len, most_splits(tokens * hq), tree);
   return p.splits == 1 ? 0 : (size_t)p.splits * tokens * hq * (d + 2) * sizeof(float);
@@ -396,7 +397,7 @@ hipError_t launch_kv8_attention(const Kv8& c, int dtype, const void* q, int64_t 
                                 const int32_t* lens, const Ragged& rows, int64_t max_new, int64_t max_len, float scale,
                                 const int64_t* mask, int64_t mask_stride, int words, void* out, void* ws, size_t ws_bytes,
                                 hipStream_t stream) {
-  if (mask && c.d > 128 && tree_many(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len)) {
+  if (mask && tree_many(c.d, max_new * (hq / c.heads), (int64_t)rows.seqs * c.heads, max_len)) {
     const AttnArgs a{c, q, qt, qh, lens, rows, hq, hq / c.heads, scale * kLog2e, 0, 0, out, nullptr, nullptr, mask, mask_stride, words, dtype};
     return launch_attend_tree(a, max_new * (hq / c.heads), max_len, ws, stream);
   }

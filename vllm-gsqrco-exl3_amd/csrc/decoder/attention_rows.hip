@@ -47,8 +47,7 @@ struct Tile {
   float ks[2], vs[2];
 };
 
-// TREE: the rows are drafts. They see the positions before the sequence's own rows, and of these what their mask says.
-template <int DT, int D, bool TREE>
+template <int DT, int D>
 __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_kernel(AttnArgs a) {
   constexpr int KS = D / 32, DD = D / 32;   // steps of the first product, 32-dim tiles of the second
   constexpr int VROW = 2 * kToks + 16;      // bytes of a dim's row of V in LDS
@@ -69,8 +68,6 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
   const int page16 = a.c.page / 16;
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
   const int64_t row_tiles = (nrows + kRowsTile - 1) / kRowsTile;
-  const int64_t base = (int64_t)len0 - (r1 - r0);  // position of the sequence's first row
-  const int64_t drafts = TREE ? min((int64_t)(r1 - r0), (int64_t)64 * a.words) : 0;
 
   // the last rows, which see most, first
   for (int64_t rt = row_tiles - 1 - blockIdx.y; rt >= 0; rt -= gridDim.y) {
@@ -78,12 +75,11 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
     const bool row_ok = r < nrows;
     const int tok = row_ok ? (int)(r / a.group) : 0, hd = head * a.group + (row_ok ? (int)(r % a.group) : 0);
     const int64_t orow = row_ok ? (int64_t)(r0 + tok) * a.hq + hd : -1;
-    const int64_t* mask = TREE ? a.mask + (int64_t)(r0 + tok) * a.mask_stride : nullptr;
     const int64_t lst = row_ok ? (int64_t)len0 - (r1 - r0) + tok : -1;
     const int last = (int)(lst < room ? lst : room - 1);
     // what the tile's rows see: rows are in order of their tokens
     const int64_t rlast = min(nrows, (rt + 1) * kRowsTile) - 1;
-    const int64_t see64 = min(TREE ? (int64_t)len0 - 1 : (int64_t)len0 - (r1 - r0) + rlast / a.group, room - 1);
+    const int64_t see64 = min((int64_t)len0 - (r1 - r0) + rlast / a.group, room - 1);
     const int see = (int)max(see64, (int64_t)-1);
     const int ntiles = (see + kToks) / kToks;
     const int tb = (int)min((int64_t)split * (a.span / kToks), (int64_t)ntiles);
@@ -229,8 +225,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = (s[e] << 7) + lo[e];
     };
-    // the last position that every row sees: the first row's last one, or of a tree the one before its rows
-    const int first_last = (int)min((int64_t)len0 - (r1 - r0) + (TREE ? -1 : rt * kRowsTile / a.group), room - 1);
+    const int first_last = (int)min((int64_t)len0 - (r1 - r0) + rt * kRowsTile / a.group, room - 1);  // of the first row
 
     // Turn t multiplies tile t + 1's K beside tile t's softmax, then tile t's V, so that the matrix cores run on while a
     // wave works on its scores: it is alone on its SIMD (at D = 256 a wave needs some 400 registers). What a turn
@@ -259,23 +254,15 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
 
       // the rows' statistics
       const int seen = last - (kToks * t + 8 * h);  // place 16 c + e of the lane is seen if it is at most this
-      uint32_t bits[2] = {0xFFFF, 0xFFFF};          // of a tree: the tokens of either chunk that the row sees
-      if constexpr (TREE && kMasked)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) bits[c] = tree_bits(mask, kToks * t + 16 * c, base, drafts, room);
-      const auto sees = [&](int c, int e) __attribute__((always_inline)) {
-        return !kMasked || (TREE ? (bits[c] >> (8 * h + e) & 1) != 0 : 16 * c + e <= seen);
-      };
       // the largest V scale of the chunks that the row sees; a NaN counts for nothing
-      const float top = fmaxf((TREE ? bits[0] != 0 : !kMasked || last >= kToks * t) ? x0.vs[0] : 0.0f,
-                              (TREE ? bits[1] != 0 : !kMasked || last >= kToks * t + 16) ? x0.vs[1] : 0.0f);
+      const float top = fmaxf(!kMasked || last >= kToks * t ? x0.vs[0] : 0.0f, !kMasked || last >= kToks * t + 16 ? x0.vs[1] : 0.0f);
       const float f[2] = {qs * x0.ks[0], qs * x0.ks[1]};
       float mx = kNoScore;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         int big = INT32_MIN;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = max(big, sees(c, e) ? s[8 * c + e] : INT32_MIN);
+        for (int e = 0; e < 8; ++e) big = max(big, !kMasked || 16 * c + e <= seen ? s[8 * c + e] : INT32_MIN);
         if (!kMasked || big != INT32_MIN) mx = fmaxf(mx, (float)big * f[c]);
       }
       mx = half_max(mx);
@@ -307,7 +294,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
           asm("" : "+v"(x));  // rounded as it was for the maximum: of scores beyond 2^24 an fma's rest would pass any weight
           float w = __builtin_amdgcn_exp2f(x - m);
           float y = w * vr;
-          if (!sees(c, e)) w = y = 0.0f;  // also where the page's scale is not finite
+          if (kMasked && 16 * c + e > seen) w = y = 0.0f;  // also where the page's scale is not finite
           l += w;
           p[c][e] = (_Float16)y;
         }
@@ -361,15 +348,12 @@ __global__ void __launch_bounds__(64 * kRowWaves, D <= 128 ? 2 : 1) attend_rows_
 
 hipError_t launch_attend_rows(const AttnArgs& a, int dtype, int64_t row_tiles, hipStream_t stream) {
   const dim3 grid((unsigned)(a.rows.seqs * a.c.heads * a.splits), (unsigned)(row_tiles < 65535 ? row_tiles : 65535));
-#define GGUF_DEC_ROWS_D(DT, D)                                                                                  \
-  if (D > 128 || !a.mask) attend_rows_kernel<DT, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a);             \
-  else attend_rows_kernel<DT, D, D <= 128><<<grid, 64 * kRowWaves, 0, stream>>>(a);  // (larger heads: attention_tree.hip)
-#define GGUF_DEC_ROWS(DT)                            \
-  switch (a.c.d) {                                   \
-    case 64: GGUF_DEC_ROWS_D(DT, 64) break;          \
-    case 128: GGUF_DEC_ROWS_D(DT, 128) break;        \
-    case 192: GGUF_DEC_ROWS_D(DT, 192) break;        \
-    default: GGUF_DEC_ROWS_D(DT, 256) break;         \
+#define GGUF_DEC_ROWS(DT)                                                                         \
+  switch (a.c.d) {                                                                                \
+    case 64: attend_rows_kernel<DT, 64><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;           \
+    case 128: attend_rows_kernel<DT, 128><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;         \
+    case 192: attend_rows_kernel<DT, 192><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;         \
+    default: attend_rows_kernel<DT, 256><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;          \
   }
   if (dtype == kF16) {
     GGUF_DEC_ROWS(kF16)
@@ -377,7 +361,6 @@ hipError_t launch_attend_rows(const AttnArgs& a, int dtype, int64_t row_tiles, h
     GGUF_DEC_ROWS(kBF16)
   }
 #undef GGUF_DEC_ROWS
-#undef GGUF_DEC_ROWS_D
   return hipGetLastError();
 }
 

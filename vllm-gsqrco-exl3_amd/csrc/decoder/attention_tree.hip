@@ -1,23 +1,29 @@
-// Attention for trees of drafts over the 8-bit paged cache, for many rows a KV head of 192 or 256 dims: some ten to some hundred
-// rows that all see a long context, and of each other what their masks say (attend.h: tree_bits).
+// Attention for trees of drafts over the 8-bit paged cache, for many rows a KV head: some ten to some hundred rows that all see a
+// long context, and of each other what their masks say.
 //
-// Products and operands are those of attention_rows.hip: S^T = K Q^T in int8 with Q as two planes, O^T += V^T P^T in fp16,
-// 32 x 32 MFMAs, a lane keeps its query row. What differs:
-//   - Two waves share 32 rows, so that either holds half of the output's dims, and two waves fit a SIMD. Of a tile of 64
-//     tokens each takes 32 scores a row; weights and running maxima go to the partner through LDS. A maximum lags its scores by up to
-//     2^8 and is a whole number, so that a partner's weights are brought to the larger of the two by a power of two, exactly.
+// Both products are transposed, S^T = K Q^T and O^T += V^T P^T, in fp16 with 32 x 32 MFMAs, so that a lane keeps one query row. With
+// lane = 32 h + n, a result's element i is row 8 (i >> 2) + 4 h + (i & 3) of column n; the 32 tokens of a block stand in K's rows in
+// such an order that the lane's 8 scores i = 8 c .. 8 c + 7 are its places of the c-th step of the second product: tokens 16 c +
+// 8 h + 0 .. 7. Scores never cross lanes. Codes become fp16 on the way to LDS, exactly.
+//   - A tile is 64 tokens. Up to 128 dims a wave takes 32 rows for itself; beyond, two waves share 32 rows (PAIR), either with half
+//     of the output's dims, so that two waves fit a SIMD, and each takes 32 scores a row; weights and running maxima go to the partner
+//     through LDS. A maximum lags its scores by up to 2^8 and is a whole number, so that a partner's weights are brought to the larger
+//     of the two by a power of two, exactly.
 //   - A wave's tile is two steps, products and weights, and the two waves of a SIMD are a step apart: one's matrix instructions run
-//     beside the other's softmax and conversion of V. (All in one step, a barrier a tile: 218 us for 8 sequences of 21 drafts at 32768
-//     tokens, as attention_rows.hip's kernel has it 236; the steps apart: 120.)
+//     beside the other's softmax and conversions. (32 sequences of 64 drafts at 8192 tokens, 32 query and 8 KV heads of 128: 413 us,
+//     in step 455; at 256 dims, where partners wait for each other anyway, no difference.)
 //   - The tiles of all (sequence, head, row tile)s in a line are cut into equal shares, one a workgroup and CU, whatever the lengths
 //     are. A workgroup whose share begins or ends inside a group leaves its sums to join_tree_kernel; a group that lies in one share is
 //     written at once.
-// Queries are rounded to integers of 15 bits a row and weights to fp16; scores are exact sums of integers, times fp32 scales; sums of
-// weights and outputs are fp32.
+// Queries are exact in fp16, but for bf16 elements below 2^-14 of the row's largest, and weights are rounded to fp16; scores, sums of
+// weights and outputs are fp32. As integers in two int8 planes, queries cost two instructions more a score and as much matrix time:
+// up to 128 dims slower (502 us to 419, the case above), beyond quicker (206 to 217, 21 drafts of 8 sequences of 32768 tokens, 24 query and
+// 4 KV heads of 256), where a second set of operands and rounded queries were not worth it.
 //
-// What bounds it: of a step at 256 dims the products take some 1550 cycles of the matrix units, weights and conversions some 2000 to
-// 2300 of the vector units, LDS and barriers, beside them. 16 drafts of 8 ragged sequences to 32768 tokens, 24 query and 4 KV heads of
-// 256 dims: 104 us, 47 drafts of 4 to 16000: 90 (the products alone: 42 and 23).
+// What bounds it: a step takes some 2100 to 2500 cycles, the products' 32 matrix instructions 1024 of them on a SIMD; the weights' 270 to
+// 300 vector instructions, 16 or 32 of them exponentials, with their waits for LDS and each other the rest. 16 drafts of 8 ragged sequences
+// to 32768 tokens (24 query and 4 KV heads of 256): 104 us, 47 drafts of 4 to 16000: 88, 64 drafts of 32 to 8192 (32 query and 8 KV heads
+// of 128): 222; the products alone 42, 23 and 102.
 #include <algorithm>
 #include <type_traits>
 
@@ -27,13 +33,11 @@ namespace gguf_dec {
 
 namespace {
 
-typedef int intx4 __attribute__((ext_vector_type(4)));
-typedef int intx16 __attribute__((ext_vector_type(16)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kToks = 64;                // tokens of a tile
 constexpr int kVRow = 2 * kToks + 16;    // bytes of a dim's row of V in LDS; 16 more than its values, for the banks
-constexpr int kAhead = 32;               // tiles whose chunks are looked up at a time
+constexpr int kAhead = 16;               // tiles whose chunks are looked up at a time
 constexpr int kPlaces = 4 * 2 * kAhead;  // places of chunks that are held: those of tile t at 4 (t % (2 kAhead))
 constexpr int kLeastTiles = 4;           // of a workgroup's share
 
@@ -58,7 +62,7 @@ struct Cut {
 
 // Queries as the products take them, and the line of all tiles, cut: what prep_tree_kernel leaves.
 struct Prep {
-  int8_t* q;       // [tokens * hq][2][d]: integers of 15 bits, in two planes
+  _Float16* q;     // [tokens * hq][d]: times a power of two that brings the row's largest to 1 .. 2, and the call's scale's sign
   float* qs;       // [tokens * hq]: what they are multiplied by, with the call's scale
   int64_t* line;   // [seqs + 1]: tiles before a sequence's
   int* begins;     // [shares]: the sequence in which a share begins
@@ -66,16 +70,18 @@ struct Prep {
   Cut* cut;        // [shares]
 };
 
-template <int D, int NG>
+// PAIR: two waves share 32 rows
+template <int D, int NW>
 struct Lay {
-  static constexpr int kThreads = 128 * NG, kRows = 32 * NG;
-  static constexpr int kKRow = D + 16;                           // bytes of a token's row of K
+  static constexpr bool kPair = D > 128;
+  static constexpr int kThreads = 64 * NW, kRows = kPair ? 16 * NW : 32 * NW;
+  static constexpr int kKRow = 2 * D + 16;                       // bytes of a token's row of K
   static constexpr int kK = 0;                                   // [2][64][kKRow]
   static constexpr int kV = kK + 2 * kToks * kKRow;              // [2][D][kVRow]
-  static constexpr int kP = kV + 2 * D * kVRow;                  // [waves][2][64] x 16 bytes
-  static constexpr int kPlace = kP + 2 * NG * 2048;              // Place [kPlaces]
-  static constexpr int kStat = kPlace + 24 * kPlaces;            // float [waves][32]
-  static constexpr int kBytes = kStat + 2 * NG * 128;
+  static constexpr int kP = kV + 2 * D * kVRow;                  // [waves][2][64] x 16 bytes, of pairs
+  static constexpr int kPlace = kP + (kPair ? NW * 2048 : 0);    // Place [kPlaces]
+  static constexpr int kStat = kPlace + 24 * kPlaces;            // float [waves][32], of pairs
+  static constexpr int kBytes = kStat + (kPair ? NW * 128 : 0);
 };
 
 // tiles of a sequence's rows: 0 without rows, at least one with them (it writes the zeros of rows that see nothing)
@@ -97,6 +103,28 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s, int rows) {
   return q;
 }
 
+// The two words of a row's mask that hold the tile at position `at`; nothing is read beyond the mask's `count` rows.
+struct Words {
+  uint64_t lo, hi;
+};
+
+__device__ __forceinline__ Words words_of(const int64_t* mask, int at, int base, int count) {
+  const int64_t from = (int64_t)at - base, i = from >> 6;  // (the tile begins in word i, or before the first)
+  Words w{0, 0};
+  if (i >= 0 && 64 * i < count) w.lo = (uint64_t)mask[i];
+  if (i + 1 >= 0 && 64 * (i + 1) < count) w.hi = (uint64_t)mask[i + 1];
+  return w;
+}
+
+// What the row sees of the tile, a bit a token (attend.h: tree_bits).
+__device__ __forceinline__ uint64_t seen_of(const Words& w, int at, int base, int count, int room) {
+  const auto below = [](int64_t n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+  const int64_t from = (int64_t)at - base;
+  const int shift = (int)(from & 63);
+  const uint64_t own = shift ? w.lo >> shift | w.hi << (64 - shift) : w.lo;
+  return ((own & below(count - from)) | below(-from)) & below((int64_t)room - at);
+}
+
 // How the line of all tiles is cut: share w of `shares` is [w total / shares, (w + 1) total / shares).
 struct Line {
   int64_t total, shares;
@@ -106,12 +134,12 @@ struct Line {
   __device__ int64_t begin(int64_t w) const { return w * total / shares; }
 };
 
-// Queries as integers (attention_rows.hip), a wave a row; and, by the last workgroup, the tiles before each sequence's, where the
+// Queries in fp16, four values a lane; and, by the first workgroup, the tiles before each sequence's, where the
 // shares begin, and which groups they cut.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int rows, int64_t most) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (blockIdx.x + 1 == gridDim.x) {
+  if (blockIdx.x == 0) {
     __shared__ int64_t part[4];
     int64_t total = 0;
     for (int s0 = 0; s0 < a.rows.seqs; s0 += 256) {
@@ -160,10 +188,11 @@ __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int 
     }
     return;
   }
+  constexpr int L = D == 192 ? 64 : D / 4, ROWS = 256 / L;  // lanes of a row (of 192 dims some idle), rows a workgroup
   const int64_t all = (int64_t)a.rows.tokens * a.hq;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < all; r += (int64_t)(gridDim.x - 1) * 4) {
-    const int64_t tok = r / a.hq;
-    const int at = min(4 * lane, D - 4);  // four values a lane
+  const int at = min(4 * (tid % L), D - 4);
+  for (int64_t r0 = ((int64_t)blockIdx.x - 1) * ROWS; r0 < all; r0 += (int64_t)(gridDim.x - 1) * ROWS) {
+    const int64_t r = min(r0 + tid / L, all - 1), tok = r / a.hq;  // (lanes past the last row take it again)
     const uint2 w = *(const uint2*)((const uint16_t*)a.q + tok * a.qt + (r - tok * a.hq) * a.qh + at);
     const uint32_t bits[4] = {w.x & 0xFFFF, w.x >> 16, w.y & 0xFFFF, w.y >> 16};
     float v[4];
@@ -174,23 +203,11 @@ __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int 
       big = max(big, __float_as_uint(v[e]) & 0x7FFFFFFFu);
     }
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off, 64));
-    const float amax = __uint_as_float(big);
-    // a row of magnitudes below 2^-100 has scores of 0
-    const float inv = amax >= 0x1p-100f && amax < __builtin_inff() ? (a.scale < 0.0f ? -16256.0f : 16256.0f) / amax : 0.0f;
-    uint32_t hi = 0, lo = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int x = (int)rintf(v[e] * inv), top = (x + 64) >> 7;
-      hi |= (uint32_t)(top & 0xFF) << 8 * e;
-      lo |= (uint32_t)((x - 128 * top) & 0xFF) << 8 * e;
-    }
-    if (4 * lane < D) {
-      *(uint32_t*)(p.q + r * 2 * D + at) = hi;
-      *(uint32_t*)(p.q + r * 2 * D + D + at) = lo;
-    }
-    // not negative: the scale's sign is the integers'
-    if (lane == 0) p.qs[r] = amax < __builtin_inff() ? fabsf(a.scale) * (amax * (1.0f / 16256.0f)) : __builtin_nanf("");
+    for (int off = 1; off < L; off <<= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off, 64));
+    const float amax = __uint_as_float(big), by = row_factor(amax), to = a.scale < 0.0f ? -by : by;
+    *(uint2*)(p.q + r * D + at) = make_uint2(pack2<kF16>(v[0] * to, v[1] * to), pack2<kF16>(v[2] * to, v[3] * to));
+    // not negative: the scale's sign is the queries'
+    if (tid % L == 0) p.qs[r] = amax < __builtin_inff() ? fabsf(a.scale) / by : __builtin_nanf("");
   }
 }
 
@@ -200,20 +217,23 @@ __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int 
 // to LDS), with a barrier behind each. The first four waves, one a SIMD, and the others (LAG: there are others) are a step apart,
 // so that on a SIMD one wave's products run beside the other's weights. The first bring V: tile t's in the step of its weights, over
 // tile t - 2's, which the others have read a step before. The others bring K: tile t + 2's in the step of tile t's weights, over tile t's.
-template <int D, int NG>
-__global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(NG > 2 ? 2 : 1, NG > 2 ? 2 : 1))) attend_tree_kernel(AttnArgs a, Prep prep, int64_t most) {
-  using L = Lay<D, NG>;
-  constexpr bool LAG = NG > 2;
-  constexpr int KS = D / 32, DD = D / 64;       // steps of the first product; 32-dim tiles of the wave's half of the dims
+template <int D, int NW>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 || D <= 128 ? 2 : 1, NW > 4 || D <= 128 ? 2 : 1)))
+attend_tree_kernel(AttnArgs a, Prep prep, int64_t most) {
+  using L = Lay<D, NW>;
+  constexpr bool LAG = NW > 4, PAIR = L::kPair;
+  constexpr int KS = D / 16;                    // steps of the first product
+  constexpr int DD = PAIR ? D / 64 : D / 32;    // 32-dim tiles of the wave's dims: of a pair's wave half of all
+  constexpr int B = PAIR ? 1 : 2;               // the wave's blocks of 32 tokens of a tile
   constexpr int PIECES = 4 * D;                 // 16-byte pieces of a tile's K, and of its V
-  constexpr int FIRST = LAG ? 256 : L::kThreads / 2;  // threads that bring V, and as many K
+  constexpr int FIRST = L::kThreads / 2;        // threads that bring V, and as many K
   constexpr int NP = PIECES / FIRST;
-  static_assert(PIECES % FIRST == 0 && L::kThreads == 2 * FIRST, "whole turns");
+  static_assert(PIECES % FIRST == 0, "whole turns");
   extern __shared__ __align__(16) char lds[];
   Place* places = (Place*)(lds + L::kPlace);
   float* stat = (float*)(lds + L::kStat);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
-  const int rg = wave >> 1, half = wave & 1;
+  const int rg = PAIR ? wave >> 1 : wave, half = PAIR ? wave & 1 : 0;
   const bool brings_v = wave < FIRST / 64, late = LAG && !brings_v;
   const int room = (int)min((int64_t)a.c.max_pages * a.c.page, (int64_t)INT32_MAX);
 
@@ -278,7 +298,9 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const uint32_t p = j * FIRST + me;
-        *(uintx4*)(lds + L::kK + (t & 1) * kToks * L::kKRow + p / (D / 16) * L::kKRow + 16 * (p % (D / 16))) = raw[j];
+        char* to = lds + L::kK + (t & 1) * kToks * L::kKRow + p / (D / 16) * L::kKRow + 32 * (p % (D / 16));
+        *(half8*)to = codes8(raw[j][0], raw[j][1]);
+        *(half8*)(to + 16) = codes8(raw[j][2], raw[j][3]);
       }
     };
     __syncthreads();  // what the last piece left in LDS has been read
@@ -304,15 +326,12 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
       return x;
     };
 
-    intx4 qhi[KS], qlo[KS];
+    half8 qf[KS];
     const Row row = row_of();
     const float qs = prep.qs[row.at];
-    const int8_t* qp = prep.q + row.at * 2 * D + 16 * h;
+    const _Float16* qp = prep.q + row.at * D + 8 * h;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      qhi[i] = *(const intx4*)(qp + 32 * i);
-      qlo[i] = *(const intx4*)(qp + D + 32 * i);
-    }
+    for (int i = 0; i < KS; ++i) qf[i] = *(const half8*)(qp + 16 * i);
     if (brings_v) {
       load_v(tb);
     } else {
@@ -329,39 +348,40 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) asm volatile("" : "+v"(qhi[i]), "+v"(qlo[i]));  // here: not waited for with the tiles' loads
+    for (int i = 0; i < KS; ++i) asm volatile("" : "+v"(qf[i]));  // here: not waited for with the tiles' loads
 
     half8* const weights = (half8*)(lds + L::kP);  // [waves][2][64]: for the waves' partners
     const int krow = 32 * half + 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);  // token of K's row n
     const char* const k0 = lds + L::kK + krow * L::kKRow + 16 * h;
     const char* const v0 = lds + L::kV + (half * (D / 2) + n) * kVRow + 16 * h;
-    half8 p[2], pp[2];  // the weights of a tile, the wave's own and its partner's
-    // The products of a step, two MFMAs at a time: O^T of tile t - 1 (the wave's half of the dims; its own tokens' weights, then its
-    // partner's), then S^T of the wave's 32 tokens of tile t. Operands are read two pairs ahead.
+    half8 p[4];  // the weights of a tile: the wave's own, then its partner's
+    // The products of a step, two MFMAs at a time: O^T of tile t - 1 (the wave's dims; its own tokens' weights, then its
+    // partner's), then S^T of the wave's tokens of tile t. Operands are read two pairs ahead.
     // BACK: the first, FRONT: the second.
-    intx16 hi, lo;
+    floatx16 s[B];
     const auto products = [&](int t, auto back, auto front) __attribute__((always_inline)) {
       constexpr bool BACK = decltype(back)::value, FRONT = decltype(front)::value;
-      constexpr int P2 = BACK ? 2 * DD : 0, PAIRS = P2 + (FRONT ? KS : 0);
+      constexpr int P2 = BACK ? 2 * DD : 0, PAIRS = P2 + (FRONT ? B * KS / 2 : 0);
       const char* const vt = v0 + ((t - 1) & 1) * D * kVRow;
       const char* const kt = k0 + (t & 1) * kToks * L::kKRow;
       half8 v[BACK ? 4 * DD : 1];
-      intx4 k[KS];
+      half8 k[B * KS];  // of a block of tokens, or of two in turn
       const auto fetch = [&](int r) __attribute__((always_inline)) {  // the operands of pair r
         if (r < P2) {
 #pragma unroll
           for (int f = 2 * r; f < 2 * r + 2; ++f)
             v[f] = *(const half8*)(vt + 64 * (half ^ (f / DD >> 1)) + 32 * (f / DD & 1) + 32 * (f % DD) * kVRow);
         } else if (r < PAIRS) {
-          k[r - P2] = *(const intx4*)(kt + 32 * (r - P2));
+#pragma unroll
+          for (int f = 2 * (r - P2); f < 2 * (r - P2) + 2; ++f) k[f] = *(const half8*)(kt + f % B * 32 * L::kKRow + 32 * (f / B));
         }
       };
-      if constexpr (BACK) {
+      if constexpr (BACK && PAIR) {
         const int me = again(lane);
         const float other = stat[32 * (wave ^ 1) + (me & 31)];
         const half8* const theirs = weights + 64 * 2 * (wave ^ 1) + me;
-        pp[0] = theirs[0];
-        pp[1] = theirs[64];
+        p[2] = theirs[0];
+        p[3] = theirs[64];
         fetch(0);
         fetch(1);
         if (__any(other != m)) {  // one of the partners has raised its maximum: both go on with the larger
@@ -371,10 +391,7 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
 #pragma unroll
           for (int i = 0; i < DD; ++i) o[i] *= al;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {  // by powers of two: the maxima are whole numbers
-            p[c] *= (_Float16)al;
-            pp[c] *= (_Float16)be;
-          }
+          for (int c = 0; c < 4; ++c) p[c] *= (_Float16)(c < 2 ? al : be);  // by powers of two: the maxima are whole numbers
         }
       } else {
         fetch(0);
@@ -382,7 +399,9 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
       }
       if constexpr (FRONT) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) hi[e] = lo[e] = 0;
+        for (int c = 0; c < B; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[c][e] = 0.0f;
       }
 #pragma unroll
       for (int r = 0; r < PAIRS; ++r) {
@@ -391,10 +410,11 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
         if (r < P2) {
 #pragma unroll
           for (int f = 2 * r; f < 2 * r + 2; ++f)
-            o[f % DD] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[f], f / DD < 2 ? p[f / DD] : pp[f / DD - 2], o[f % DD], 0, 0, 0);
+            o[f % DD] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[f], p[f / DD], o[f % DD], 0, 0, 0);
         } else {
-          hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[r - P2], qhi[r - P2], hi, 0, 0, 0);
-          lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[r - P2], qlo[r - P2], lo, 0, 0, 0);
+#pragma unroll
+          for (int f = 2 * (r - P2); f < 2 * (r - P2) + 2; ++f)
+            s[f % B] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[f], qf[f / B], s[f % B], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -403,11 +423,18 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
     __syncthreads();
     if (late) __syncthreads();
     for (int t = tb; t < te; ++t) {
+      const bool masked = kToks * t + kToks > open;  // some row does not see all
+      Words words{0, 0};
+      if (masked) words = words_of(a.mask + row_of().tok * a.mask_stride, kToks * t, base, drafts);
       if (t > tb) products(t, std::true_type(), std::true_type());
       else products(t, std::false_type(), std::true_type());
       const Place* at = places_of(t);
-      float own[2] = {at[2 * half].vs, at[2 * half + 1].vs};
-      const float f[2] = {qs * at[2 * half].ks, qs * at[2 * half + 1].ks};
+      float own[2 * B], f[2 * B];  // of the wave's chunks
+#pragma unroll
+      for (int c = 0; c < 2 * B; ++c) {
+        own[c] = at[2 * half + c].vs;
+        f[c] = qs * at[2 * half + c].ks;
+      }
       // the largest V scale of the chunks that the row sees (a NaN counts for nothing)
       float highest = fmaxf(fmaxf(at[0].vs, at[1].vs), fmaxf(at[2].vs, at[3].vs));
       __syncthreads();
@@ -420,31 +447,39 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
         put_k(t);  // tile t + 2's, in tile t's place
         load_k(min(t + 3, tlast));
       }
-      floatx16 s;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float x = (float)((hi[e] << 7) + lo[e]) * f[e >> 3];
-        asm("" : "+v"(x));  // rounded here: of scores beyond 2^24 an fma's rest would pass any weight
-        s[e] = x;
-      }
-      if (kToks * t + kToks > open) {
+      // scores are s f. Where some row does not see all, or scores are so large that an fma's rest would pass any weight, they are
+      // multiplied for themselves, and f is 1.
+      const auto scaled = [&](int c, int e) __attribute__((always_inline)) {
+        float x = s[c][e] * f[2 * c + (e >> 3)];
+        asm("" : "+v"(x));
+        return x;
+      };
+      if (masked) {
+        const uint64_t seen = seen_of(words, kToks * t, base, drafts, room);
         highest = 0.0f;
-        const int64_t* mask = a.mask + row_of().tok * a.mask_stride;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c)
-          if (tree_bits(mask, kToks * t + 16 * c, base, drafts, room)) highest = fmaxf(highest, at[c].vs);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t bits = tree_bits(mask, kToks * t + 32 * half + 16 * c, base, drafts, room);
+        for (int c = 0; c < 4; ++c)
+          if (seen >> 16 * c & 0xFFFF) highest = fmaxf(highest, at[c].vs);
+#pragma unroll
+        for (int c = 0; c < 2 * B; ++c) {
+          const uint32_t bits = (uint32_t)(seen >> (32 * half + 16 * c)) & 0xFFFF;
           if (bits == 0) own[c] = 0.0f;  // also where the page's scale is not finite
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!(bits >> (8 * h + e) & 1)) s[8 * c + e] = -__builtin_inff();
+          for (int e = 0; e < 8; ++e) {
+            const float x = scaled(c >> 1, 8 * (c & 1) + e);
+            s[c >> 1][8 * (c & 1) + e] = bits >> (8 * h + e) & 1 ? x : -__builtin_inff();
+          }
+          f[c] = 1.0f;
         }
       }
       float mx = kNoScore;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
+      for (int c = 0; c < 2 * B; ++c) {
+        float big = s[c >> 1][8 * (c & 1)];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) big = fmaxf(big, s[c >> 1][8 * (c & 1) + e]);
+        mx = fmaxf(mx, big * f[c]);
+      }
       mx = half_max(mx);
       // the maximum may lag: weights stay below 2^8, and the sums are scaled again only where it does not do, or
       // where the largest V scale grew
@@ -459,19 +494,30 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
         ref = nref;
         inv_ref = nref > 0.0f ? kWeight / nref : 0.0f;
       }
-      const int me = again(lane);
-      half8* const ours = weights + 64 * 2 * wave + me;
-      stat[32 * wave + (me & 31)] = m;
+      if (__any(fabsf(m) > 0x1p20f)) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 2 * B; ++c) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[c >> 1][8 * (c & 1) + e] = scaled(c >> 1, 8 * (c & 1) + e);
+          f[c] = 1.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2 * B; ++c) {
         const float vr = own[c] * inv_ref;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float w = __builtin_amdgcn_exp2f(s[8 * c + e] - m);
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 1][8 * (c & 1) + e], f[c], -m));
           l += w;
           p[c][e] = (_Float16)(w * vr);
         }
-        ours[64 * c] = p[c];
+      }
+      if constexpr (PAIR) {
+        const int me = again(lane);
+        half8* const ours = weights + 64 * 2 * wave + me;
+        stat[32 * wave + (me & 31)] = m;
+        ours[0] = p[0];
+        ours[64] = p[1];
       }
       __syncthreads();
     }
@@ -481,13 +527,16 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
 
     // the rows' sums over both halves of the tokens
     l += __shfl_xor(l, 32, 64);
-    if (h == 0) stat[32 * wave + n] = l;
-    __syncthreads();
+    if constexpr (PAIR) {
+      if (h == 0) stat[32 * wave + n] = l;
+      __syncthreads();
+      l += stat[32 * (wave ^ 1) + n];
+    }
     const Row mine = row_of();
     if (!mine.ok) continue;
-    const float all = l + stat[32 * (wave ^ 1) + n], by = ref / kWeight;
+    const float by = ref / kWeight;
     if (whole) {
-      const float inv = all == 0.0f ? 0.0f : by / all;
+      const float inv = l == 0.0f ? 0.0f : by / l;
 #pragma unroll
       for (int i = 0; i < DD; ++i)
 #pragma unroll
@@ -505,15 +554,16 @@ __global__ void __launch_bounds__(128 * NG) __attribute__((amdgpu_waves_per_eu(N
         for (int e = 0; e < 16; e += 4)
           *(floatx4*)(a.part + r * D + half * (D / 2) + 32 * i + 2 * e + 4 * h) =
               floatx4{o[i][e] * by, o[i][e + 1] * by, o[i][e + 2] * by, o[i][e + 3] * by};
-      if (h == 0 && half == 0) *(float2*)(a.stat + r * 2) = make_float2(m, all);
+      if (h == 0 && half == 0) *(float2*)(a.stat + r * 2) = make_float2(m, l);
     }
   }
 }
 
-// Joins the rows of the groups that are cut, one at a time: its waves take the parts in turn, D / 64 dims a lane, and join through LDS.
+// Joins the rows of the groups that are cut. Of few parts a wave takes some rows at a time, all loads under way at once; of many a
+// workgroup takes a row, its waves the parts in turn.
 template <int D>
 __global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, int rows) {
-  constexpr int E = D / 64;
+  constexpr int E = D / 64, FEW = 4;
   __shared__ float sums[4][64][E];
   __shared__ float ls[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -523,11 +573,47 @@ __global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, i
     const Seq q = seq_of(a, cut.seq, rows);
     const int head = (int)(cut.group / q.row_tiles), rt = (int)(cut.group - (int64_t)head * q.row_tiles);
     const int64_t nrows = min((int64_t)rows, (int64_t)q.n * a.group - (int64_t)rt * rows);
-    for (int64_t r = blockIdx.x; r < nrows; r += gridDim.x) {
+    const auto slot = [&](int w, int64_t r) { return (2 * (int64_t)w + (w == cut.first && !cut.own)) * rows + r; };
+    const auto store = [&](int64_t r, int at, auto& v, float sum) __attribute__((always_inline)) {
       const int64_t row = (int64_t)rt * rows + r;
-      const auto slot = [&](int w) { return (2 * (int64_t)w + (w == cut.first && !cut.own)) * rows + r; };
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int64_t to = ((int64_t)(q.r0 + row / a.group) * a.hq + head * a.group + row % a.group) * D + at;
+#pragma unroll
+      for (int e = 0; e < (int)(sizeof(v) / 4); ++e) {
+        if (a.dtype == kF16) store1<kF16>(a.out, to + e, v[e] * inv);
+        else store1<kBF16>(a.out, to + e, v[e] * inv);
+      }
+    };
+    if (cut.last - cut.first < FEW) {  // uniform
+      constexpr int L = D == 192 ? 64 : D / 4;  // lanes of a row, four dims each (of 192 some do another's over)
+      const int at = min(4 * (lane % L), D - 4);
+      for (int64_t r = ((int64_t)blockIdx.x * 4 + wave) * (64 / L) + lane / L; r < nrows; r += (int64_t)gridDim.x * (256 / L)) {
+        float2 ml[FEW];
+        floatx4 v[FEW];
+#pragma unroll
+        for (int j = 0; j < FEW; ++j) {
+          const bool ok = cut.first + j <= cut.last;
+          const int64_t from = slot(ok ? cut.first + j : cut.first, r);
+          ml[j] = ok ? *(const float2*)(a.stat + from * 2) : make_float2(kNoScore, 0.0f);
+          v[j] = ok ? *(const floatx4*)(a.part + from * D + at) : floatx4{0, 0, 0, 0};
+        }
+        float mx = ml[0].x, sum = 0.0f, acc[4] = {};
+#pragma unroll
+        for (int j = 1; j < FEW; ++j) mx = fmaxf(mx, ml[j].x);
+#pragma unroll
+        for (int j = 0; j < FEW; ++j) {
+          const float f = __builtin_amdgcn_exp2f(ml[j].x - mx);
+          sum += ml[j].y * f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += v[j][e] * f;
+        }
+        store(r, at, acc, sum);
+      }
+      continue;
+    }
+    for (int64_t r = blockIdx.x; r < nrows; r += gridDim.x) {
       float mx = kNoScore;
-      for (int w = cut.first + lane; w <= cut.last; w += 64) mx = fmaxf(mx, a.stat[slot(w) * 2]);
+      for (int w = cut.first + lane; w <= cut.last; w += 64) mx = fmaxf(mx, a.stat[slot(w, r) * 2]);
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
       float sum = 0.0f, acc[E];
@@ -535,26 +621,20 @@ __global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, i
       for (int e = 0; e < E; ++e) acc[e] = 0.0f;
 #pragma unroll 4
       for (int w = cut.first + wave; w <= cut.last; w += 4) {
-        const float2 ml = *(const float2*)(a.stat + slot(w) * 2);
+        const float2 ml = *(const float2*)(a.stat + slot(w, r) * 2);
         const float f = __builtin_amdgcn_exp2f(ml.x - mx);
         sum += ml.y * f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += a.part[slot(w) * D + E * lane + e] * f;
+        for (int e = 0; e < E; ++e) acc[e] += a.part[slot(w, r) * D + E * lane + e] * f;
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) sums[wave][lane][e] = acc[e];
       if (lane == 0) ls[wave] = sum;
       __syncthreads();
       if (wave == 0) {
-        sum = ls[0] + ls[1] + ls[2] + ls[3];
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int64_t to = ((int64_t)(q.r0 + row / a.group) * a.hq + head * a.group + row % a.group) * D + E * lane;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float y = (sums[0][lane][e] + sums[1][lane][e] + sums[2][lane][e] + sums[3][lane][e]) * inv;
-          if (a.dtype == kF16) store1<kF16>(a.out, to + e, y);
-          else store1<kBF16>(a.out, to + e, y);
-        }
+        for (int e = 0; e < E; ++e) acc[e] = sums[0][lane][e] + sums[1][lane][e] + sums[2][lane][e] + sums[3][lane][e];
+        store(r, E * lane, acc, ls[0] + ls[1] + ls[2] + ls[3]);
       }
       __syncthreads();
     }
@@ -562,7 +642,7 @@ __global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, i
 }
 
 struct Plan {
-  int groups;        // row groups of 32 a workgroup
+  int waves;         // of a workgroup
   int64_t shares;
   int64_t heads;     // (sequence, head, row tile)s, at most a workgroup's share each
   size_t q, qs, line, begins, cuts, cut, part, stat, bytes;  // parts of the workspace, and its size
@@ -570,15 +650,18 @@ struct Plan {
 
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 
-// `rows`: of a KV head. As few workgroups a KV head as there can be, of as few rows; shares of a workgroup a CU.
+// `rows`: of a KV head. As few workgroups a KV head as there can be, of as few rows; shares of a workgroup a CU, or two of four waves
+// of up to 128 dims.
 Plan plan_of(int d, int64_t rows, int64_t tokens, int hq, int64_t seqs, int heads, int64_t max_len) {
   Plan p;
-  const int64_t units = std::max<int64_t>(1, (rows + 31) / 32), row_tiles = (units + 3) / 4;
-  p.groups = (units + row_tiles - 1) / row_tiles <= 2 ? 2 : 4;
+  const bool pair = d > 128;
+  const int64_t units = std::max<int64_t>(1, (rows + 31) / 32), most = pair ? 4 : 8, row_tiles = (units + most - 1) / most;
+  p.waves = (units + row_tiles - 1) / row_tiles <= most / 2 ? 4 : 8;
+  const int cus = gguf::device_cus() * (!pair && p.waves == 4 ? 2 : 1);
   const int64_t tiles = std::max<int64_t>(1, (max_len + kToks - 1) / kToks);
   // (each factor is capped where the product is beyond every number of workgroups)
   const int64_t work = std::min<int64_t>(seqs * heads, 1 << 20) * std::min<int64_t>(row_tiles, 1 << 20) * std::min<int64_t>(tiles, 1 << 20);
-  p.shares = std::max<int64_t>(1, std::min<int64_t>(gguf::device_cus(), (work + kLeastTiles - 1) / kLeastTiles));
+  p.shares = std::max<int64_t>(1, std::min<int64_t>(cus, (work + kLeastTiles - 1) / kLeastTiles));
   p.q = 0;
   p.qs = p.q + padded((size_t)tokens * hq * 2 * d);
   p.line = p.qs + padded((size_t)tokens * hq * sizeof(float));
@@ -587,29 +670,32 @@ Plan plan_of(int d, int64_t rows, int64_t tokens, int hq, int64_t seqs, int head
   p.cuts = p.begins + padded((size_t)p.shares * sizeof(int));
   p.cut = p.cuts + 256;
   p.part = p.cut + padded((size_t)p.shares * sizeof(Cut));
-  const size_t slots = p.shares == 1 ? 0 : 2 * (size_t)p.shares * 32 * p.groups;
+  const size_t slots = p.shares == 1 ? 0 : 2 * (size_t)p.shares * (pair ? 16 : 32) * p.waves;
   p.stat = p.part + slots * d * sizeof(float);
   p.bytes = p.stat + slots * 2 * sizeof(float);
   return p;
 }
 
-template <int D, int NG>
+template <int D, int NW>
 hipError_t launch(const AttnArgs& a, const Prep& prep, const Plan& p, hipStream_t stream) {
-  using L = Lay<D, NG>;
+  using L = Lay<D, NW>;
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return e;
   struct Tag {};
   gguf::once_per_device<Tag>(dev, [&] {
-    (void)hipFuncSetAttribute((const void*)attend_tree_kernel<D, NG>, hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    (void)hipFuncSetAttribute((const void*)attend_tree_kernel<D, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   });
-  const int64_t rows = ((int64_t)a.rows.tokens * a.hq + 3) / 4;
+  constexpr int per = D == 192 ? 4 : 1024 / D;
+  const int64_t rows = ((int64_t)a.rows.tokens * a.hq + per - 1) / per;
   const unsigned blocks = (unsigned)std::min<int64_t>(rows, 1 << 20) + 1;
   if (a.dtype == kF16) prep_tree_kernel<kF16, D><<<blocks, 256, 0, stream>>>(a, prep, L::kRows, p.shares);
   else prep_tree_kernel<kBF16, D><<<blocks, 256, 0, stream>>>(a, prep, L::kRows, p.shares);
-  attend_tree_kernel<D, NG><<<(unsigned)p.shares, L::kThreads, L::kBytes, stream>>>(a, prep, p.shares);
-  if (p.shares > 1)  // a row a workgroup, or four where there are many
-    join_tree_kernel<D><<<dim3(p.heads <= 32 ? L::kRows : L::kRows / 4, (unsigned)p.heads), 256, 0, stream>>>(a, prep, L::kRows);
+  attend_tree_kernel<D, NW><<<(unsigned)p.shares, L::kThreads, L::kBytes, stream>>>(a, prep, p.shares);
+  if (p.shares > 1) {  // some thousand workgroups, of a row or more
+    const int64_t each = std::min<int64_t>(L::kRows, std::max<int64_t>(L::kRows / 16, 4096 / p.heads));
+    join_tree_kernel<D><<<dim3((unsigned)each, (unsigned)p.heads), 256, 0, stream>>>(a, prep, L::kRows);
+  }
   return hipGetLastError();
 }
 
@@ -622,11 +708,17 @@ size_t tree_workspace(int d, int64_t rows, int64_t tokens, int hq, int64_t seqs,
 hipError_t launch_attend_tree(AttnArgs a, int64_t rows, int64_t max_len, void* ws, hipStream_t stream) {
   const Plan p = plan_of(a.c.d, rows, a.rows.tokens, a.hq, a.rows.seqs, a.c.heads, max_len);
   char* w = (char*)ws;
-  const Prep prep{(int8_t*)w, (float*)(w + p.qs), (int64_t*)(w + p.line), (int*)(w + p.begins), (int*)(w + p.cuts), (Cut*)(w + p.cut)};
+  const Prep prep{(_Float16*)w, (float*)(w + p.qs), (int64_t*)(w + p.line), (int*)(w + p.begins), (int*)(w + p.cuts), (Cut*)(w + p.cut)};
   a.part = (float*)(w + p.part);
   a.stat = (float*)(w + p.stat);
-  if (a.c.d == 192) return p.groups == 2 ? launch<192, 2>(a, prep, p, stream) : launch<192, 4>(a, prep, p, stream);
-  return p.groups == 2 ? launch<256, 2>(a, prep, p, stream) : launch<256, 4>(a, prep, p, stream);
+#define GGUF_DEC_TREE(D) return p.waves == 4 ? launch<D, 4>(a, prep, p, stream) : launch<D, 8>(a, prep, p, stream);
+  switch (a.c.d) {
+    case 64: GGUF_DEC_TREE(64)
+    case 128: GGUF_DEC_TREE(128)
+    case 192: GGUF_DEC_TREE(192)
+    default: GGUF_DEC_TREE(256)
+  }
+#undef GGUF_DEC_TREE
 }
 
 }  // namespace gguf_dec
