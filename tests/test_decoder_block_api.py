@@ -236,3 +236,15 @@ def test_tree_workspaces():
         for hint in (2 ** 62, 2 ** 63 - 1):
             assert bytes_of(hint, 6) == bytes_of(tokens, 6)
             assert 0 < bytes_of(hint, hint) == bytes_of(tokens, 2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("size", [(3, (1 << 30) + 1), (1 << 31, 8), (3, 1 << 40, 8), (1 << 40, 1 << 40, 8)], ids=str)
+def test_norms_of_too_many_values(size):
+    """A C caller's sizes beyond what an index holds."""
+    lib = ctypes.CDLL(decoder.LIB_PATH)
+    lib.gguf_decoder_last_error.restype = ctypes.c_char_p
+    x = _desc(torch.zeros(3, 8) if len(size) == 2 else torch.zeros(3, 3, 8))
+    x.size[:len(size)] = list(size)
+    null = ctypes.c_void_p(None)
+    assert lib.gguf_residual_norm(ctypes.byref(x), null, null, 0, null, null, ctypes.c_float(1), ctypes.c_float(0), ctypes.byref(x), null, null) == 1
+    assert "too many" in lib.gguf_decoder_last_error().decode()

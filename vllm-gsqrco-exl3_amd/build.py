@@ -10,7 +10,8 @@ vllm_gguf_plugin/_C_gguf_ops.so, which links libgguf_mi355x.so next to it and re
 torch.ops._C_gguf when vllm_gguf_plugin._C_gguf loads it. csrc/bench/peaks.hip (bench.py's
 measurement kernels, outside the C ABI) is built into vllm_gguf_plugin/libgguf_peaks.so.
 
-csrc/decoder/*.hip (attention over the 8-bit cache, the gated delta rule, log probabilities) become
+csrc/decoder/*.hip (rotation into the 8-bit cache, attention over it and kept paths of drafts, block norms, the gated
+delta rule, log probabilities) become
 vllm_gguf_plugin/libgguf_decoder.so, the C ABI of include/gguf_decoder.h, and csrc/decoder/torch_ops.cpp
 its registration _C_gguf_decoder_ops.so, which vllm_gguf_plugin.decoder loads.
 """
