@@ -238,7 +238,7 @@ def test_tree_workspaces():
             assert 0 < bytes_of(hint, hint) == bytes_of(tokens, 2 ** 31 - 1)
 
 
-@pytest.mark.parametrize("size", [(3, (1 << 30) + 1), (1 << 31, 8), (3, 1 << 40, 8), (1 << 40, 1 << 40, 8)], ids=str)
+@pytest.mark.parametrize("size", [(3, (1 << 30) + 1), (3, 2, (1 << 31) - 1), (1 << 20, 1 << 20, 8), ((1 << 31) - 1, 2, 8)], ids=str)
 def test_norms_of_too_many_values(size):
     """A C caller's sizes beyond what an index holds."""
     lib = ctypes.CDLL(decoder.LIB_PATH)

@@ -409,7 +409,7 @@ int gguf_residual_norm(const gguf_tensor* x, const gguf_tensor* residual, const 
   if (!shaped(x, nd) || !is_float(x->dtype)) return fail("%s: x must be a float [rows, n] or [rows, heads, n]", op);
   const int64_t n = x->size[nd - 1], heads = nd == 3 ? x->size[1] : 1;
   if (n < 1 || heads < 1) return fail("%s: x has no columns", op);
-  if (n > (1 << 30) || heads > INT_MAX || x->size[0] > INT_MAX / heads) return fail("%s: x has too many rows or columns", op);
+  if (n > (1 << 30) || x->size[0] > INT_MAX / heads) return fail("%s: x has too many rows or columns", op);
   const int64_t rows = x->size[0] * heads;
   const auto like = [&](const gguf_tensor* t) {
     if (!shaped(t, nd)) return false;
