@@ -5,8 +5,8 @@
 // dims of a piece, or that hold whole pairs. So a row's lanes need each other for the norm's sum only.
 //
 // What bounds it: a step of single tokens the chain lens -> table -> page -> codes (32 sequences, 24 + 4 heads of 256 dims in
-// bf16: 7.2 us a call in a graph, kv8_append alone 5.4); a prompt the memory (8192 tokens of 24 + 4 heads of 256: 256 MB read and
-// written in 55 us, 4.7 TB/s, what a copy reaches).
+// bf16: 7.2 us a call in a graph, kv8_append alone 5.4); a prompt the memory (8192 tokens of 24 + 4 heads of 256: 252 MB read and
+// written in 71 us, 3.6 TB/s, a copy reaches 5; in a loop, where the last level of cache holds a part, in 55). Times of that loop:
 // - The two passes over a page's new values, for the scale and for the codes, run forwards and backwards, so that the last rows
 //   are at hand for the second: of a page of 64 tokens of 256 dims half of K's and all of V's are read once. Holding all of K's
 //   costs registers that spill (2 x 2 pieces: 69 us the prompt, 10.0 us the step).
