@@ -40,6 +40,7 @@ constexpr int kVRow = 2 * kToks + 16;    // bytes of a dim's row of V in LDS; 16
 constexpr int kAhead = 16;               // tiles whose chunks are looked up at a time
 constexpr int kPlaces = 4 * 2 * kAhead;  // places of chunks that are held: those of tile t at 4 (t % (2 kAhead))
 constexpr int kLeastTiles = 4;           // of a workgroup's share
+constexpr int kParts = 32;               // of a group that is cut, for a wave
 
 // v, made again where it is needed: what comes of a thread's number (its places in LDS and memory) would otherwise be kept over the
 // tiles, in registers that the products need
@@ -54,10 +55,12 @@ struct Place {
   float ks, vs;
 };
 
-// A group of tiles that lies in several shares, from share `first` on (it begins there) to `last`.
+// A group of tiles that lies in several shares, from share `first` on (it begins there) to `last`, and what its rows are.
 struct Cut {
-  int seq, first, last, own;  // own: it is the first of share `first`
-  int64_t group;              // among its sequence's
+  int first, last, own;  // own: it is the first of share `first`
+  int head, r0;          // KV head; the sequence's first token
+  int64_t row0;          // the group's first row among the sequence's of the head
+  int rows;
 };
 
 // Queries as the products take them, and the line of all tiles, cut: what prep_tree_kernel leaves.
@@ -128,7 +131,7 @@ __device__ __forceinline__ uint64_t seen_of(const Words& w, int at, int base, in
 // How the line of all tiles is cut: share w of `shares` is [w total / shares, (w + 1) total / shares).
 struct Line {
   int64_t total, shares;
-  __device__ Line(const AttnArgs& a, const Prep& p, int64_t most) : total(p.line[a.rows.seqs]) {
+  __device__ Line(int64_t all, int64_t most) : total(all) {
     shares = min(most, max((total + kLeastTiles - 1) / kLeastTiles, (int64_t)1));
   }
   __device__ int64_t begin(int64_t w) const { return w * total / shares; }
@@ -140,7 +143,8 @@ template <int DT, int D>
 __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int rows, int64_t most) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (blockIdx.x == 0) {
-    __shared__ int64_t part[4];
+    constexpr int HELD = 1024;  // sequences whose line is looked up in LDS
+    __shared__ int64_t part[4], held[HELD];
     int64_t total = 0;
     for (int s0 = 0; s0 < a.rows.seqs; s0 += 256) {
       const int s = s0 + tid;
@@ -165,26 +169,30 @@ __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int 
         total += part[w];
       }
       if (s < a.rows.seqs) p.line[s] = before + x - cost;
+      if (s < HELD) held[s] = before + x - cost;
     }
     if (tid == 0) p.line[a.rows.seqs] = total, *p.cuts = 0;
     __syncthreads();
-    const Line line(a, p, most);
+    const Line line(total, most);
+    const bool all_held = a.rows.seqs <= HELD;
     for (int64_t w = tid; w < line.shares && total > 0; w += 256) {
       const int64_t at = line.begin(w);
       int s = 0;  // the last sequence with line[s] <= at: one that has tiles
       for (int lo = 0, hi = a.rows.seqs - 1; lo <= hi;) {
         const int mid = lo + (hi - lo) / 2;
-        if (p.line[mid] <= at) s = mid, lo = mid + 1;
+        if ((all_held ? held[mid] : p.line[mid]) <= at) s = mid, lo = mid + 1;
         else hi = mid - 1;
       }
       p.begins[w] = s;
       if (w == 0) continue;
-      const int tiles = seq_of(a, s, rows).tiles;
-      const int64_t group = (at - p.line[s]) / tiles, lo = p.line[s] + group * tiles, hi = lo + tiles;
+      const Seq q = seq_of(a, s, rows);
+      const int64_t from = all_held ? held[s] : p.line[s], group = (at - from) / q.tiles, lo = from + group * q.tiles, hi = lo + q.tiles;
       if (at == lo || line.begin(w - 1) > lo) continue;  // it begins with the group, or an earlier share's begin lies inside it
       int64_t last = w;
       while (line.begin(last + 1) < hi) ++last;
-      p.cut[atomicAdd(p.cuts, 1)] = Cut{s, (int)w - 1, (int)last, line.begin(w - 1) == lo, group};
+      const int64_t row0 = group % q.row_tiles * rows;
+      p.cut[atomicAdd(p.cuts, 1)] = Cut{(int)w - 1, (int)last, line.begin(w - 1) == lo, (int)(group / q.row_tiles), q.r0, row0,
+                                        (int)min((int64_t)rows, (int64_t)q.n * a.group - row0)};
     }
     return;
   }
@@ -237,7 +245,7 @@ attend_tree_kernel(AttnArgs a, Prep prep, int64_t most) {
   const bool brings_v = wave < FIRST / 64, late = LAG && !brings_v;
   const int room = (int)min((int64_t)a.c.max_pages * a.c.page, (int64_t)INT32_MAX);
 
-  const Line line(a, prep, most);
+  const Line line(prep.line[a.rows.seqs], most);
   if ((int64_t)blockIdx.x >= line.shares || line.total == 0) return;
   const int64_t begin = line.begin(blockIdx.x), end = line.begin((int64_t)blockIdx.x + 1);
   int seq = prep.begins[blockIdx.x];
@@ -559,59 +567,65 @@ attend_tree_kernel(AttnArgs a, Prep prep, int64_t most) {
   }
 }
 
-// Joins the rows of the groups that are cut. Of few parts a wave takes some rows at a time, all loads under way at once; of many a
-// workgroup takes a row, its waves the parts in turn.
+// Joins the rows of the groups that are cut. Of up to kParts parts a wave takes some rows at a time, AT parts' loads under way at once; of
+// more a workgroup takes a row, its waves the parts in turn.
 template <int D>
-__global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, int rows) {
-  constexpr int E = D / 64, FEW = 4;
+__global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, int rows, int most) {
+  constexpr int E = D / 64, AT = 4;
   __shared__ float sums[4][64][E];
   __shared__ float ls[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int cuts = *prep.cuts;
-  for (int i = blockIdx.y; i < cuts; i += gridDim.y) {
-    const Cut cut = prep.cut[i];
-    const Seq q = seq_of(a, cut.seq, rows);
-    const int head = (int)(cut.group / q.row_tiles), rt = (int)(cut.group - (int64_t)head * q.row_tiles);
-    const int64_t nrows = min((int64_t)rows, (int64_t)q.n * a.group - (int64_t)rt * rows);
+  for (int i = blockIdx.y; i < most; i += gridDim.y) {
+    const Cut cut = prep.cut[i];  // fetched beside their number
+    if (i >= cuts) break;
     const auto slot = [&](int w, int64_t r) { return (2 * (int64_t)w + (w == cut.first && !cut.own)) * rows + r; };
     const auto store = [&](int64_t r, int at, auto& v, float sum) __attribute__((always_inline)) {
-      const int64_t row = (int64_t)rt * rows + r;
+      const int64_t row = cut.row0 + r;
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int64_t to = ((int64_t)(q.r0 + row / a.group) * a.hq + head * a.group + row % a.group) * D + at;
+      const int64_t to = ((int64_t)(cut.r0 + row / a.group) * a.hq + cut.head * a.group + row % a.group) * D + at;
 #pragma unroll
       for (int e = 0; e < (int)(sizeof(v) / 4); ++e) {
         if (a.dtype == kF16) store1<kF16>(a.out, to + e, v[e] * inv);
         else store1<kBF16>(a.out, to + e, v[e] * inv);
       }
     };
-    if (cut.last - cut.first < FEW) {  // uniform
+    if (cut.last - cut.first < kParts) {  // uniform
       constexpr int L = D == 192 ? 64 : D / 4;  // lanes of a row, four dims each (of 192 some do another's over)
       const int at = min(4 * (lane % L), D - 4);
-      for (int64_t r = ((int64_t)blockIdx.x * 4 + wave) * (64 / L) + lane / L; r < nrows; r += (int64_t)gridDim.x * (256 / L)) {
-        float2 ml[FEW];
-        floatx4 v[FEW];
+      for (int64_t r = ((int64_t)blockIdx.x * 4 + wave) * (64 / L) + lane / L; r < cut.rows; r += (int64_t)gridDim.x * (256 / L)) {
+        float mx = kNoScore, sum = 0.0f, acc[4] = {};
+        for (int w0 = cut.first; w0 <= cut.last; w0 += AT) {
+          float2 ml[AT];
+          floatx4 v[AT];
 #pragma unroll
-        for (int j = 0; j < FEW; ++j) {
-          const bool ok = cut.first + j <= cut.last;
-          const int64_t from = slot(ok ? cut.first + j : cut.first, r);
-          ml[j] = ok ? *(const float2*)(a.stat + from * 2) : make_float2(kNoScore, 0.0f);
-          v[j] = ok ? *(const floatx4*)(a.part + from * D + at) : floatx4{0, 0, 0, 0};
-        }
-        float mx = ml[0].x, sum = 0.0f, acc[4] = {};
+          for (int j = 0; j < AT; ++j) {
+            const bool ok = w0 + j <= cut.last;
+            const int64_t from = slot(ok ? w0 + j : w0, r);
+            ml[j] = ok ? *(const float2*)(a.stat + from * 2) : make_float2(kNoScore, 0.0f);
+            v[j] = ok ? *(const floatx4*)(a.part + from * D + at) : floatx4{0, 0, 0, 0};
+          }
+          float nm = mx;
 #pragma unroll
-        for (int j = 1; j < FEW; ++j) mx = fmaxf(mx, ml[j].x);
+          for (int j = 0; j < AT; ++j) nm = fmaxf(nm, ml[j].x);
+          const float al = __builtin_amdgcn_exp2f(mx - nm);
+          mx = nm;
+          sum *= al;
 #pragma unroll
-        for (int j = 0; j < FEW; ++j) {
-          const float f = __builtin_amdgcn_exp2f(ml[j].x - mx);
-          sum += ml[j].y * f;
+          for (int e = 0; e < 4; ++e) acc[e] *= al;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += v[j][e] * f;
+          for (int j = 0; j < AT; ++j) {
+            const float f = __builtin_amdgcn_exp2f(ml[j].x - mx);
+            sum += ml[j].y * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += v[j][e] * f;
+          }
         }
         store(r, at, acc, sum);
       }
       continue;
     }
-    for (int64_t r = blockIdx.x; r < nrows; r += gridDim.x) {
+    for (int64_t r = blockIdx.x; r < cut.rows; r += gridDim.x) {
       float mx = kNoScore;
       for (int w = cut.first + lane; w <= cut.last; w += 64) mx = fmaxf(mx, a.stat[slot(w, r) * 2]);
 #pragma unroll
@@ -694,7 +708,7 @@ hipError_t launch(const AttnArgs& a, const Prep& prep, const Plan& p, hipStream_
   attend_tree_kernel<D, NW><<<(unsigned)p.shares, L::kThreads, L::kBytes, stream>>>(a, prep, p.shares);
   if (p.shares > 1) {  // some thousand workgroups, of a row or more
     const int64_t each = std::min<int64_t>(L::kRows, std::max<int64_t>(L::kRows / 16, 4096 / p.heads));
-    join_tree_kernel<D><<<dim3((unsigned)each, (unsigned)p.heads), 256, 0, stream>>>(a, prep, L::kRows);
+    join_tree_kernel<D><<<dim3((unsigned)each, (unsigned)p.heads), 256, 0, stream>>>(a, prep, L::kRows, (int)p.shares);
   }
   return hipGetLastError();
 }
