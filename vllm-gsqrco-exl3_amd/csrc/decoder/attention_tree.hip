@@ -22,7 +22,7 @@
 //
 // What bounds it: a step takes some 2100 to 2500 cycles, the products' 32 matrix instructions 1024 of them on a SIMD; the weights' 270 to
 // 300 vector instructions, 16 or 32 of them exponentials, with their waits for LDS and each other the rest. 16 drafts of 8 ragged sequences
-// to 32768 tokens (24 query and 4 KV heads of 256): 104 us, 47 drafts of 4 to 16000: 88, 64 drafts of 32 to 8192 (32 query and 8 KV heads
+// to 32768 tokens (24 query and 4 KV heads of 256): 103 us, 47 drafts of 4 to 16000: 85, 64 drafts of 32 to 8192 (32 query and 8 KV heads
 // of 128): 222; the products alone 28, 20 and 88 at a library product's rate.
 #include <algorithm>
 #include <type_traits>
@@ -567,7 +567,7 @@ attend_tree_kernel(AttnArgs a, Prep prep, int64_t most) {
   }
 }
 
-// Joins the rows of the groups that are cut. Of up to kParts parts a wave takes some rows at a time, AT parts' loads under way at once; of
+// Joins the rows of the groups that are cut: of the cases above 32 and 67 MB of sums, 10 and 13 us. Of up to kParts parts a wave takes some rows at a time, AT parts' loads under way at once; of
 // more a workgroup takes a row, its waves the parts in turn.
 template <int D>
 __global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, int rows, int most) {
