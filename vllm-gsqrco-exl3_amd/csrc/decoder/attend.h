@@ -65,40 +65,22 @@ struct Chunk {
   float ks, vs;
 };
 
-// Where chunk ch of a sequence lies in its table: page and first token. One past position `see` is not seen.
-struct Spot {
-  bool seen;
-  int pi, off;
-};
-
-__device__ __forceinline__ Spot spot_of(int page16, int64_t ch, int see) {
-  Spot s;
-  s.seen = see >= 0 && ch <= see / 16;
-  s.pi = s.seen ? (int)ch / page16 : 0;
-  s.off = s.seen ? ((int)ch - s.pi * page16) * 16 : 0;
-  return s;
-}
-
-// (page, head) of a spot whose table says page pid: always one of the cache's
-__device__ __forceinline__ int place_of(const Kv8& c, const Spot& s, int pid, int head) {
-  return (s.seen && pid >= 0 && pid < c.pages ? pid : 0) * c.heads + head;
-}
-
-// The chunk, from the scales at its place. One that is not seen has scales of 0; a page out of range reads as NaN, and a V scale
-// that is not finite is NaN for the rows that see it and no measure for the others.
-__device__ __forceinline__ Chunk chunk_at(const Kv8& c, const Spot& s, int pid, int head, float ks, float vs) {
-  const bool ok = s.seen && pid >= 0 && pid < c.pages;
-  const float none = s.seen ? __builtin_nanf("") : 0.0f;
-  Chunk r{place_of(c, s, pid, head), s.off, ok ? ks : none, ok ? vs : none};
+// Chunk ch of a sequence. One past position `see` has scales of 0; a page out of range reads as NaN, and a V scale
+// that is not finite is NaN for the rows that see it and no measure for the others. ph is always a page's.
+__device__ __forceinline__ Chunk chunk_of(const Kv8& c, const int32_t* table, int page16, int head, int64_t ch, int see) {
+  const bool seen = see >= 0 && ch <= see / 16;
+  const int pi = seen ? (int)ch / page16 : 0;
+  const int pid = table[pi];
+  const bool ok = seen && pid >= 0 && pid < c.pages;
+  Chunk r;
+  r.ph = (ok ? pid : 0) * c.heads + head;
+  r.off = seen ? ((int)ch - pi * page16) * 16 : 0;
+  const float none = seen ? __builtin_nanf("") : 0.0f;
+  r.ks = ok ? c.ks[r.ph] : none;
+  r.vs = ok ? c.vs[r.ph] : none;
   if (!(r.vs <= 3.0e38f)) r.vs = __builtin_nanf("");
   if (fabsf(r.vs) < kLeastScale) r.vs = 0.0f;
   return r;
-}
-
-__device__ __forceinline__ Chunk chunk_of(const Kv8& c, const int32_t* table, int page16, int head, int64_t ch, int see) {
-  const Spot s = spot_of(page16, ch, see);
-  const int pid = table[s.pi], at = place_of(c, s, pid, head);
-  return chunk_at(c, s, pid, head, c.ks[at], c.vs[at]);
 }
 
 // max over lanes l and l ^ 32

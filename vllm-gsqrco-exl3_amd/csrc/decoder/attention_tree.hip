@@ -567,8 +567,9 @@ attend_tree_kernel(AttnArgs a, Prep prep, int64_t most) {
   }
 }
 
-// Joins the rows of the groups that are cut: of the cases above 32 and 67 MB of sums, 10 and 13 us. Of up to kParts parts a wave takes some rows at a time, AT parts' loads under way at once; of
-// more a workgroup takes a row, its waves the parts in turn.
+// Joins the rows of the groups that are cut. Of up to kParts parts a wave takes some rows at a time, AT parts' loads under way at once; of
+// more a workgroup takes a row, its waves the parts in turn. Bound by memory: two groups' sums a share at most, some 30 MB of the first
+// case above and 60 of the last, in 10 and 13 us.
 template <int D>
 __global__ void __launch_bounds__(256) join_tree_kernel(AttnArgs a, Prep prep, int rows, int most) {
   constexpr int E = D / 64, AT = 4;
