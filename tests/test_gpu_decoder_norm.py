@@ -125,6 +125,20 @@ def test_many_long_rows(dec, n):
     _run(dec, (1030, n), BF16, F32, 9, True, True, "sigmoid", True, 0.5)
 
 
+@pytest.mark.parametrize("dtype,rdtype", [(BF16, F32), (F16, F16), (F32, F32)], ids=str)
+@pytest.mark.parametrize("n", [63, 65, 127, 1023, 1025, 4095, 8191, 8193])
+def test_odd_lengths(dec, n, dtype, rdtype):
+    """Rows of single values, a workgroup each, around what its threads hold; a part of a batch gives the batch's bits."""
+    _run(dec, (3, n), dtype, rdtype, 10, True, True, "silu", True, 0.5)
+    _run(dec, (2, 3, n), dtype, dtype, 11, True, False, "sigmoid", False)
+    g = torch.Generator().manual_seed(12)
+    x, r, w = torch.randn(300, n, generator=g).to(dtype).cuda(), torch.randn(300, n, generator=g).to(rdtype).cuda(), torch.randn(n, generator=g).cuda()
+    a, b = dec.residual_norm(x, r, w, inner_weight=w)
+    for lo, hi in ((0, 1), (100, 117), (299, 300)):
+        c, d = dec.residual_norm(x[lo:hi], r[lo:hi], w, inner_weight=w)
+        assert torch.equal(c, a[lo:hi]) and torch.equal(d, b[lo:hi])
+
+
 def test_broadcast_gate_and_residual(dec):
     """Strides of 0: one gate, one residual row for all rows."""
     g = torch.Generator().manual_seed(7)
