@@ -65,7 +65,7 @@ struct Cut {
 
 // Queries as the products take them, and the line of all tiles, cut: what prep_tree_kernel leaves.
 struct Prep {
-  _Float16* q;     // [tokens * hq][d]: times a power of two that brings the row's largest to 1 .. 2, and the call's scale's sign
+  _Float16* q;     // [tokens * hq][d]: bf16 times a power of two that brings the row's largest to 1 .. 2; and the call's scale's sign
   float* qs;       // [tokens * hq]: what they are multiplied by, with the call's scale
   int64_t* line;   // [seqs + 1]: tiles before a sequence's
   int* begins;     // [shares]: the sequence in which a share begins
@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int 
     }
 #pragma unroll
     for (int off = 1; off < L; off <<= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off, 64));
-    const float amax = __uint_as_float(big), by = row_factor(amax), to = a.scale < 0.0f ? -by : by;
+    // fp16 queries as they are: scaled, elements 2^-15 of the row's largest would become subnormal and lose bits
+    const float amax = __uint_as_float(big), by = DT == kBF16 ? row_factor(amax) : 1.0f, to = a.scale < 0.0f ? -by : by;
     *(uint2*)(p.q + r * D + at) = make_uint2(pack2<kF16>(v[0] * to, v[1] * to), pack2<kF16>(v[2] * to, v[3] * to));
     // not negative: the scale's sign is the queries'
     if (tid % L == 0) p.qs[r] = amax < __builtin_inff() ? fabsf(a.scale) / by : __builtin_nanf("");
