@@ -15,11 +15,28 @@ namespace gguf_dec {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.9259629911e-8f, kLn2 = 0.6931471805599453f;
 
+// Where h is rounded to 8 or 11 bits: by the hardware's 2^x of an argument rounded to fp32, off by up to 2^-24 of the argument (2^-17 of the
+// result), and 0 where e^-g passes fp32 (g below -88). Where h is fp32: sigmoid(g) = t^[g < 0] / (1 + t), t = e^-|g|, to some steps of
+// fp32 and down to its least number. What rounding the argument left, lo, goes into t = 2^hi (1 + lo ln 2); and as the hardware's 2^x has no
+// subnormal results, below 2^-100 (where 1 + t is 1) it is taken of hi + 64, and 2^-64 multiplied in last. For all types that would take
+// 8192 x 48 heads of 128 from 61 to 72 us in bf16; in fp32 they take 104 instead of 103, 8192 rows of 4097 values 164 instead of 152.
+template <int RT>
 __device__ __forceinline__ float act_of(float g, int act) {
-  const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));  // of -inf: 1 / inf
-  return act == kActSilu ? g * s : act == kActSigmoid ? s : g;
+#pragma clang fp contract(off)  // hi + 64 is of the rounded hi
+  if constexpr (RT != kF32) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));  // of -inf: 1 / inf
+    return act == kActSilu ? g * s : act == kActSigmoid ? s : g;
+  }
+  const float a = fabsf(g) > 200.0f ? 200.0f : fabsf(g);  // e^-200 is 0; a NaN stays
+  const float hi = -a * kLog2e, lo = __builtin_fmaf(-a, kLog2eRest, __builtin_fmaf(-a, kLog2e, -hi));
+  const bool least = g < 0.0f && hi < -100.0f;
+  const float e = __builtin_amdgcn_exp2f(least ? hi + 64.0f : hi);
+  const float t = __builtin_fmaf(e, lo * kLn2, e);
+  const float x = act == kActSilu ? g : 1.0f;
+  const float y = (g < 0.0f ? x * t : x) * (least ? 0x1p-64f : __builtin_amdgcn_rcpf(1.0f + t));
+  return act == kActNone ? g : y;
 }
 
 // Sum over the row's lanes (a power of two up to 64, aligned) or over the workgroup, of whose waves each holds ITEMS parts. Each
@@ -131,7 +148,7 @@ __global__ void __launch_bounds__(WG ? 1024 : 256) norm_kernel(NormArgs a, int l
       if constexpr (!HELD) gate(c, g[0]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (a.gate) u[i][e] *= act_of(g[HELD ? i : 0][e], a.act);
+        if (a.gate) u[i][e] *= act_of<RT>(g[HELD ? i : 0][e], a.act);
         h[i][e] += a.scale * u[i][e];
         if (c < a.n) sum[i] += h[i][e] * h[i][e];
       }
@@ -186,10 +203,13 @@ __global__ void __launch_bounds__(1024) norm_odd_kernel(NormArgs a) {
       }
     }
     sum[0] = 0.0f;
+    if (a.gate) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) u[i] *= act_of<RT>(g[i], a.act);
+    }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
-      if (a.gate) u[i] *= act_of(g[i], a.act);
       h[i] += a.scale * u[i];
       if (c < a.n) {
         sum[0] += h[i] * h[i];
@@ -231,7 +251,7 @@ __global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
     const auto hidden = [&](int c) __attribute__((always_inline)) {
       float u = load1<DT>(a.x, xa + c);
       if (a.inner) u *= by * a.inner[c];
-      if (a.gate) u *= act_of(load1<DT>(a.gate, ga + c), a.act);
+      if (a.gate) u *= act_of<RT>(load1<DT>(a.gate, ga + c), a.act);
       return (a.residual ? load1<RT>(a.residual, ra + c) : 0.0f) + a.scale * u;
     };
     sum[0] = 0.0f;
