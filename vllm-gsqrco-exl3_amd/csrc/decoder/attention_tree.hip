@@ -188,8 +188,7 @@ __global__ void __launch_bounds__(256) prep_tree_kernel(AttnArgs a, Prep p, int 
       const Seq q = seq_of(a, s, rows);
       const int64_t from = all_held ? held[s] : p.line[s], group = (at - from) / q.tiles, lo = from + group * q.tiles, hi = lo + q.tiles;
       if (at == lo || line.begin(w - 1) > lo) continue;  // it begins with the group, or an earlier share's begin lies inside it
-      int64_t last = w;
-      while (line.begin(last + 1) < hi) ++last;
+      const int64_t last = (hi * line.shares + line.total - 1) / line.total - 1;  // the last share that begins before hi
       const int64_t row0 = group % q.row_tiles * rows;
       p.cut[atomicAdd(p.cuts, 1)] = Cut{(int)w - 1, (int)last, line.begin(w - 1) == lo, (int)(group / q.row_tiles), q.r0, row0,
                                         (int)min((int64_t)rows, (int64_t)q.n * a.group - row0)};
