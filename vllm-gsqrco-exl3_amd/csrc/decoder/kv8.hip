@@ -63,28 +63,22 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Kv8 c, const void* __r
     for (int w = 0; w < kThreads / 64; ++w) big = max(big, most[w]);
 
     float* scale = (is_v ? c.vs : c.ks) + (int64_t)pid * c.heads + head;
-    float fresh = __uint_as_float(big) / 127.0f;
-    if (fresh < kLeastScale) fresh = 0.0f;
-    const float was = older > 0 ? *scale : 0.0f;
-    const float now = fresh <= was ? was : fresh;  // a NaN on either side is kept: fresh's here, was's as was > 0 fails
-    const float s = was != was ? was : now;
-    const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-    const bool shrink = older > 0 && !(s == was);
-    const float ratio = shrink ? was / s : 1.0f;
+    const Rescale s = rescale_of(older > 0 ? *scale : 0.0f, __uint_as_float(big));
+    const bool shrink = older > 0 && s.shrink;
     __syncthreads();  // every thread has read the old scale
-    if (tid == 0) *scale = s;
+    if (tid == 0) *scale = s.scale;
 
     int8_t* codes = (is_v ? c.v : c.k) + ((int64_t)pid * c.heads + head) * page * d;
     if (!is_v) {
       if (shrink)
-        for (int i = tid; i < older * d / 4; i += kThreads) ((uint32_t*)codes)[i] = rescale4(((uint32_t*)codes)[i], ratio);
+        for (int i = tid; i < older * d / 4; i += kThreads) ((uint32_t*)codes)[i] = rescale4(((uint32_t*)codes)[i], s.ratio);
       for (int i = tid; i < (hi - lo) * per; i += kThreads) {
         const int t = lo + i / per, at = 8 * (i % per);
         float v[8];
         load8<DT>(x, (row0 + t) * st + base + at, v);
         uint32_t w[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(code_of(v[e] * inv) & 0xFF) << 8 * (e & 3);
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(code_of(v[e] * s.inv) & 0xFF) << 8 * (e & 3);
         *(uint2*)(codes + (int64_t)t * d + at) = make_uint2(w[0], w[1]);
       }
     } else {
@@ -110,7 +104,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Kv8 c, const void* __r
           if (is_new || is_old) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float y = is_new ? v[e] * inv : (float)(int8_t)(w[e][t >> 2] >> 8 * (t & 3)) * ratio;
+              const float y = is_new ? v[e] * s.inv : (float)(int8_t)(w[e][t >> 2] >> 8 * (t & 3)) * s.ratio;
               w[e][t >> 2] = (w[e][t >> 2] & ~(0xFFu << 8 * (t & 3))) | (uint32_t)(code_of(y) & 0xFF) << 8 * (t & 3);
             }
           }
