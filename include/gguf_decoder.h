@@ -108,7 +108,7 @@ GGUF_DEC_API int gguf_kv8_read(const gguf_kv8_cache* cache, const gguf_tensor* b
  * cache split over workgroups; with fewer bytes than gguf_kv8_attention_workspace_bytes (0 included) the
  * call is split less. max_new, max_len: the largest n_s and seq_lens[s], hints.
  * Precision: sums and the softmax's statistics are fp32. A weight times its page's V scale enters the second product
- * in fp16: to 2^-12 of itself down to 2^-21 of the row's largest weight times the largest V scale that the row sees, below
+ * in fp16: to 2^-11 of itself down to 2^-21 of the row's largest weight times the largest V scale that the row sees, below
  * that to 2^-32 of these. Queries: where max_new * q_heads / heads is at most 64, exact but for bf16 elements below 2^-14
  * of the row's largest; above, integers of 15 bits, to 2^-15 of the row's largest magnitude (0 where that is below 2^-100).
  * A query row with an infinity or a NaN is NaN. */

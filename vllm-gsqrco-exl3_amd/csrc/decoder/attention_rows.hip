@@ -9,7 +9,7 @@
 //
 // K stays in 8 bits: the first product is int8, with Q as 15-bit integers q = s (128 hi + lo), s the row's
 // largest magnitude / 16256, in two products whose int32 sums are exact (128 * 127 * 127 * 256 < 2^30). What rounding Q
-// changes of a score is below 2^-15 of the largest |q| times |k|, where the weights are rounded to fp16 (2^-12)
+// changes of a score is below 2^-15 of the largest |q| times |k|, where the weights are rounded to fp16 (2^-11)
 // and outputs to 8 or 11 bits. Beside two fp16 steps this halves what the waves read of K from LDS, which bounds the kernel
 // next to the matrix cores, and K needs no conversion.
 // V is converted to fp16 once a workgroup, from registers to LDS.
