@@ -128,7 +128,7 @@ GGUF_DEC_API int gguf_kv8_attention(const gguf_tensor* query, const gguf_kv8_cac
  * with c and s at cos_sin[positions[token], i] and [.., r / 2 + i] (i' where interleaved). cos_sin: fp32 [positions, r], r a
  * multiple of 16 up to d (dims from r on do not turn), unit inner stride, rows 16-byte aligned; positions: int64 [tokens],
  * where a tree of drafts has its depths. A position out of the table's range turns by NaN. Everything is fp32; query_out (contiguous, 16-byte
- * aligned, like query) is rounded once, a key is rounded to its code only. All rows of query are turned,
+ * aligned, like query) is rounded once, a key is rounded to its code only. Squares are summed as in gguf_residual_norm. All rows of query are turned,
  * those of no sequence too. Keys and values enter the cache as by gguf_kv8_append. */
 GGUF_DEC_API int gguf_kv8_rotary_append(const gguf_kv8_cache* cache, const gguf_tensor* query, const gguf_tensor* key,
                                         const gguf_tensor* value, const gguf_tensor* cos_sin, const gguf_tensor* positions,
@@ -162,11 +162,11 @@ GGUF_DEC_API int gguf_kv8_keep(const gguf_kv8_cache* cache, const gguf_tensor* p
  * (fp32 / fp16 / bf16 [rows, n] or [rows, heads, n], unit inner stride; any other strides, 0 included). Each part may be NULL:
  *   u = x;   u = u / sqrt(mean(u^2) + eps) * inner_weight;   u = u * act(gate);   h = residual + scale * u
  *   out = h / sqrt(mean(h^2) + eps) * weight
- * act: 0 the gate itself, 1 its sigmoid, 2 silu. gate: like x (other strides); residual: x's shape, x's dtype or fp32; weights: fp32 [n].
- * hidden (h): contiguous, residual's dtype (x's without one); out: contiguous, x's dtype, not read or written without weight. Neither
+ * act: 0 the gate itself, 1 its sigmoid, 2 silu; without a gate it is not looked at. gate: like x (other strides); residual: x's shape, x's dtype or fp32; weights: fp32 [n].
+ * hidden (h): contiguous, residual's dtype (x's without one), written by every call; out: contiguous, x's dtype, not read or written without weight. Neither
  * overlaps an input. Everything between is fp32: out comes from h before its rounding. Where hidden is not fp32, a sigmoid is
  * known to 2^-17 of itself and is 0 for gates below -88; where it is, to some steps of fp32. Squares are summed in fp32, so a row of
- * magnitudes beyond 2^63 is taken for infinite. */
+ * magnitudes beyond 2^63 is taken for infinite, and without eps one below 2^-63 loses bits of its mean. */
 GGUF_DEC_API int gguf_residual_norm(const gguf_tensor* x, const gguf_tensor* residual, const gguf_tensor* gate, int act,
                                     const gguf_tensor* inner_weight, const gguf_tensor* weight, float scale, float eps,
                                     const gguf_tensor* hidden, const gguf_tensor* out, void* stream);

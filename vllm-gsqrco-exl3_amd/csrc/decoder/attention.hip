@@ -348,12 +348,15 @@ hipError_t launch_attend(const AttnArgs& a, dim3 grid, hipStream_t stream) {
 // 15.0 / 18.0, eight of 60 rows 37.9 / 40.4, of 36 rows 45.8 / 38.1.
 // A tree takes its form for many rows (attention_tree.hip) by its work, since that form's fixed costs are larger: from 33 rows of a
 // (sequence, KV head) on (65 of heads of 64), and 2^23 of rows times tokens over all of them (3 * 2^23 of heads up to 128). Calls in us,
-// few / many: head size 256, four KV heads, 96 rows of one sequence of 16000 tokens 45.2 / 56.8, of four of 4000 59.9 / 52.3, of
-// eight 74.2 / 56.1; 48 rows of four of 4000 36.6 / 43.7, of eight of 16000 129 / 102; 24 rows of eight of 16000 93.3 / 98.1, of 32 of 8000
-// 201 / 182; 384 rows of one of 2000 38.2 / 50.5. Head size 192, one KV head, 96 rows of eight of 16000 60.1 / 48.9, 192 of four of 4000
-// 28.6 / 41.8. Head size 128, eight KV heads, 128 rows of two of 8000 40.1 / 59.6, of four 67.0 / 63.0, of eight of 4000 62.4 / 64.4, of
-// 32 of 4000 303 / 126; 48 rows of eight of 16000 118 / 110, 32 rows 83.8 / 109. Head size 64, eight KV heads, 128 rows of two of 8000
-// 32.3 / 48.7, of 32 of 4000 140 / 84.3; 64 rows of 32 of 2000 43.4 / 52.6, of 16 of 16000 137 / 138.
+// few / many: head size 256, four KV heads, 96 rows of one sequence of 16000 tokens 45.8 / 48.7, of one of 32768 84.5 / 49.2, of two of
+// 16000 76.2 / 52.4, of four of 4000 61.1 / 52.4, of eight 76.7 / 50.1; 48 rows of four of 4000 36.6 / 42.7, of eight of 16000 131 / 99.6; 24 rows of
+// eight of 16000 94.0 / 94.6, of 32 of 8000 196 / 168, of 64 of 16000 709 / 597; 384 rows of one of 2000 35.5 / 38.3. Head size 192, one KV head,
+// 96 rows of eight of 16000 60.1 / 47.1, 192 of four of 4000 28.5 / 39.9. Head size 128, eight KV heads, 128 rows of two of 8000 37.7 /
+// 54.1, of four 61.3 / 51.9, of eight of 4000 55.1 / 51.6, of 32 of 4000 306 / 117; 48 rows of eight of 16000 117 / 105, 32 rows
+// 87.3 / 101. Head size 64, eight KV heads, 128 rows of two of 8000 30.9 / 46.0, of 32 of 4000 136 / 81.3; 64 rows of 32 of 2000
+// 43.0 / 50.6, of 16 of 16000 133 / 129.
+// At three of these points, of heads of 256, the rule takes the slower side: 96 rows of four sequences of 4000 (6.1 million rows times tokens),
+// and 24 rows of 32 and of 64 sequences (as 30 rows of 32 of 16000: 371 / 311).
 static bool tree_many(int d, int64_t rows, int64_t groups, int64_t max_len) {
   return rows > (d == 64 ? 64 : 32) && (double)rows * (double)groups * (double)max_len >= (d > 128 ? 1 : 3) * 8388608.0;
 }

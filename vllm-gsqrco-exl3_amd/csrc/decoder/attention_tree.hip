@@ -20,10 +20,17 @@
 // up to 128 dims slower (502 us to 419, the case above), beyond quicker (206 to 217, 21 drafts of 8 sequences of 32768 tokens, 24 query and
 // 4 KV heads of 256), where a second set of operands and rounded queries were not worth it.
 //
-// What bounds it: a step takes some 2100 to 2500 cycles, the products' 32 matrix instructions 1024 of them on a SIMD; the weights' 270 to
-// 300 vector instructions, 16 or 32 of them exponentials, with their waits for LDS and each other the rest. 16 drafts of 8 ragged sequences
-// to 32768 tokens (24 query and 4 KV heads of 256): 103 us, 47 drafts of 4 to 16000: 85, 64 drafts of 32 to 8192 (32 query and 8 KV heads
-// of 128): 222; the products alone 28, 20 and 88 at a library product's rate.
+// Weights are in fp16 as the matrix instructions take 16 bits: bf16 would leave them 8 bits for 11, and a second plane of them would double the
+// second product. Against 64 bits this takes the error of fp16 outputs from their own rounding's 2.1e-4 (relative, all of an output) to
+// 2.9e-4; bf16 outputs' stays 1.7e-3.
+//
+// What bounds it: by clock values stored by each workgroup, a step takes 2200 to 2600 cycles, the products' 32 matrix instructions 1024 of them on
+// a SIMD; the weights' 270 to 300 vector instructions, 16 or 32 of them exponentials, with their waits for LDS and each other the rest.
+// Outside the steps a piece (a share's part of one group) takes some 17500 cycles for its start, where places, K's first tiles and the
+// queries are loaded one behind the other, and 7500 for its last product and its sums: 14 of 76 us on average where a share is one
+// piece (16 drafts of 8 ragged sequences to 32768 tokens, 24 query and 4 KV heads of 256: 101 us a call), 14 of 58 (47 drafts of 4 to 16000:
+// 83), 24 of 156 at two pieces (64 drafts of 32 to 8192, 32 query and 8 KV heads of 128: 224). The products alone take 28, 20 and 88 at a
+// library product's rate.
 #include <algorithm>
 #include <type_traits>
 

@@ -15,7 +15,7 @@ constexpr int kThreads = 256;
 // a later row's source lies behind every place written before.
 //
 // Bound: latency of a few dependent loads (lengths, path, table, scales, codes); a path is some rows of some hundred bytes. 8 drafts of one
-// sequence 5.5 us, 64 drafts of 64 sequences over pages of 16 tokens 9.6.
+// sequence 5.7 us, 64 drafts of 64 sequences over pages of 16 tokens 9.8; where pages' scales have to grow 9.9.
 __global__ void __launch_bounds__(kThreads) keep_kernel(Kv8 c, const int32_t* __restrict__ path, int64_t path_stride, int m,
                                                         const int32_t* __restrict__ lens, Ragged rows) {
   __shared__ int ph[kMostKept], off[kMostKept], from[kMostKept];  // a row's (page, head), place in it, and page of the table

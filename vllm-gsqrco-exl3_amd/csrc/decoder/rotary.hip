@@ -5,7 +5,8 @@
 // dims of a piece, or that hold whole pairs. So a row's lanes need each other for the norm's sum only.
 //
 // What bounds it: a step of single tokens the chain lens -> table -> page -> codes (32 sequences, 24 + 4 heads of 256 dims in
-// bf16: 7.2 us a call in a graph, kv8_append alone 5.4); a prompt the memory (8192 tokens of 24 + 4 heads of 256: 252 MB read and
+// bf16: 7.2 us a call in a graph, kv8_append alone 5.4, where no page's scale grows; where all do and older codes are rounded again, the
+// kernel takes 9.8 us for 8.1, 16 fp16 drafts of 8 sequences 9.1 for 8.0, a prompt no longer); a prompt the memory (8192 tokens of 24 + 4 heads of 256: 252 MB read and
 // written in 71 us, 3.6 TB/s, a copy reaches 5; in a loop, where the last level of cache holds a part, in 55). Times of that loop:
 // - The two passes over a page's new values, for the scale and for the codes, run forwards and backwards, so that the last rows
 //   are at hand for the second: of a page of 64 tokens of 256 dims half of K's and all of V's are read once. Holding all of K's
@@ -101,8 +102,9 @@ __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float inv) {
 
 // The first `blocks` workgroups take the cache's (sequence, page, head)s of K and V, one at a time, so that a scale has one
 // writer; the others take the queries' rows.
-// A (page, head)'s new values are read once, into registers, for its scale and then for the codes, up to 64 tokens of 256 dims; what a
-// page holds beyond that is read twice. V's codes, whose tokens are innermost, turn in LDS.
+// A (page, head)'s new values go through registers for its scale and then for the codes: the last kThreads / kLanes of its keys (32 of 256
+// dims) and the last 64 of its values stay there, what it has beyond that is read (keys: normed and turned) again. V's codes, whose tokens
+// are innermost, turn in LDS.
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs a, int blocks, int page_blocks) {
   constexpr int L = kLanes<D>, ROWS = kThreads / L;  // rows that the workgroup takes at a time

@@ -193,8 +193,8 @@ def residual_norm(x, residual=None, weight=None, *, inner_weight=None, gate=None
                   eps: float = 1e-6):
     """Norms before and after a block with its gate and residual, over the last dimension of x [rows, n] or [rows, heads, n]:
         u = x, normed by inner_weight, times act(gate);  h = residual + scale * u;  out = h, normed by weight
-    with RMS norms (weights fp32 [n]); every part may be missing. act: "none", "sigmoid" or "silu" of a gate like x. Returns (out,
-    h): out in x's dtype (None without weight), h in residual's (x's dtype or fp32)."""
+    with RMS norms (weights fp32 [n]); every part may be missing. act: "none" (the gate itself), "sigmoid" or "silu" of a gate like x;
+    without a gate it does nothing. Returns (out, h): out in x's dtype (None without weight), h in residual's (x's dtype or fp32)."""
     if act not in _ACTS:
         raise RuntimeError(f"residual_norm: act={act!r} is not one of {', '.join(_ACTS)}")
     out, hidden = _ops.residual_norm(x, residual, gate, _ACTS[act], inner_weight, weight, scale, eps)
