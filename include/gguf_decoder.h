@@ -165,7 +165,7 @@ GGUF_DEC_API int gguf_kv8_keep(const gguf_kv8_cache* cache, const gguf_tensor* p
  * act: 0 the gate itself, 1 its sigmoid, 2 silu; without a gate it is not looked at. gate: like x (other strides); residual: x's shape, x's dtype or fp32; weights: fp32 [n].
  * hidden (h): contiguous, residual's dtype (x's without one), written by every call; out: contiguous, x's dtype, not read or written without weight. Neither
  * overlaps an input. Everything between is fp32: out comes from h before its rounding. Where hidden is not fp32, a sigmoid is
- * known to 2^-17 of itself and is 0 for gates below -88; where it is, to some steps of fp32. Squares are summed in fp32, so a row of
+ * known to 2^-17 of itself and may be 0 for gates below -87; where it is, to some steps of fp32. Squares are summed in fp32, so a row of
  * magnitudes beyond 2^63 is taken for infinite, and without eps one below 2^-63 loses bits of its mean. */
 GGUF_DEC_API int gguf_residual_norm(const gguf_tensor* x, const gguf_tensor* residual, const gguf_tensor* gate, int act,
                                     const gguf_tensor* inner_weight, const gguf_tensor* weight, float scale, float eps,
