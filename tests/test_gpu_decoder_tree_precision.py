@@ -13,7 +13,7 @@ import torch
 
 from _gpu import poison_allocator
 from test_gpu_decoder_kv8 import _cu, _i32, _random_cache, _table, _values
-from test_gpu_decoder_tree import HINTS, _bits, _random_mask
+from test_gpu_decoder_tree import HINTS, _bits, _random_mask, _run
 
 pytestmark = pytest.mark.gpu
 F16 = torch.float16
@@ -55,3 +55,10 @@ def test_roundings(dec, hq, heads, d, page, by, hint):
         allowed += (1.25 ** 2 * 2.0 ** -22 / 3 * (ref.square() + mean) + (2.0 ** -15 * size).square()).sum()
         row += n
     assert square <= allowed, (square / allowed).sqrt()
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("ends,news", [((70001,), (17,)), ((66000, 5), (12, 5)), ((30, 40000, 41000), (30, 16, 16))], ids=str)
+def test_groups_over_all_shares(dec, d, ends, news):
+    """One KV head: a group of rows cut into as many shares as there are, alone and behind or before others."""
+    _run(dec, ends, news, 3, 1, d, 64, F16, 52, max_len=1 << 24)
